@@ -7,6 +7,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 #include <math.h>
+#include <atomic>
 
 #define TIS_API extern "C" __attribute__((visibility("default")))
 
@@ -223,6 +224,17 @@ inline cudaError_t tis_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     cfg.numAttrs = tis_pdl_enabled() ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
+
+// Whether a launcher sees the current device for the first time (a kernel's attributes are set on each device).
+struct DeviceOnce {
+    std::atomic<unsigned long long> seen{0};
+    bool first() {
+        int device = 0;
+        cudaGetDevice(&device);
+        const unsigned long long bit = 1ull << (device & 63);
+        return !(seen.load(std::memory_order_relaxed) & bit) && (seen.fetch_or(bit), true);
+    }
+};
 
 // Dispatch on the storage dtype inside a launcher.
 #define TIS_DISPATCH_DTYPE(dtype, T, ...)                                   \

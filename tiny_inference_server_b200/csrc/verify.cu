@@ -1,0 +1,245 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// Request b has drafts d_0 .. d_{L-1}, the draft's distributions q_i (none: the drafts are certain, q_i one at d_i), the target's
+// p_0 .. p_L and numbers u_0 .. u_k in [0, 1).  Draft i is kept while u_i q_i(d_i) < p_i(d_i) (kept with chance min(1, p / q)).
+// Behind the first draft that is not, the next token is drawn from max(p_i - q_i, 0), or from p_i where that has no mass; behind L
+// kept ones from p_L.  The draw is by inverse CDF in index order: the lowest token whose running sum exceeds u_k times the whole.
+// What is not a positive number (zero, negative, infinite, NaN) has no mass.
+//
+// Products, differences and sums are in 64 bits: a product of two floats is then exact, a sum of a vocabulary's floats is off by
+// some 1e-15 of itself, and a token does not depend on how the row is shared out.  (In 32 bits the sum of 131072 entries is off by
+// more than many a token's mass.)
+//
+// Only one row of p, and behind a rejection one of q, is read: the kernel is bound by those bytes, and for few requests by the
+// chain draft -> its probabilities -> row -> sum -> place.  Every warp works out for itself which row it is (a lane a draft: no
+// barrier), so the chain has one exchange: a cluster of up to 16 CTAs shares the row, a warp takes a contiguous run of it, and the
+// runs' sums go to every CTA of the cluster.  All CTAs then know whose run holds the number; that warp reads its run again, from its SM's L1.
+#include "cluster_reduce.cuh"
+
+namespace {
+
+constexpr int VERIFY_THREADS = 512;
+constexpr int VERIFY_WARPS = VERIFY_THREADS / 32;
+constexpr int VERIFY_MAX_CLUSTER = 16;
+constexpr int VERIFY_MAX_DRAFTS = 31;       // a lane a draft, one more for the token behind them
+constexpr unsigned ALL = 0xffffffffu;
+
+struct VerifyParams {
+    const float* p; long long p_request, p_row;
+    const float* q; long long q_request, q_row;     // null: drafts without a distribution
+    const int* drafts; const float* u; const int* lens;
+    int* tokens; int* accepted;
+    int k, V;
+};
+
+__device__ __forceinline__ double mass(float x) { return x > 0.f && x < INFINITY ? (double)x : 0.0; }
+
+// What is left of a row: entries of p less those of q.
+struct Row {
+    const float* p; const float* q;         // q null: nothing is taken away but the entry `without`
+    int without;
+    int V;
+    bool wide;                              // rows that start on 16 bytes
+    // entries i .. i + 3 (beyond the row: no mass)
+    __device__ __forceinline__ void four(int i, double (&r)[4]) const {
+        float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (wide && i + 3 < V) {
+            const float4 x = *reinterpret_cast<const float4*>(p + i);
+            a[0] = x.x; a[1] = x.y; a[2] = x.z; a[3] = x.w;
+            if (q != nullptr) {
+                const float4 y = *reinterpret_cast<const float4*>(q + i);
+                b[0] = y.x; b[1] = y.y; b[2] = y.z; b[3] = y.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (i + e < V) {
+                    a[e] = p[i + e];
+                    if (q != nullptr) b[e] = q[i + e];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = i + e == without ? 0.0 : fmax(mass(a[e]) - mass(b[e]), 0.0);
+    }
+};
+
+__device__ __forceinline__ double warp_total(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(ALL, v, o);
+    return v;
+}
+__device__ __forceinline__ double warp_running(double v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double w = __shfl_up_sync(ALL, v, o);
+        if (lane >= o) v += w;
+    }
+    return v;
+}
+__device__ __forceinline__ void store_to_rank(double* local, unsigned rank, double v) {
+    asm volatile("st.shared::cluster.f64 [%0], %1;\n"
+                 ::"r"(cluster_reduce::map_to_rank(cluster_reduce::shared_addr(local), rank)), "d"(v) : "memory");
+}
+
+// `run`: entries of a warp's run, a multiple of 128; rank r of the cluster has runs 16 r .. 16 r + 15.
+__global__ void __launch_bounds__(VERIFY_THREADS)
+verify_kernel(const VerifyParams v, int run) {
+    __shared__ double run_sum[2][VERIFY_WARPS];
+    __shared__ double rank_sum[2][VERIFY_MAX_CLUSTER];     // written by every rank; one set for each of the two passes
+    pdl_launch_dependents();
+    unsigned ranks, rank;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(ranks));
+    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
+    cluster_reduce::cluster_arrive();                       // waited for before the first store to another CTA
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const size_t b = blockIdx.x / ranks;
+    pdl_wait();
+
+    // ---- which drafts are kept: a lane a draft, every warp for itself ----
+    const int L = v.lens != nullptr ? min(max(v.lens[b], 0), v.k) : v.k;
+    const int draft = lane < v.k ? v.drafts[b * v.k + lane] : -1;
+    const bool real = draft >= 0 && draft < v.V;
+    const double u_last = (double)v.u[b * (v.k + 1) + v.k];
+    bool keep = false;
+    if (lane < L && real) {
+        const double p = mass(v.p[(long long)b * v.p_request + lane * v.p_row + draft]);
+        const double q = v.q != nullptr ? mass(v.q[(long long)b * v.q_request + lane * v.q_row + draft]) : 1.0;
+        keep = (double)v.u[b * (v.k + 1) + lane] * q < p;
+    }
+    const int kept = __ffs(~__ballot_sync(ALL, keep)) - 1;  // (at most 31 lanes keep one)
+    const int refused = __shfl_sync(ALL, draft, kept);      // the draft at that place, if there is one
+
+    Row row;
+    row.p = v.p + (long long)b * v.p_request + kept * v.p_row;
+    row.q = kept < L && v.q != nullptr ? v.q + (long long)b * v.q_request + kept * v.q_row : nullptr;
+    row.without = kept < L && v.q == nullptr ? refused : -1;
+    row.V = v.V;
+    const int first = ((int)rank * VERIFY_WARPS + warp) * run, end = min(first + run, v.V);
+    int token = -1;
+    bool mine = false;
+    for (int pass = 0; pass < 2; ++pass) {
+        row.wide = ((reinterpret_cast<uintptr_t>(row.p) | reinterpret_cast<uintptr_t>(row.q)) & 15) == 0;
+        // ---- sums of the runs, of the CTAs, of the row ----
+        double sum = 0.0;
+#pragma unroll 4
+        for (int i = first + lane * 4; i < end; i += 128) {
+            double r[4];
+            row.four(i, r);
+            sum += (r[0] + r[1]) + (r[2] + r[3]);
+        }
+        sum = warp_total(sum);
+        if (lane == 0) run_sum[pass][warp] = sum;
+        __syncthreads();
+        // (the runs' sums added one after another, the same bits in every lane and warp)
+        double cta = 0.0;
+#pragma unroll
+        for (int w = 0; w < VERIFY_WARPS; ++w) cta += run_sum[pass][w];
+        if (pass == 0) cluster_reduce::cluster_wait();      // every CTA of the cluster has started
+        if (warp == 0 && lane < (int)ranks) store_to_rank(&rank_sum[pass][rank], (unsigned)lane, cta);
+        __syncwarp();
+        cluster_reduce::cluster_arrive();
+        cluster_reduce::cluster_wait();
+        double total = 0.0;
+        for (unsigned r = 0; r < ranks; ++r) total += rank_sum[pass][r];
+        if (total > 0.0) {
+            // ---- whose run holds the number: the first rank, run, lane whose running sum exceeds it (the last with mass where
+            // rounding left it beyond all of them) ----
+            const double target = u_last * total;
+            double before = 0.0, running = 0.0;
+            int owner = -1;
+            for (unsigned r = 0; r < ranks; ++r) {
+                const double s = rank_sum[pass][r];
+                if (s > 0.0) { owner = (int)r; before = running; }
+                running += s;
+                if (s > 0.0 && running > target) break;
+            }
+            if (owner != (int)rank) break;
+            running = before;
+            owner = -1;
+            for (int w = 0; w < VERIFY_WARPS; ++w) {
+                const double s = run_sum[pass][w];
+                if (s > 0.0) { owner = w; before = running; }
+                running += s;
+                if (s > 0.0 && running > target) break;
+            }
+            if (owner != warp) break;
+            running = before;
+            for (int i = first; i < end; i += 128) {        // (uniform in the warp)
+                double r[4];
+                row.four(i + lane * 4, r);                  // (beyond the run's end: the row's end too, no mass)
+                const double s = (r[0] + r[1]) + (r[2] + r[3]);
+                const double upto = warp_running(s, lane);
+                const unsigned has = __ballot_sync(ALL, s > 0.0);
+                const unsigned over = __ballot_sync(ALL, s > 0.0 && running + upto > target);
+                if (has != 0) {
+                    const int at = over != 0 ? __ffs(over) - 1 : 31 - __clz(has);
+                    double c = running + (upto - s);
+                    int found = -1;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool passed = found >= 0 && c > target;
+                        c += r[e];
+                        if (!passed && r[e] > 0.0) found = i + lane * 4 + e;
+                    }
+                    token = __shfl_sync(ALL, found, at);    // (of the last piece with mass, if none exceeds the number)
+                }
+                if (over != 0) break;
+                running += __shfl_sync(ALL, upto, 31);
+            }
+            mine = true;
+            break;
+        }
+        if (pass == 1 || (row.q == nullptr && row.without < 0)) {      // no mass anywhere: no token
+            mine = rank == 0 && warp == 0;
+            break;
+        }
+        row.q = nullptr;                                    // nothing is left of p - q: p itself
+        row.without = -1;
+    }
+    if (mine) {
+        if (lane <= v.k) v.tokens[b * (v.k + 1) + lane] = lane < kept ? draft : (lane == kept ? token : -1);
+        if (lane == 0) v.accepted[b] = kept;
+    }
+}
+
+}  // namespace
+
+// n requests of up to k drafts over V tokens.  p: rows p + b p_request + i p_row (i <= k) of V floats; q likewise (i < k; null: none);
+// drafts [n][k], u [n][k + 1], lens [n] (null: k each); tokens [n][k + 1]: the kept drafts, the drawn token (-1: no mass), -1 behind.
+TIS_API int tis_verify_drafts(const float* p, long long p_request, long long p_row, const float* q, long long q_request,
+                              long long q_row, const int* drafts, const float* u, const int* lens, int* tokens, int* accepted,
+                              int n, int k, int V, cudaStream_t stream) {
+    if (n <= 0) return TIS_OK;
+    if (k < 0 || k > VERIFY_MAX_DRAFTS || V <= 0 || V > (1 << 30)) {
+        tis_set_error("verify_drafts: %d drafts, vocabulary of %d", k, V);
+        return TIS_BAD_SIZE;
+    }
+    int ranks = VERIFY_MAX_CLUSTER;
+    while (ranks > 1 && ((long long)n * ranks > 4 * 148 || V <= (ranks / 2) * VERIFY_THREADS * 4)) ranks >>= 1;
+    if ((long long)n * ranks > 0x7fffffffLL) {
+        tis_set_error("verify_drafts: %d requests", n);
+        return TIS_BAD_SIZE;
+    }
+    static DeviceOnce configured;
+    if (configured.first() && cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return tis_check_launch("verify_drafts (cluster size)");
+    const int runs = ranks * VERIFY_WARPS;
+    const int run = ((V + runs - 1) / runs + 127) / 128 * 128;
+    VerifyParams v{p, p_request, p_row, q, q_request, q_row, drafts, u, lens, tokens, accepted, k, V};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n * ranks));
+    cfg.blockDim = dim3(VERIFY_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = (unsigned)ranks;
+    attrs[0].val.clusterDim.y = 1;
+    attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = tis_pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, verify_kernel, v, run);
+    return tis_check_launch("verify_drafts");
+}

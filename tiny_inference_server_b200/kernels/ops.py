@@ -19,7 +19,7 @@ import torch
 from . import build as _build
 
 _lib = None
-ABI_VERSION = 17
+ABI_VERSION = 18
 #: launches of this library's kernels so far (library matrix products are not counted)
 launches = 0
 #: calls by kind, for tests that must know which kernel a product or an attention went to
@@ -29,6 +29,11 @@ calls: "collections.Counter[str]" = collections.Counter()
 
 class KernelError(RuntimeError):
     pass
+
+
+#: argument kinds of launchers whose pointers are passed as plain numbers: p a pointer, i an int, l a 64-bit int, f a float
+_ARGUMENTS = {"tis_verify_drafts": "pllpllpppppiiip"}
+_KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 
 
 def library():
@@ -47,6 +52,8 @@ def library():
     lib.tis_last_error.restype = ctypes.c_char_p
     lib.tis_abi_version.restype = ctypes.c_int
     lib.tis_chunked_recurrence_floats.restype = ctypes.c_size_t
+    for name, kinds in _ARGUMENTS.items():
+        getattr(lib, name).argtypes = [_KINDS[c] for c in kinds]
     if lib.tis_abi_version() != ABI_VERSION:
         raise KernelError(f"{path}: launcher interface {lib.tis_abi_version()}, expected {ABI_VERSION}")
     _lib = lib
@@ -91,6 +98,19 @@ def _stream():
 
 def _f(x: float):
     return ctypes.c_float(x)
+
+
+def _on_this_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """A launch goes to the current device: raise for a tensor that lies elsewhere."""
+    device = -1
+    for t in tensors:
+        if t is not None:
+            if not t.is_cuda:
+                raise KernelError(f"{what}: a tensor on {t.device}; the kernels take CUDA tensors")
+            if device < 0:
+                device = _current_device()
+            if t.get_device() != device:
+                raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{device}")
 
 
 # ---------------------------------------------------------------------------------------
@@ -1850,6 +1870,65 @@ def sample_rows(logits: torch.Tensor, temps: torch.Tensor, top_ks: torch.Tensor,
                                _p(seen_bitmap), words, _p(seeds), _p(counters), _p(out_tokens), _p(probs_out),
                                _stream()), lib)
     return out_tokens
+
+
+#: most drafts of a request (csrc/verify.cu has a lane for each and one for the token behind them)
+VERIFY_MAX_DRAFTS = 31
+
+
+def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor], drafts: torch.Tensor, uniforms: torch.Tensor,
+                  draft_lens: Optional[torch.Tensor] = None, tokens: Optional[torch.Tensor] = None,
+                  accepted: Optional[torch.Tensor] = None):
+    """Which drafted tokens of n requests are kept, and the token drawn behind them: (``tokens`` (n, k + 1), ``accepted`` (n,)),
+    int32.  A row of ``tokens`` is the ``accepted`` first drafts, the drawn token, then -1.
+
+    ``target_probs`` (n, k + 1, V) float32: the target's probabilities at every draft's place and behind the last, as
+    ``sample_rows`` leaves them in ``probs_out``; ``draft_probs`` (n, k, V): those that the drafts were drawn from (None: drafts
+    without a distribution, as by arg-max).  Rows of both may have any stride.  ``drafts`` (n, k) int32; ``uniforms`` (n, k + 1) float32
+    in [0, 1); ``draft_lens`` (n,) int32: how many of its k drafts a request has (None: all; it is held between 0 and k).
+
+    Draft i is kept while ``uniforms[i] * q_i(d_i) < p_i(d_i)``.  The token behind is the lowest whose running sum exceeds
+    ``uniforms[k]`` times the whole sum, over ``max(p_i - q_i, 0)`` at the first draft that is not kept (``p_i`` where
+    nothing is left of the difference; without a distribution ``q_i`` is one at the draft) and over the target's row behind the last
+    draft.  Entries that are not positive numbers have no mass; a row without mass gives the token -1.  A draft outside the
+    vocabulary is not kept.  Computed in 64 bits: the tokens do not depend on how the work is shared out."""
+    n, k1, v = target_probs.shape
+    k = k1 - 1
+    f32, i32 = torch.float32, torch.int32
+    if target_probs.dtype != f32 or uniforms.dtype != f32 or drafts.dtype != i32 or k1 < 1 or v < 1 or k > VERIFY_MAX_DRAFTS:
+        raise KernelError(f"verify_drafts: float32 probabilities and numbers, int32 drafts, up to {VERIFY_MAX_DRAFTS} drafts, not "
+                          f"{target_probs.dtype} {tuple(target_probs.shape)}, {uniforms.dtype}, {drafts.dtype}")
+    if drafts.shape != (n, k) or uniforms.shape != (n, k1) or (draft_lens is not None and draft_lens.shape != (n,)):
+        raise KernelError(f"verify_drafts: drafts {tuple(drafts.shape)}, numbers {tuple(uniforms.shape)} for probabilities "
+                          f"{tuple(target_probs.shape)}")
+    if target_probs.stride(2) != 1 and v > 1:
+        raise KernelError("verify_drafts: a row of probabilities is contiguous")
+    if draft_probs is not None and (draft_probs.dtype != f32 or draft_probs.shape != (n, k, v) or (draft_probs.stride(2) != 1 and v > 1)):
+        raise KernelError(f"verify_drafts: draft probabilities {draft_probs.dtype} {tuple(draft_probs.shape)} for {tuple(target_probs.shape)}")
+    device = target_probs.device
+    if tokens is None:
+        tokens = torch.empty((n, k1), dtype=i32, device=device)
+    if accepted is None:
+        accepted = torch.empty(n, dtype=i32, device=device)
+    if tokens.shape != (n, k1) or accepted.shape != (n,) or tokens.dtype != i32 or accepted.dtype != i32:
+        raise KernelError(f"verify_drafts: results {tuple(tokens.shape)} {tokens.dtype}, {tuple(accepted.shape)} {accepted.dtype}")
+    if not (drafts.is_contiguous() and uniforms.is_contiguous() and tokens.is_contiguous() and accepted.is_contiguous()):
+        raise KernelError("verify_drafts: drafts, numbers and results are contiguous")
+    if draft_lens is not None and (draft_lens.dtype != i32 or not draft_lens.is_contiguous()):
+        raise KernelError("verify_drafts: numbers of drafts are contiguous int32")
+    _on_this_device("verify_drafts", target_probs, draft_probs, drafts, uniforms, draft_lens, tokens, accepted)
+    if n == 0:
+        return tokens, accepted
+    lib = library()
+    if draft_probs is not None and k:
+        q, q_request, q_row = draft_probs.data_ptr(), draft_probs.stride(0), draft_probs.stride(1)
+    else:
+        q, q_request, q_row = None, 0, 0
+    calls["verify_drafts"] += 1
+    _check(lib.tis_verify_drafts(target_probs.data_ptr(), target_probs.stride(0), target_probs.stride(1), q, q_request, q_row,
+                                 drafts.data_ptr(), uniforms.data_ptr(), draft_lens.data_ptr() if draft_lens is not None else None,
+                                 tokens.data_ptr(), accepted.data_ptr(), n, k, v, _stream()), lib)
+    return tokens, accepted
 
 
 def sample_stage_limit(entries: int) -> None:
