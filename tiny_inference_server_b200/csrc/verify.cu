@@ -13,7 +13,10 @@
 // Only one row of p, and behind a rejection one of q, is read: the kernel is bound by those bytes, and for few requests by the
 // chain draft -> its probabilities -> row -> sum -> place.  Every warp works out for itself which row it is (a lane a draft: no
 // barrier), so the chain has one exchange: a cluster of up to 16 CTAs shares the row, a warp takes a contiguous run of it, and the
-// runs' sums go to every CTA of the cluster.  All CTAs then know whose run holds the number; that warp reads its run again, from its SM's L1.
+// runs' sums go to every CTA of the cluster.  All CTAs then know whose run holds the number; that warp goes through the sums of its
+// run's steps and reads one step again.  Measured: 64 requests of 131072 tokens, behind a rejection each (67 MB) 20 us, of it 10 at
+// the rate of memory (64-bit sums of every entry: 37 us, the conversions; a search entry by entry of the whole run: 6 us more);
+// one request of 32000 tokens 5.3 us.
 #include "cluster_reduce.cuh"
 
 namespace {
@@ -21,6 +24,7 @@ namespace {
 constexpr int VERIFY_THREADS = 512;
 constexpr int VERIFY_WARPS = VERIFY_THREADS / 32;
 constexpr int VERIFY_MAX_CLUSTER = 16;
+constexpr int VERIFY_STEPS = 32;            // sums of a run that are kept, to find the place of the number in it
 constexpr int VERIFY_MAX_DRAFTS = 31;       // a lane a draft, one more for the token behind them
 constexpr unsigned ALL = 0xffffffffu;
 
@@ -32,7 +36,8 @@ struct VerifyParams {
     int k, V;
 };
 
-__device__ __forceinline__ double mass(float x) { return x > 0.f && x < INFINITY ? (double)x : 0.0; }
+__device__ __forceinline__ float positive(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
+__device__ __forceinline__ double mass(float x) { return (double)positive(x); }
 
 // What is left of a row: entries of p less those of q.
 struct Row {
@@ -40,27 +45,74 @@ struct Row {
     int without;
     int V;
     bool wide;                              // rows that start on 16 bytes
-    // entries i .. i + 3 (beyond the row: no mass)
-    __device__ __forceinline__ void four(int i, double (&r)[4]) const {
-        float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-        if (wide && i + 3 < V) {
-            const float4 x = *reinterpret_cast<const float4*>(p + i);
-            a[0] = x.x; a[1] = x.y; a[2] = x.z; a[3] = x.w;
-            if (q != nullptr) {
-                const float4 y = *reinterpret_cast<const float4*>(q + i);
-                b[0] = y.x; b[1] = y.y; b[2] = y.z; b[3] = y.w;
-            }
-        } else {
+    // entries i .. i + 3 as they are (beyond the row: zero)
+    __device__ __forceinline__ float4 four(const float* x, int i) const {
+        if (wide && i + 3 < V) return *reinterpret_cast<const float4*>(x + i);
+        const int last = V - 1;             // (read again rather than skipped: loads that nothing decides about go out together)
+        float4 r = make_float4(x[min(i, last)], x[min(i + 1, last)], x[min(i + 2, last)], x[min(i + 3, last)]);
+        if (i + 3 > last) {
+            if (i > last) r.x = 0.f;
+            if (i + 1 > last) r.y = 0.f;
+            if (i + 2 > last) r.z = 0.f;
+            r.w = 0.f;
+        }
+        return r;
+    }
+    // what is left of entries i .. i + 3, in 64 bits
+    __device__ __forceinline__ void piece(const float4& a, const float4& b, int i, double (&r)[4]) const {
+        const float x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = i + e == without ? 0.0 : fmax(mass(x[e]) - mass(y[e]), 0.0);
+    }
+    template <int N> __device__ __forceinline__ void load(int i, float4 (&a)[N], float4 (&b)[N]) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) a[n] = four(p, i + n * 128);
+#pragma unroll
+        for (int n = 0; n < N; ++n) b[n] = q != nullptr ? four(q, i + n * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    // What is left of N pieces of four entries, 128 apart, added up.  A conversion to 64 bits costs as much as a dozen 32-bit
+    // sums, so a difference and a sum are kept as two floats each, the rounded result and what the rounding lost (Dekker 1971,
+    // Knuth's two-sum), and converted once: off by some 2^-46 of itself.
+    template <int N, bool Q> __device__ __forceinline__ double sum(int i) const {
+        float4 a[N], b[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) a[n] = four(p, i + n * 128);
+        if (Q) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) b[n] = four(q, i + n * 128);
+        }
+        float s = 0.f, lost = 0.f, top = 0.f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const float x[4] = {a[n].x, a[n].y, a[n].z, a[n].w};
+            const float y[4] = {Q ? b[n].x : 0.f, Q ? b[n].y : 0.f, Q ? b[n].z : 0.f, Q ? b[n].w : 0.f};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (i + e < V) {
-                    a[e] = p[i + e];
-                    if (q != nullptr) b[e] = q[i + e];
+                float d = fmaxf(x[e], 0.f), d_lost = 0.f;       // (a NaN and what is negative: no mass)
+                if (Q) {
+                    const float q1 = fmaxf(y[e], 0.f), both = fminf(d, q1), left = d - both;
+                    top = fmaxf(top, q1);
+                    d_lost = (d - left) - both;
+                    d = left;
+                } else if (i + n * 128 + e == without) {
+                    d = 0.f;
                 }
+                const float t = s + d, v = t - s;
+                lost += (s - (t - v)) + (d - v);
+                if (Q) lost += d_lost;
+                s = t;
             }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = i + e == without ? 0.0 : fmax(mass(a[e]) - mass(b[e]), 0.0);
+        top = fmaxf(top, s);
+        if (top < INFINITY) return (double)s + (double)lost;
+        double exact = 0.0;                                     // an infinity has no mass either
+#pragma unroll 1
+        for (int n = 0; n < N; ++n) {
+            double r[4];
+            piece(four(p, i + n * 128), q != nullptr ? four(q, i + n * 128) : make_float4(0.f, 0.f, 0.f, 0.f), i + n * 128, r);
+            exact += (r[0] + r[1]) + (r[2] + r[3]);
+        }
+        return exact;
     }
 };
 
@@ -82,9 +134,11 @@ __device__ __forceinline__ void store_to_rank(double* local, unsigned rank, doub
                  ::"r"(cluster_reduce::map_to_rank(cluster_reduce::shared_addr(local), rank)), "d"(v) : "memory");
 }
 
-// `run`: entries of a warp's run, a multiple of 128; rank r of the cluster has runs 16 r .. 16 r + 15.
-__global__ void __launch_bounds__(VERIFY_THREADS)
-verify_kernel(const VerifyParams v, int run) {
+// A warp's run is `steps` steps of `strides` times 128 N entries; rank r of the cluster has runs 16 r .. 16 r + 15.
+template <int N>
+__global__ void __launch_bounds__(VERIFY_THREADS, 2)
+verify_kernel(const VerifyParams v, int steps, int strides) {
+    __shared__ double step_sum[VERIFY_WARPS][VERIFY_STEPS];
     __shared__ double run_sum[2][VERIFY_WARPS];
     __shared__ double rank_sum[2][VERIFY_MAX_CLUSTER];     // written by every rank; one set for each of the two passes
     pdl_launch_dependents();
@@ -115,20 +169,26 @@ verify_kernel(const VerifyParams v, int run) {
     row.q = kept < L && v.q != nullptr ? v.q + (long long)b * v.q_request + kept * v.q_row : nullptr;
     row.without = kept < L && v.q == nullptr ? refused : -1;
     row.V = v.V;
-    const int first = ((int)rank * VERIFY_WARPS + warp) * run, end = min(first + run, v.V);
+    const int stride = 128 * N, step = strides * stride;
+    const int first = ((int)rank * VERIFY_WARPS + warp) * steps * step;
     int token = -1;
     bool mine = false;
     for (int pass = 0; pass < 2; ++pass) {
         row.wide = ((reinterpret_cast<uintptr_t>(row.p) | reinterpret_cast<uintptr_t>(row.q)) & 15) == 0;
         // ---- sums of the runs, of the CTAs, of the row ----
         double sum = 0.0;
-#pragma unroll 4
-        for (int i = first + lane * 4; i < end; i += 128) {
-            double r[4];
-            row.four(i, r);
-            sum += (r[0] + r[1]) + (r[2] + r[3]);
+        for (int j = 0; j < steps && first + j * step < v.V; ++j) {
+            const int from = first + j * step, to = min(from + step, v.V);
+            double s = 0.0;
+            if (row.q != nullptr) {
+                for (int i = from; i < to; i += stride) s += row.sum<N, true>(i + lane * 4);
+            } else {
+                for (int i = from; i < to; i += stride) s += row.sum<N, false>(i + lane * 4);
+            }
+            s = warp_total(s);
+            if (lane == 0) step_sum[warp][j] = s;
+            sum += s;
         }
-        sum = warp_total(sum);
         if (lane == 0) run_sum[pass][warp] = sum;
         __syncthreads();
         // (the runs' sums added one after another, the same bits in every lane and warp)
@@ -164,28 +224,49 @@ verify_kernel(const VerifyParams v, int run) {
                 if (s > 0.0 && running > target) break;
             }
             if (owner != warp) break;
+            __syncwarp();
             running = before;
-            for (int i = first; i < end; i += 128) {        // (uniform in the warp)
-                double r[4];
-                row.four(i + lane * 4, r);                  // (beyond the run's end: the row's end too, no mass)
-                const double s = (r[0] + r[1]) + (r[2] + r[3]);
-                const double upto = warp_running(s, lane);
-                const unsigned has = __ballot_sync(ALL, s > 0.0);
-                const unsigned over = __ballot_sync(ALL, s > 0.0 && running + upto > target);
-                if (has != 0) {
-                    const int at = over != 0 ? __ffs(over) - 1 : 31 - __clz(has);
-                    double c = running + (upto - s);
-                    int found = -1;
+            int place = -1;
+            for (int j = 0; j < steps && first + j * step < v.V; ++j) {
+                const double s = step_sum[warp][j];
+                if (s > 0.0) { place = j; before = running; }
+                running += s;
+                if (s > 0.0 && running > target) break;
+            }
+            running = before;
+            const int from = first + place * step, to = min(from + step, v.V);
+            bool found = false;
+            for (int i = from; i < to && !found; i += stride) {
+                float4 a[N], b[N];
+                row.load<N>(i + lane * 4, a, b);
+                double s[N], upto[N], r[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const bool passed = found >= 0 && c > target;
-                        c += r[e];
-                        if (!passed && r[e] > 0.0) found = i + lane * 4 + e;
-                    }
-                    token = __shfl_sync(ALL, found, at);    // (of the last piece with mass, if none exceeds the number)
+                for (int n = 0; n < N; ++n) {
+                    row.piece(a[n], b[n], i + lane * 4 + n * 128, r);
+                    s[n] = (r[0] + r[1]) + (r[2] + r[3]);
+                    upto[n] = warp_running(s[n], lane);
                 }
-                if (over != 0) break;
-                running += __shfl_sync(ALL, upto, 31);
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    if (found) continue;
+                    const unsigned has = __ballot_sync(ALL, s[n] > 0.0);
+                    const unsigned over = __ballot_sync(ALL, s[n] > 0.0 && running + upto[n] > target);
+                    if (has != 0) {
+                        row.piece(a[n], b[n], i + lane * 4 + n * 128, r);
+                        double c = running + (upto[n] - s[n]);
+                        int entry = -1;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool passed = entry >= 0 && c > target;
+                            c += r[e];
+                            if (!passed && r[e] > 0.0) entry = i + lane * 4 + n * 128 + e;
+                        }
+                        // (of the last piece with mass, if none exceeds the number)
+                        token = __shfl_sync(ALL, entry, over != 0 ? __ffs(over) - 1 : 31 - __clz(has));
+                    }
+                    found = over != 0;
+                    running += __shfl_sync(ALL, upto[n], 31);
+                }
             }
             mine = true;
             break;
@@ -203,6 +284,16 @@ verify_kernel(const VerifyParams v, int run) {
     }
 }
 
+template <int N> int verify_launch(const cudaLaunchConfig_t& cfg, const VerifyParams& v, long long run) {
+    static DeviceOnce configured;
+    if (configured.first() && cudaFuncSetAttribute(verify_kernel<N>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return tis_check_launch("verify_drafts (cluster size)");
+    const long long strides = (run + 128 * N * VERIFY_STEPS - 1) / (128 * N * VERIFY_STEPS);
+    const long long steps = (run + 128 * N * strides - 1) / (128 * N * strides);
+    cudaLaunchKernelEx(&cfg, verify_kernel<N>, v, (int)steps, (int)strides);
+    return tis_check_launch("verify_drafts");
+}
+
 }  // namespace
 
 // n requests of up to k drafts over V tokens.  p: rows p + b p_request + i p_row (i <= k) of V floats; q likewise (i < k; null: none);
@@ -215,17 +306,16 @@ TIS_API int tis_verify_drafts(const float* p, long long p_request, long long p_r
         tis_set_error("verify_drafts: %d drafts, vocabulary of %d", k, V);
         return TIS_BAD_SIZE;
     }
+    // CTAs a request: as many as are all resident (two to an SM) and have four entries a thread.  us at 1, 2, 4, 8, 16 a request: 64
+    // requests of 131072 tokens -, 28.5, 20.1, 27.1, 37.3 (a second round of CTAs goes through the whole chain); one request of 32000 -,
+    // 9.3, 8.0, 5.9, 5.3.  A thread's loads ahead (1, 2, 4 pieces): as many as its run has.
     int ranks = VERIFY_MAX_CLUSTER;
-    while (ranks > 1 && ((long long)n * ranks > 4 * 148 || V <= (ranks / 2) * VERIFY_THREADS * 4)) ranks >>= 1;
+    while (ranks > 1 && ((long long)n * ranks > 2 * 148 || V <= (ranks / 2) * VERIFY_THREADS * 4)) ranks >>= 1;
     if ((long long)n * ranks > 0x7fffffffLL) {
         tis_set_error("verify_drafts: %d requests", n);
         return TIS_BAD_SIZE;
     }
-    static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        return tis_check_launch("verify_drafts (cluster size)");
-    const int runs = ranks * VERIFY_WARPS;
-    const int run = ((V + runs - 1) / runs + 127) / 128 * 128;
+    const long long runs = (long long)ranks * VERIFY_WARPS, run = (V + runs - 1) / runs;
     VerifyParams v{p, p_request, p_row, q, q_request, q_row, drafts, u, lens, tokens, accepted, k, V};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n * ranks));
@@ -240,6 +330,7 @@ TIS_API int tis_verify_drafts(const float* p, long long p_request, long long p_r
     attrs[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attrs;
     cfg.numAttrs = tis_pdl_enabled() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, verify_kernel, v, run);
-    return tis_check_launch("verify_drafts");
+    if (run <= 128) return verify_launch<1>(cfg, v, run);
+    if (run <= 256) return verify_launch<2>(cfg, v, run);
+    return verify_launch<4>(cfg, v, run);
 }
