@@ -1,0 +1,326 @@
+// Products of few rows with weights of four bits: out[r][n] = sum over k of x[r][k] (code[k][n] - zero[k / group][n]) scale[k / group][n].
+//
+// Bound by the weights' bytes: half a byte a weight, and two or three a group for its scale and zero point.  Every weight is read
+// once, by a 16-byte load of a lane straight into registers, several of them under way at a time; a lane's 16 bytes are its parts
+// of four 16 x 16 operands of mma.sync (16 columns of the matrix as the operand's rows, the rows of x as its narrow side), laid out so
+// beforehand (weights/w4.py has the layout).  A shift, a mask and a difference make two of them bfloat16 numbers: 0x4300 | code is 128 + code,
+// exactly, and so is (128 + code) - (128 + zero).  So the products are of whole numbers up to 15, exact in 32 bits, and a group's sum is
+// multiplied by its scale once, in 32 bits: weights are never rounded.
+//
+// x in float32 goes through the same products as three bfloat16 numbers each, cut off and not rounded: 8 + 8 + 8 bits hold all 24
+// of a float, so nothing is lost there either.
+//
+// A CTA of eight warps takes a few strips of 16 columns; its warps share them out (`ws` of them side by side) and the chunks of
+// 64 entries of the sum (`wk` of them take turns), and add up in shared memory, in a fixed order.  x waits in shared memory, whole or in
+// stages; its rows lie 64 bytes off a multiple of 128 apart, so that the eight rows x four pieces of 16 bytes that a warp reads at a time
+// are free of bank conflicts.
+#include "common.cuh"
+
+namespace {
+
+constexpr int W4_THREADS = 256, W4_WARPS = 8;
+constexpr int W4_STRIP = 16, W4_CHUNK = 64;
+constexpr int W4_PAD = 32;                  // elements behind a staged row
+constexpr int W4_ROWS = 64;                 // rows of a slab in bfloat16
+constexpr int W4_ROWS_F32 = 21;             // and in float32, three numbers each
+
+struct W4Params {
+    const uint4* words; const unsigned* scales; const unsigned short* zeros;
+    const void* x; long long ldx;
+    void* out; long long ldo;
+    int rows, slab, K, N, chunks, strips, groups, group_shift;      // group_shift: log2 of the halves of a chunk in a group
+    int ws, wk, stage_chunks, stages;
+    bool f32, vectors;
+};
+
+__device__ __forceinline__ uint4 load_stream(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two codes (bits 0-3 and 16-19 of w) less their zero point; `base` is 128 + zero in both halves
+__device__ __forceinline__ unsigned weight_pair(unsigned w, unsigned base) {
+    const unsigned v = (w & 0x000f000fu) | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&base));
+    return *reinterpret_cast<const unsigned*>(&d);
+}
+__device__ __forceinline__ float low_half(unsigned v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float high_half(unsigned v) { return __uint_as_float(v & 0xffff0000u); }
+
+// one float as three bfloat16 numbers that add up to it
+__device__ __forceinline__ void three(float x, unsigned short (&v)[3]) {
+    const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    const float rest = fabsf(x) < INFINITY ? x - hi : 0.f;
+    const float mid = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+    v[0] = x != x ? 0x7fc0 : (unsigned short)(__float_as_uint(hi) >> 16);
+    v[1] = (unsigned short)(__float_as_uint(mid) >> 16);
+    v[2] = (unsigned short)(__float_as_uint(rest - mid) >> 16);
+}
+
+// Entries [k0, k0 + count) of the slab's rows of x into shared memory, zero beyond K.  In float32 the rows stand three times, the
+// high parts, the middle ones, the low ones.
+__device__ __forceinline__ void stage_rows(const W4Params& p, bf16* to, int stride, int row0, int rows, int k0, int count) {
+    const int pieces = count / 8;
+    for (int i = threadIdx.x; i < rows * pieces; i += W4_THREADS) {
+        const int r = i / pieces, k = k0 + (i - r * pieces) * 8;
+        bf16* dst = to + (size_t)r * stride + (k - k0);
+        if (!p.f32) {
+            const bf16* src = static_cast<const bf16*>(p.x) + (long long)(row0 + r) * p.ldx + k;
+            if (p.vectors) {
+                const int bytes = k < p.K ? 16 : 0;         // (whole pieces: K is a multiple of 8 here)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
+                             ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(bytes ? src : static_cast<const bf16*>(p.x)), "r"(bytes) : "memory");
+            } else {
+                unsigned short v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = k + e < p.K ? reinterpret_cast<const unsigned short*>(src)[e] : (unsigned short)0;
+                *reinterpret_cast<uint4*>(dst) = make_uint4(v[0] | (unsigned)v[1] << 16, v[2] | (unsigned)v[3] << 16,
+                                                            v[4] | (unsigned)v[5] << 16, v[6] | (unsigned)v[7] << 16);
+            }
+        } else {
+            const float* src = static_cast<const float*>(p.x) + (long long)(row0 + r) * p.ldx + k;
+            float f[8];
+            if (p.vectors && k < p.K) {
+                const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+                f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = k + e < p.K ? src[e] : 0.f;
+            }
+            unsigned short v[8][3];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) three(f[e], v[e]);
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+                *reinterpret_cast<uint4*>(dst + (size_t)q * rows * stride) =
+                    make_uint4(v[0][q] | (unsigned)v[1][q] << 16, v[2][q] | (unsigned)v[3][q] << 16,
+                               v[4][q] | (unsigned)v[5][q] << 16, v[6][q] | (unsigned)v[7][q] << 16);
+        }
+    }
+}
+
+// NT: eights of staged rows; SP: strips of a warp; AHEAD: chunks that it has under way.
+template <int NT, int SP, int AHEAD, bool ZEROS>
+__global__ void __launch_bounds__(W4_THREADS, 2)
+w4_kernel(const W4Params p) {
+    extern __shared__ __align__(16) unsigned char w4_smem[];
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int side = warp % p.ws, turn = warp / p.ws;
+    const int strip0 = ((int)blockIdx.x * p.ws + side) * SP;
+    const int row0 = (int)blockIdx.y * p.slab, rows = min(p.slab, p.rows - row0);
+    const bool halves = p.group_shift == 0;                 // groups of 32: two a chunk
+    const int items = p.stages * p.stage_chunks / p.wk;     // chunks of a warp, some of the last ones beyond the sum's end
+
+    struct Item { uint4 w[SP]; unsigned s[SP][2]; unsigned z[SP]; };
+    auto load = [&](int i) -> Item {
+        Item it;
+        const int c = min(turn + p.wk * i, p.chunks - 1);
+        const int a = min((2 * c) >> p.group_shift, p.groups - 1), b = halves ? min(2 * c + 1, p.groups - 1) : a;
+#pragma unroll
+        for (int s = 0; s < SP; ++s) {
+            const size_t strip = min(strip0 + s, p.strips - 1);
+            it.w[s] = load_stream(p.words + (strip * p.chunks + c) * 32 + lane);
+            it.s[s][0] = __ldg(p.scales + (strip * p.groups + a) * 8 + g);
+            it.s[s][1] = halves ? __ldg(p.scales + (strip * p.groups + b) * 8 + g) : it.s[s][0];
+            if (ZEROS) {
+                it.z[s] = __ldg(p.zeros + (strip * p.groups + a) * 8 + g);
+                it.z[s] |= halves ? (unsigned)__ldg(p.zeros + (strip * p.groups + b) * 8 + g) << 16 : it.z[s] << 16;
+            }
+        }
+        return it;
+    };
+
+    Item ring[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) ring[i] = load(i);   // weights do not come from the kernel before
+    pdl_wait();
+
+    const int count = p.stage_chunks * W4_CHUNK, stride = count + W4_PAD;
+    bf16* x_smem = reinterpret_cast<bf16*>(w4_smem);
+    const size_t buffer = (size_t)NT * 8 * stride;
+    stage_rows(p, x_smem, stride, row0, rows, 0, count);
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+
+    float total[SP][NT][4], sum[SP][NT][4];
+#pragma unroll
+    for (int s = 0; s < SP; ++s)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) total[s][n][e] = sum[s][n][e] = 0.f;
+
+    const int per_stage = p.stage_chunks / p.wk;
+    const bf16* x_lane = x_smem;
+    int left = 0, stage = 0;
+    for (int i = 0; i < items; i += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (i + u >= items) break;
+            if (left == 0) {                                // the next stage of x: on its way since the one before began
+                left = per_stage;
+                asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+                __syncthreads();
+                if (stage + 1 < p.stages) {
+                    stage_rows(p, x_smem + ((stage + 1) & 1) * buffer, stride, row0, rows, (stage + 1) * count, count);
+                    asm volatile("cp.async.commit_group;\n" ::: "memory");
+                }
+                x_lane = x_smem + (stage & 1) * buffer + (size_t)g * stride + t * 8 + turn * W4_CHUNK;
+                ++stage;
+            }
+            const bf16* xc = x_lane + (size_t)(per_stage - left) * p.wk * W4_CHUNK;
+            --left;
+            if (turn + p.wk * (i + u) >= p.chunks) continue;            // (uniform in the warp)
+            const Item it = ring[u];
+            ring[u] = load(i + u + AHEAD);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4 x[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) x[n] = *reinterpret_cast<const uint4*>(xc + (size_t)n * 8 * stride + 32 * h);
+#pragma unroll
+                for (int s = 0; s < SP; ++s) {
+                    unsigned low = 0x43084308u, high = 0x43084308u;     // 128 + zero of the columns g and g + 8
+                    if (ZEROS) {
+                        const unsigned z = h ? it.z[s] >> 16 : it.z[s] & 0xffffu;
+                        low = 0x43004300u | (z & 0xffu) * 0x00010001u;
+                        high = 0x43004300u | (z >> 8) * 0x00010001u;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const unsigned w = h ? (j ? it.w[s].w : it.w[s].z) : (j ? it.w[s].y : it.w[s].x);
+                        const unsigned a[4] = {weight_pair(w, low), weight_pair(w >> 4, high), weight_pair(w >> 8, low), weight_pair(w >> 12, high)};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_bf16(sum[s][n], a, j ? x[n].z : x[n].x, j ? x[n].w : x[n].y);
+                    }
+                    if (h == 1 || halves) {
+                        const float s0 = low_half(it.s[s][h]), s1 = high_half(it.s[s][h]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            total[s][n][0] = fmaf(sum[s][n][0], s0, total[s][n][0]);
+                            total[s][n][1] = fmaf(sum[s][n][1], s0, total[s][n][1]);
+                            total[s][n][2] = fmaf(sum[s][n][2], s1, total[s][n][2]);
+                            total[s][n][3] = fmaf(sum[s][n][3], s1, total[s][n][3]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sum[s][n][e] = 0.f;
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // ---- the warps' turns added up, float32's three parts too (the small ones first), and stored ----
+    __syncthreads();
+    const int cols = p.ws * SP * W4_STRIP, pitch = cols + 1;
+    float* part = reinterpret_cast<float*>(w4_smem);        // [turn][staged row][column]
+#pragma unroll
+    for (int s = 0; s < SP; ++s)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                part[((size_t)turn * NT * 8 + n * 8 + t * 2 + (e & 1)) * pitch + (side * SP + s) * W4_STRIP + g + (e >> 1) * 8] = total[s][n][e];
+    __syncthreads();
+    const int first = (int)blockIdx.x * cols;
+    for (int i = threadIdx.x; i < rows * cols; i += W4_THREADS) {
+        const int r = i / cols, c = i - r * cols;
+        if (first + c >= p.N) continue;
+        float v = 0.f;
+        for (int q = p.f32 ? 2 : 0; q >= 0; --q)
+            for (int w = 0; w < p.wk; ++w) v += part[((size_t)w * NT * 8 + q * rows + r) * pitch + c];
+        const long long at = (long long)(row0 + r) * p.ldo + first + c;
+        if (p.f32) static_cast<float*>(p.out)[at] = v;
+        else static_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(v);
+    }
+}
+
+constexpr int W4_SMEM = 100 * 1024;         // two CTAs an SM
+
+template <int NT, int SP, int AHEAD, bool ZEROS> int w4_launch(W4Params p, int slabs, cudaStream_t stream) {
+    // warps side by side, and those that take turns: few columns leave the SMs to share out the sum
+    const int strips = (p.strips + SP - 1) / SP;
+    p.ws = 1;
+    while (p.ws < W4_WARPS && strips / (2 * p.ws) >= 4 * 148) p.ws *= 2;
+    p.wk = W4_WARPS / p.ws;
+    // x in one stage where it fits, else in two buffers
+    const int unit = p.wk;
+    const size_t row = (size_t)NT * 8 * 2;
+    int whole = (p.chunks + unit - 1) / unit * unit;
+    if (row * (whole * W4_CHUNK + W4_PAD) <= W4_SMEM) {
+        p.stage_chunks = whole;
+        p.stages = 1;
+    } else {
+        p.stage_chunks = (int)((W4_SMEM / 2 / row - W4_PAD) / W4_CHUNK) / unit * unit;
+        if (p.stage_chunks < unit) p.stage_chunks = unit;
+        p.stages = (p.chunks + p.stage_chunks - 1) / p.stage_chunks;
+    }
+    const size_t staged = row * (p.stage_chunks * W4_CHUNK + W4_PAD) * (p.stages > 1 ? 2 : 1);
+    const size_t parts = (size_t)p.wk * NT * 8 * (p.ws * SP * W4_STRIP + 1) * 4;
+    const size_t smem = staged > parts ? staged : parts;
+    static DeviceOnce configured;
+    if (configured.first() && cudaFuncSetAttribute(w4_kernel<NT, SP, AHEAD, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
+        return tis_check_launch("gemm_w4 (shared memory)");
+    if (smem > 227 * 1024) {
+        tis_set_error("gemm_w4: %zu bytes of shared memory", smem);
+        return TIS_BAD_SIZE;
+    }
+    const int ctas = (p.strips + p.ws * SP - 1) / (p.ws * SP);
+    tis_launch(w4_kernel<NT, SP, AHEAD, ZEROS>, dim3((unsigned)ctas, (unsigned)slabs), dim3(W4_THREADS), smem, stream, p);
+    return tis_check_launch("gemm_w4");
+}
+
+template <int NT, int SP, int AHEAD> int w4_zeros(const W4Params& p, int slabs, cudaStream_t stream) {
+    return p.zeros != nullptr ? w4_launch<NT, SP, AHEAD, true>(p, slabs, stream) : w4_launch<NT, SP, AHEAD, false>(p, slabs, stream);
+}
+
+}  // namespace
+
+// out (rows, N) = x (rows, K) times the packed weights; dtype is that of x and out, rows of both contiguous, row strides free.
+TIS_API int tis_gemm_w4(int dtype, const void* x, long long ldx, const void* words, const void* scales, const void* zeros, void* out,
+                        long long ldo, int rows, int K, int N, int group, cudaStream_t stream) {
+    if (rows <= 0 || N <= 0) return TIS_OK;
+    if (dtype != TIS_F32 && dtype != TIS_BF16) {
+        tis_set_error("gemm_w4: dtype code %d", dtype);
+        return TIS_BAD_DTYPE;
+    }
+    if (K <= 0 || K > (1 << 30) || N > (1 << 30) || group < 32 || (group & (group - 1)) != 0) {
+        tis_set_error("gemm_w4: %d x %d in groups of %d", K, N, group);
+        return TIS_BAD_SIZE;
+    }
+    W4Params p = {};
+    p.words = static_cast<const uint4*>(words);
+    p.scales = static_cast<const unsigned*>(scales);
+    p.zeros = static_cast<const unsigned short*>(zeros);
+    p.x = x; p.ldx = ldx; p.out = out; p.ldo = ldo;
+    p.rows = rows; p.K = K; p.N = N;
+    p.chunks = (K + W4_CHUNK - 1) / W4_CHUNK;
+    p.strips = (N + W4_STRIP - 1) / W4_STRIP;
+    p.groups = (int)(((long long)K + group - 1) / group);
+    for (int h = group / 32; h > 1; h >>= 1) ++p.group_shift;
+    p.f32 = dtype == TIS_F32;
+    p.vectors = K % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (p.f32 ? 4 : 8) == 0;
+    // rows in slabs of about the same size
+    const int most = p.f32 ? W4_ROWS_F32 : W4_ROWS;
+    const int slabs = (rows + most - 1) / most;
+    if (slabs > 65535) {
+        tis_set_error("gemm_w4: %d rows", rows);
+        return TIS_BAD_SIZE;
+    }
+    p.slab = (rows + slabs - 1) / slabs;
+    const int eights = ((p.f32 ? 3 : 1) * p.slab + 7) / 8;
+    switch (eights) {
+        case 1: return w4_zeros<1, 2, 4>(p, slabs, stream);
+        case 2: return w4_zeros<2, 2, 2>(p, slabs, stream);
+        case 3: return w4_zeros<3, 1, 4>(p, slabs, stream);
+        case 4: return w4_zeros<4, 1, 4>(p, slabs, stream);
+        case 5: return w4_zeros<5, 1, 2>(p, slabs, stream);
+        case 6: return w4_zeros<6, 1, 2>(p, slabs, stream);
+        default: return w4_zeros<8, 1, 1>(p, slabs, stream);
+    }
+}

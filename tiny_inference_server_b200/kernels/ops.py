@@ -32,7 +32,7 @@ class KernelError(RuntimeError):
 
 
 #: argument kinds of launchers whose pointers are passed as plain numbers: p a pointer, i an int, l a 64-bit int, f a float
-_ARGUMENTS = {"tis_verify_drafts": "pllpllpppppiiip"}
+_ARGUMENTS = {"tis_verify_drafts": "pllpllpppppiiip", "tis_gemm_w4": "iplppppliiiip"}
 _KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 
 
@@ -656,6 +656,32 @@ def gemm_f32_out(a: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
 # ---------------------------------------------------------------------------------------
 # row-wise kernels
 # ---------------------------------------------------------------------------------------
+
+def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``a (n, K) @ w (K, N)`` for weights of four bits (``weights.w4.pack_w4``), a and the result in bfloat16 or float32; row strides
+    free.  Every weight is taken as it is, (code - zero) * scale, and a sum is rounded once, when it is stored.
+
+    For few rows: the weights are streamed once for up to 64 rows of bfloat16 and 21 of float32, and again for as many more.  (A prompt's rows
+    are better off with ``weights.w4.unpack_w4`` and ``gemm``.)"""
+    words = w.words
+    n, k = a.shape
+    dtype = a.dtype
+    if k != w.k or (dtype is not torch.bfloat16 and dtype is not torch.float32) or (k > 1 and a.stride(1) != 1):
+        raise KernelError(f"gemm_w4: rows {dtype} {tuple(a.shape)} (bfloat16 or float32, contiguous) for weights {w.k} x {w.n}")
+    if out is None:
+        out = torch.empty((n, w.n), dtype=dtype, device=a.device)
+    elif out.dtype is not dtype or out.shape != (n, w.n) or (w.n > 1 and out.stride(1) != 1):
+        raise KernelError(f"gemm_w4: result {out.dtype} {tuple(out.shape)} for {n} rows of {dtype} and weights {w.k} x {w.n}")
+    _on_this_device("gemm_w4", a, out, words)
+    if n == 0:
+        return out
+    lib = library()
+    calls["gemm_w4"] += 1
+    _check(lib.tis_gemm_w4(_dt(a), a.data_ptr(), a.stride(0), words.data_ptr(), w.scales.data_ptr(),
+                           None if w.zeros is None else w.zeros.data_ptr(), out.data_ptr(), out.stride(0), n, k, w.n, w.group,
+                           _stream()), lib)
+    return out
+
 
 def embed_rows(table: torch.Tensor, tokens: torch.Tensor, out: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """out[r] = float(table[tokens[r]]) * scale; out is the float32 residual stream (n, d)."""

@@ -1,0 +1,123 @@
+"""Weights of four bits: codes 0..15 with a scale, and perhaps a zero point, per group of entries along the sum.
+
+A weight of a (K, N) matrix is ``(code[k, n] - zero[k // group, n]) * scale[k // group, n]`` (zero 8 where no zero points are
+kept).  ``quantize_w4`` finds codes by rounding to nearest, ``pack_w4`` lays codes out once as ``kernels.ops.gemm_w4`` streams
+them, ``unpack_w4`` gives the matrix back (for products of many rows).
+
+Layout.  16 columns ("strip") by 64 entries of the sum ("chunk") are 512 bytes in a row: 16 bytes of each lane of a warp, which are
+that lane's parts of four 16 x 16 operands of ``mma.sync`` (columns as rows).  Lane (g, t) = (lane // 4, lane % 4) holds columns g
+and g + 8; its word 2 h + j the entries 32 h + 8 t + 4 j + (0..3) of the chunk: bits 0-3 and 16-19 the first two of column g, 4-7 and
+20-23 those of column g + 8, 8-11 and 24-27 the last two of column g, 12-15 and 28-31 those of column g + 8.  So a shift and
+a mask give two neighbouring entries in the halves of a register, and the entries that a lane needs of a row of activations are
+16 contiguous bytes.  Scales and zero points lie as pairs (column g, column g + 8) by strip and group.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Tuple
+
+import torch
+
+STRIP, CHUNK = 16, 64
+
+
+@dataclass(frozen=True)
+class W4Weights:
+    """Codes in the kernel's layout: ``words`` (strips, chunks, 32, 4) int32, ``scales`` (strips, groups, 8, 2) bfloat16, ``zeros``
+    the same in uint8 (None: 8 everywhere)."""
+    words: torch.Tensor
+    scales: torch.Tensor
+    zeros: Optional[torch.Tensor]
+    k: int
+    n: int
+    group: int
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.k, self.n
+
+    @property
+    def device(self) -> torch.device:
+        return self.words.device
+
+
+def _groups(k: int, group: int) -> int:
+    if group < 32 or group & (group - 1):
+        raise ValueError(f"groups of {group} entries: a power of two from 32 on is wanted (one of K or more: a scale per column)")
+    return -(-k // group)
+
+
+def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False):
+    """(codes (K, N) uint8, scales (groups, N) bfloat16, zeros (groups, N) uint8 or None) of a matrix, rounded to nearest: without zero
+    points the largest entry of a group by size becomes 7 or -7 steps; with them the group's range, zero included, 15 steps."""
+    if w.dim() != 2 or not w.is_floating_point() or 0 in w.shape:
+        raise ValueError(f"a matrix of floating-point weights is wanted, not {w.dtype} {tuple(w.shape)}")
+    k, n = w.shape
+    groups = _groups(k, group)
+    x = torch.zeros((groups * group, n), dtype=torch.float32, device=w.device)
+    x[:k] = w
+    x = x.reshape(groups, group, n)
+    if zeros:
+        low, high = x.amin(1).clamp(max=0.0), x.amax(1).clamp(min=0.0)
+        scales = ((high - low) / 15.0).to(torch.bfloat16)
+    else:
+        scales = (x.abs().amax(1) / 7.0).to(torch.bfloat16)
+    scales = torch.where(scales > 0, scales, 1.0).to(torch.bfloat16)        # (a group of zeros)
+    step = scales.float()[:, None]
+    zero = (-low / step[:, 0]).round().clamp(0, 15) if zeros else None
+    codes = ((x / step).round() + (zero[:, None] if zeros else 8.0)).clamp(0, 15)
+    return codes.to(torch.uint8).reshape(groups * group, n)[:k].contiguous(), scales, None if zero is None else zero.to(torch.uint8)
+
+
+def _pairs(x: torch.Tensor) -> torch.Tensor:
+    """(groups, N) by strip and group as pairs of the columns g and g + 8 (columns beyond N: zero)."""
+    groups, n = x.shape
+    strips = -(-n // STRIP)
+    y = torch.zeros((groups, strips * STRIP), dtype=x.dtype, device=x.device)
+    y[:, :n] = x
+    return y.reshape(groups, strips, 2, 8).permute(1, 0, 3, 2).contiguous()
+
+
+def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, group: int = 128) -> W4Weights:
+    """Lay codes (K, N) uint8 (0..15), scales (groups, N) bfloat16 and zero points (groups, N) uint8 (0..15; None: 8) out for ``gemm_w4``."""
+    if codes.dim() != 2 or codes.dtype != torch.uint8 or 0 in codes.shape:
+        raise ValueError(f"codes (K, N) in uint8 are wanted, not {codes.dtype} {tuple(codes.shape)}")
+    k, n = codes.shape
+    groups = _groups(k, group)
+    if scales.dtype != torch.bfloat16 or tuple(scales.shape) != (groups, n):
+        raise ValueError(f"scales {scales.dtype} {tuple(scales.shape)}: bfloat16 ({groups}, {n}) is wanted")
+    if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != (groups, n)):
+        raise ValueError(f"zero points {zeros.dtype} {tuple(zeros.shape)}: uint8 ({groups}, {n}) is wanted")
+    if scales.device != codes.device or (zeros is not None and zeros.device != codes.device):
+        raise ValueError("codes, scales and zero points lie on different devices")
+    if int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15):
+        raise ValueError("codes and zero points are 0..15")
+    strips, chunks = -(-n // STRIP), -(-k // CHUNK)
+    words = torch.empty((strips, chunks, 32, 4), dtype=torch.int32, device=codes.device)
+    for a in range(0, strips, 1024):                          # (in pieces: the working copies are several times the codes)
+        b = min(a + 1024, strips)
+        x = torch.zeros((chunks * CHUNK, (b - a) * STRIP), dtype=torch.uint8, device=codes.device)
+        part = codes[:, a * STRIP:b * STRIP]
+        x[:k, : part.shape[1]] = part
+        # chunk, half h, t, word j, pair i, entry e of the pair; strip, column half c, g
+        x = x.reshape(chunks, 2, 4, 2, 2, 2, b - a, 2, 8)
+        # strip, chunk, g, t, h, j, e, i, c: nibble 4 e + 2 i + c
+        x = x.permute(6, 0, 8, 2, 1, 3, 5, 4, 7).reshape(b - a, chunks, 32, 4, 4, 2)
+        x = x[..., 0] | (x[..., 1] << 4)                      # bytes, the low nibble first
+        words[a:b] = x.contiguous().view(torch.int32).squeeze(-1)
+    return W4Weights(words, _pairs(scales), None if zeros is None else _pairs(zeros), k, n, group)
+
+
+def unpack_w4(w: W4Weights, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The (K, N) matrix of packed weights: every weight worked out in 32 bits and rounded to ``dtype`` once."""
+    strips, chunks = w.words.shape[:2]
+    x = w.words.contiguous().view(torch.uint8).reshape(strips, chunks, 8, 4, 2, 2, 4)
+    x = torch.stack([x & 15, x >> 4], -1).reshape(strips, chunks, 8, 4, 2, 2, 2, 2, 2)          # strip, chunk, g, t, h, j, e, i, c
+    codes = x.permute(1, 4, 3, 5, 7, 6, 0, 8, 2).reshape(chunks * CHUNK, strips * STRIP)[: w.k, : w.n]
+
+    def rows(pairs):
+        y = pairs.permute(1, 0, 3, 2).reshape(pairs.shape[1], strips * STRIP)[:, : w.n]
+        return y.repeat_interleave(w.group, 0)[: w.k].float()
+
+    zero = rows(w.zeros) if w.zeros is not None else 8.0
+    return ((codes.float() - zero) * rows(w.scales)).to(dtype)
