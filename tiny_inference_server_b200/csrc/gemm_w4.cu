@@ -104,179 +104,218 @@ __device__ __forceinline__ void stage_rows(const W4Params& p, bf16* to, int stri
     }
 }
 
-// NT: eights of staged rows; SP: strips of a warp; AHEAD: chunks that it has under way.
-template <int NT, int SP, int AHEAD, bool ZEROS>
+// NT: eights of staged rows; SP: strips of a warp; AHEAD: chunks that it has under way; HALVES: groups of 32, two a chunk.
+template <int NT, int SP, int AHEAD, bool HALVES, bool ZEROS>
 __global__ void __launch_bounds__(W4_THREADS, 2)
 w4_kernel(const W4Params p) {
     extern __shared__ __align__(16) unsigned char w4_smem[];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int side = warp % p.ws, turn = warp / p.ws;
-    const int strip0 = ((int)blockIdx.x * p.ws + side) * SP;
     const int row0 = (int)blockIdx.y * p.slab, rows = min(p.slab, p.rows - row0);
-    const bool halves = p.group_shift == 0;                 // groups of 32: two a chunk
-    const int items = p.stages * p.stage_chunks / p.wk;     // chunks of a warp, some of the last ones beyond the sum's end
+    constexpr int GROUPS = HALVES ? 2 : 1;                  // of a chunk
+    const int strips_of_tile = p.ws * SP, tiles = (p.strips + strips_of_tile - 1) / strips_of_tile;
+    const int mine = turn < p.chunks ? (p.chunks - turn + p.wk - 1) / p.wk : 0;         // this warp's chunks of a tile
 
-    struct Item { uint4 w[SP]; unsigned s[SP][2]; unsigned z[SP]; };
-    auto load = [&](int i) -> Item {
-        Item it;
-        const int c = min(turn + p.wk * i, p.chunks - 1);
-        const int a = min((2 * c) >> p.group_shift, p.groups - 1), b = halves ? min(2 * c + 1, p.groups - 1) : a;
+    struct Item { uint4 w[SP]; unsigned s[SP][GROUPS]; unsigned z[ZEROS ? SP : 1][GROUPS]; };
+    // ---- the loads: chunks one after another, tile after tile.  (Places in 32 bits: of 16 bytes, of pairs of scales.) ----
+    int load_tile = blockIdx.x, load_i = 0;
+    unsigned words[SP], groups[SP];
+    auto aim = [&]() {
 #pragma unroll
         for (int s = 0; s < SP; ++s) {
-            const size_t strip = min(strip0 + s, p.strips - 1);
-            it.w[s] = load_stream(p.words + (strip * p.chunks + c) * 32 + lane);
-            it.s[s][0] = __ldg(p.scales + (strip * p.groups + a) * 8 + g);
-            it.s[s][1] = halves ? __ldg(p.scales + (strip * p.groups + b) * 8 + g) : it.s[s][0];
-            if (ZEROS) {
-                it.z[s] = __ldg(p.zeros + (strip * p.groups + a) * 8 + g);
-                it.z[s] |= halves ? (unsigned)__ldg(p.zeros + (strip * p.groups + b) * 8 + g) << 16 : it.z[s] << 16;
+            const unsigned strip = (unsigned)min(load_tile * strips_of_tile + side * SP + s, p.strips - 1);
+            words[s] = (strip * (unsigned)p.chunks + turn) * 32 + lane;
+            groups[s] = strip * (unsigned)p.groups * 8 + g;
+        }
+    };
+    auto load = [&](Item& it, int i) {
+        if (load_tile < tiles && i < mine) {
+            const int c = turn + p.wk * i;
+#pragma unroll
+            for (int s = 0; s < SP; ++s) {
+                it.w[s] = load_stream(p.words + words[s]);
+                words[s] += p.wk * 32;
+#pragma unroll
+                for (int h = 0; h < GROUPS; ++h) {
+                    const unsigned a = groups[s] + 8 * (HALVES ? min(2 * c + h, p.groups - 1) : (2 * c) >> p.group_shift);
+                    it.s[s][h] = __ldg(p.scales + a);
+                    if (ZEROS) it.z[s][h] = __ldg(p.zeros + a);
+                }
             }
         }
-        return it;
     };
-
+    // behind AHEAD loads: the chunks of a tile are taken AHEAD at a time, and the next tile's follow
+    auto advance = [&]() {
+        load_i += AHEAD;
+        if (load_i >= mine) {
+            load_i = 0;
+            load_tile += gridDim.x;
+            if (load_tile < tiles) aim();
+        }
+    };
     Item ring[AHEAD];
+    aim();
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) ring[i] = load(i);   // weights do not come from the kernel before
+    for (int u = 0; u < AHEAD; ++u) load(ring[u], u);       // (weights do not come from the kernel before)
+    advance();
     pdl_wait();
 
     const int count = p.stage_chunks * W4_CHUNK, stride = count + W4_PAD;
     bf16* x_smem = reinterpret_cast<bf16*>(w4_smem);
-    const size_t buffer = (size_t)NT * 8 * stride;
+    const size_t buffer = (size_t)NT * 8 * stride;          // elements
+    const int buffers = p.stages > 1 ? 2 : 1;
+    const int cols = strips_of_tile * W4_STRIP, pitch = cols + 1;
+    float* part = reinterpret_cast<float*>(x_smem + buffers * buffer);          // [two][turn][staged row][column]
+    const int part_floats = p.wk * NT * 8 * pitch;
+
     stage_rows(p, x_smem, stride, row0, rows, 0, count);
     asm volatile("cp.async.commit_group;\n" ::: "memory");
-
-    float total[SP][NT][4], sum[SP][NT][4];
-#pragma unroll
-    for (int s = 0; s < SP; ++s)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) total[s][n][e] = sum[s][n][e] = 0.f;
-
     const int per_stage = p.stage_chunks / p.wk;
-    const bf16* x_lane = x_smem;
-    int left = 0, stage = 0;
-    for (int i = 0; i < items; i += AHEAD) {
+    bool staged = false;                                    // (x in one stage: it stays)
+    int stages_done = 0, flip = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, flip ^= 1) {
+        float total[SP][NT][4];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            if (i + u >= items) break;
-            if (left == 0) {                                // the next stage of x: on its way since the one before began
-                left = per_stage;
+        for (int s = 0; s < SP; ++s)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) total[s][n][e] = 0.f;
+        for (int stage = 0; stage < p.stages; ++stage) {
+            const int now = p.stages > 1 ? stages_done & 1 : 0;
+            if (!staged) {
+                // the stage that was ordered last is here; the next one, of the next tile's behind this tile's last, is ordered
                 asm volatile("cp.async.wait_group 0;\n" ::: "memory");
                 __syncthreads();
-                if (stage + 1 < p.stages) {
-                    stage_rows(p, x_smem + ((stage + 1) & 1) * buffer, stride, row0, rows, (stage + 1) * count, count);
+                if (p.stages > 1) {
+                    if (stage + 1 < p.stages || tile + (int)gridDim.x < tiles)
+                        stage_rows(p, x_smem + (now ^ 1) * buffer, stride, row0, rows, (stage + 1 < p.stages ? stage + 1 : 0) * count, count);
                     asm volatile("cp.async.commit_group;\n" ::: "memory");
+                    ++stages_done;
                 }
-                x_lane = x_smem + (stage & 1) * buffer + (size_t)g * stride + t * 8 + turn * W4_CHUNK;
-                ++stage;
+                staged = p.stages == 1;
             }
-            const bf16* xc = x_lane + (size_t)(per_stage - left) * p.wk * W4_CHUNK;
-            --left;
-            if (turn + p.wk * (i + u) >= p.chunks) continue;            // (uniform in the warp)
-            const Item it = ring[u];
-            ring[u] = load(i + u + AHEAD);
+            const bf16* x_lane = x_smem + now * buffer + (size_t)g * stride + t * 8 + turn * W4_CHUNK;
+            // (chunks of the stage: per_stage of this warp's, in steps of AHEAD, per_stage being a multiple of that where there are several stages)
+            for (int i = stage * per_stage; i < min(mine, (stage + 1) * per_stage); i += AHEAD) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint4 x[NT];
+                for (int u = 0; u < AHEAD; ++u) {
+                    Item& it = ring[u];
+                    if (i + u < mine) {                     // (uniform in the warp)
+                    const int local = (i + u - stage * per_stage) * p.wk;
+                    const bf16* xc = x_lane + local * W4_CHUNK;
+                    float sum[SP][NT][4];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) x[n] = *reinterpret_cast<const uint4*>(xc + (size_t)n * 8 * stride + 32 * h);
+                    for (int h = 0; h < 2; ++h) {
+                        uint4 x[NT];
 #pragma unroll
-                for (int s = 0; s < SP; ++s) {
-                    unsigned low = 0x43084308u, high = 0x43084308u;     // 128 + zero of the columns g and g + 8
-                    if (ZEROS) {
-                        const unsigned z = h ? it.z[s] >> 16 : it.z[s] & 0xffffu;
-                        low = 0x43004300u | (z & 0xffu) * 0x00010001u;
-                        high = 0x43004300u | (z >> 8) * 0x00010001u;
-                    }
+                        for (int n = 0; n < NT; ++n) x[n] = *reinterpret_cast<const uint4*>(xc + (size_t)n * 8 * stride + 32 * h);
+                        if (h == 0 || HALVES) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const unsigned w = h ? (j ? it.w[s].w : it.w[s].z) : (j ? it.w[s].y : it.w[s].x);
-                        const unsigned a[4] = {weight_pair(w, low), weight_pair(w >> 4, high), weight_pair(w >> 8, low), weight_pair(w >> 12, high)};
+                            for (int s = 0; s < SP; ++s)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_bf16(sum[s][n], a, j ? x[n].z : x[n].x, j ? x[n].w : x[n].y);
-                    }
-                    if (h == 1 || halves) {
-                        const float s0 = low_half(it.s[s][h]), s1 = high_half(it.s[s][h]);
+                                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            total[s][n][0] = fmaf(sum[s][n][0], s0, total[s][n][0]);
-                            total[s][n][1] = fmaf(sum[s][n][1], s0, total[s][n][1]);
-                            total[s][n][2] = fmaf(sum[s][n][2], s1, total[s][n][2]);
-                            total[s][n][3] = fmaf(sum[s][n][3], s1, total[s][n][3]);
+                                    for (int e = 0; e < 4; ++e) sum[s][n][e] = 0.f;
+                        }
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) sum[s][n][e] = 0.f;
+                        for (int s = 0; s < SP; ++s) {
+                            // 128 + zero of the columns g and g + 8
+                            const unsigned z = ZEROS ? it.z[ZEROS ? s : 0][HALVES ? h : 0] : 0x0808u;
+                            const unsigned low = 0x43004300u | (z & 0xffu) * 0x00010001u, high = 0x43004300u | (z >> 8) * 0x00010001u;
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const unsigned w = h ? (j ? it.w[s].w : it.w[s].z) : (j ? it.w[s].y : it.w[s].x);
+                                const unsigned a[4] = {weight_pair(w, low), weight_pair(w >> 4, high),
+                                                       weight_pair(w >> 8, low), weight_pair(w >> 12, high)};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) mma_bf16(sum[s][n], a, j ? x[n].z : x[n].x, j ? x[n].w : x[n].y);
+                            }
+                            if (h == 1 || HALVES) {
+                                const unsigned sc = it.s[s][HALVES ? h : 0];
+                                const float s0 = low_half(sc), s1 = high_half(sc);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    total[s][n][0] = fmaf(sum[s][n][0], s0, total[s][n][0]);
+                                    total[s][n][1] = fmaf(sum[s][n][1], s0, total[s][n][1]);
+                                    total[s][n][2] = fmaf(sum[s][n][2], s1, total[s][n][2]);
+                                    total[s][n][3] = fmaf(sum[s][n][3], s1, total[s][n][3]);
+                                }
+                            }
                         }
                     }
+                    }
+                    load(it, load_i + u);                   // its place is free: the chunk AHEAD further
                 }
+                advance();
             }
         }
-    }
-
-    // ---- the warps' turns added up, float32's three parts too (the small ones first), and stored ----
-    __syncthreads();
-    const int cols = p.ws * SP * W4_STRIP, pitch = cols + 1;
-    float* part = reinterpret_cast<float*>(w4_smem);        // [turn][staged row][column]
+        // ---- the warps' turns added up, float32's three parts too (the small ones first), and stored.  Two tiles' sums lie side by
+        // side: a warp may be a tile ahead of the slowest, not two ----
+        float* here = part + flip * part_floats;
 #pragma unroll
-    for (int s = 0; s < SP; ++s)
+        for (int s = 0; s < SP; ++s)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                part[((size_t)turn * NT * 8 + n * 8 + t * 2 + (e & 1)) * pitch + (side * SP + s) * W4_STRIP + g + (e >> 1) * 8] = total[s][n][e];
-    __syncthreads();
-    const int first = (int)blockIdx.x * cols;
-    for (int i = threadIdx.x; i < rows * cols; i += W4_THREADS) {
-        const int r = i / cols, c = i - r * cols;
-        if (first + c >= p.N) continue;
-        float v = 0.f;
-        for (int q = p.f32 ? 2 : 0; q >= 0; --q)
-            for (int w = 0; w < p.wk; ++w) v += part[((size_t)w * NT * 8 + q * rows + r) * pitch + c];
-        const long long at = (long long)(row0 + r) * p.ldo + first + c;
-        if (p.f32) static_cast<float*>(p.out)[at] = v;
-        else static_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(v);
+                for (int e = 0; e < 4; ++e)
+                    here[((size_t)turn * NT * 8 + n * 8 + t * 2 + (e & 1)) * pitch + (side * SP + s) * W4_STRIP + g + (e >> 1) * 8] = total[s][n][e];
+        __syncthreads();
+        const int first = tile * cols;
+        for (int i = threadIdx.x; i < rows * cols; i += W4_THREADS) {
+            const int r = i / cols, c = i - r * cols;
+            if (first + c >= p.N) continue;
+            float v = 0.f;
+            for (int q = p.f32 ? 2 : 0; q >= 0; --q)
+                for (int w = 0; w < p.wk; ++w) v += here[((size_t)w * NT * 8 + q * rows + r) * pitch + c];
+            const long long at = (long long)(row0 + r) * p.ldo + first + c;
+            if (p.f32) static_cast<float*>(p.out)[at] = v;
+            else static_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(v);
+        }
     }
 }
 
-constexpr int W4_SMEM = 100 * 1024;         // two CTAs an SM
+constexpr int W4_SMEM = 112 * 1024;         // two CTAs an SM
 
-template <int NT, int SP, int AHEAD, bool ZEROS> int w4_launch(W4Params p, int slabs, cudaStream_t stream) {
-    // warps side by side, and those that take turns: few columns leave the SMs to share out the sum
-    const int strips = (p.strips + SP - 1) / SP;
+template <int NT, int SP, int AHEAD, bool HALVES, bool ZEROS> int w4_launch(W4Params p, int slabs, cudaStream_t stream) {
+    auto bytes = [&](int stage_chunks, int buffers) {
+        const size_t count = (size_t)stage_chunks * W4_CHUNK;
+        const size_t staged = (size_t)NT * 8 * (count + W4_PAD) * 2 * buffers;
+        return staged + (size_t)2 * p.wk * NT * 8 * (p.ws * SP * W4_STRIP + 1) * 4;
+    };
+    // x in one stage where it fits: all warps share out the sum.  Else four of them stand side by side, for fewer passes over x.
     p.ws = 1;
-    while (p.ws < W4_WARPS && strips / (2 * p.ws) >= 4 * 148) p.ws *= 2;
-    p.wk = W4_WARPS / p.ws;
-    // x in one stage where it fits, else in two buffers
-    const int unit = p.wk;
-    const size_t row = (size_t)NT * 8 * 2;
-    int whole = (p.chunks + unit - 1) / unit * unit;
-    if (row * (whole * W4_CHUNK + W4_PAD) <= W4_SMEM) {
-        p.stage_chunks = whole;
-        p.stages = 1;
-    } else {
-        p.stage_chunks = (int)((W4_SMEM / 2 / row - W4_PAD) / W4_CHUNK) / unit * unit;
-        if (p.stage_chunks < unit) p.stage_chunks = unit;
+    p.wk = W4_WARPS;
+    p.stages = 1;
+    p.stage_chunks = (p.chunks + p.wk - 1) / p.wk * p.wk;
+    if (bytes(p.stage_chunks, 1) > W4_SMEM) {
+        p.ws = 4;
+        p.wk = 2;
+        const int unit = p.wk * AHEAD;
+        p.stage_chunks = unit;
+        while (bytes(p.stage_chunks + unit, 2) <= W4_SMEM) p.stage_chunks += unit;
         p.stages = (p.chunks + p.stage_chunks - 1) / p.stage_chunks;
     }
-    const size_t staged = row * (p.stage_chunks * W4_CHUNK + W4_PAD) * (p.stages > 1 ? 2 : 1);
-    const size_t parts = (size_t)p.wk * NT * 8 * (p.ws * SP * W4_STRIP + 1) * 4;
-    const size_t smem = staged > parts ? staged : parts;
+    const size_t smem = bytes(p.stage_chunks, p.stages > 1 ? 2 : 1);
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(w4_kernel<NT, SP, AHEAD, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
+    if (configured.first() && cudaFuncSetAttribute(w4_kernel<NT, SP, AHEAD, HALVES, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
         return tis_check_launch("gemm_w4 (shared memory)");
     if (smem > 227 * 1024) {
         tis_set_error("gemm_w4: %zu bytes of shared memory", smem);
         return TIS_BAD_SIZE;
     }
-    const int ctas = (p.strips + p.ws * SP - 1) / (p.ws * SP);
-    tis_launch(w4_kernel<NT, SP, AHEAD, ZEROS>, dim3((unsigned)ctas, (unsigned)slabs), dim3(W4_THREADS), smem, stream, p);
+    const int tiles = (p.strips + p.ws * SP - 1) / (p.ws * SP);
+    const int most = 2 * 148;
+    tis_launch(w4_kernel<NT, SP, AHEAD, HALVES, ZEROS>, dim3((unsigned)(tiles < most ? tiles : most), (unsigned)slabs), dim3(W4_THREADS), smem, stream, p);
     return tis_check_launch("gemm_w4");
 }
 
-template <int NT, int SP, int AHEAD> int w4_zeros(const W4Params& p, int slabs, cudaStream_t stream) {
-    return p.zeros != nullptr ? w4_launch<NT, SP, AHEAD, true>(p, slabs, stream) : w4_launch<NT, SP, AHEAD, false>(p, slabs, stream);
+template <int NT, int SP, int AHEAD, bool HALVES> int w4_zeros(const W4Params& p, int slabs, cudaStream_t stream) {
+    return p.zeros != nullptr ? w4_launch<NT, SP, AHEAD, HALVES, true>(p, slabs, stream) : w4_launch<NT, SP, AHEAD, HALVES, false>(p, slabs, stream);
+}
+template <int NT, int SP, int AHEAD> int w4_forms(const W4Params& p, int slabs, cudaStream_t stream) {
+    return p.group_shift == 0 ? w4_zeros<NT, SP, AHEAD, true>(p, slabs, stream) : w4_zeros<NT, SP, AHEAD, false>(p, slabs, stream);
 }
 
 }  // namespace
@@ -315,12 +354,12 @@ TIS_API int tis_gemm_w4(int dtype, const void* x, long long ldx, const void* wor
     p.slab = (rows + slabs - 1) / slabs;
     const int eights = ((p.f32 ? 3 : 1) * p.slab + 7) / 8;
     switch (eights) {
-        case 1: return w4_zeros<1, 2, 4>(p, slabs, stream);
-        case 2: return w4_zeros<2, 2, 2>(p, slabs, stream);
-        case 3: return w4_zeros<3, 1, 4>(p, slabs, stream);
-        case 4: return w4_zeros<4, 1, 4>(p, slabs, stream);
-        case 5: return w4_zeros<5, 1, 2>(p, slabs, stream);
-        case 6: return w4_zeros<6, 1, 2>(p, slabs, stream);
-        default: return w4_zeros<8, 1, 1>(p, slabs, stream);
+        case 1: return p.strips <= 2 * 148 ? w4_forms<1, 1, 4>(p, slabs, stream) : w4_forms<1, 2, 4>(p, slabs, stream);
+        case 2: return w4_forms<2, 2, 2>(p, slabs, stream);
+        case 3: return w4_forms<3, 1, 4>(p, slabs, stream);
+        case 4: return w4_forms<4, 1, 4>(p, slabs, stream);
+        case 5: return w4_forms<5, 1, 2>(p, slabs, stream);
+        case 6: return w4_forms<6, 1, 2>(p, slabs, stream);
+        default: return w4_forms<8, 1, 2>(p, slabs, stream);
     }
 }
