@@ -95,6 +95,52 @@ class AttentionTilePlanner(StepPlanner):
                        (arrays["w0"], arrays["wn"], nw), nrw, keys_identity=len(facts) > 5 and bool(facts[5]))
 
 
+class SharedPrefixPlan:
+    """The rows of a batch whose requests share keys, cut into tiles for ``ops.shared_prefix_attention``.
+
+    ``groups``: in the order of the rows, (keys shared by the group's requests, [(slot, rows) of every request]): a request's rows
+    follow one another, a group's requests too.  A request without anything to share is a group of its own, with 0 keys.  The plan is
+    made once for a batch and holds as long as its requests, rows and shared keys do; the rows' positions are not part of it.
+
+    Tiles are counted in row heads: (row, query head) of a kv head, the G heads of a row one after another.  ``own``: up to OWN_TILE of one
+    request; ``wide`` (``narrow``): up to WIDE_TILE (OWN_TILE) of one group.  Each is (first row head, row heads, slot, shared keys),
+    int32 on the device; a group's keys are read through the table of its first request."""
+
+    OWN_TILE, WIDE_TILE = 16, 64
+
+    def __init__(self, groups: Sequence[Tuple[int, Sequence[Tuple[int, int]]]], num_heads: int, kv_heads: int, device="cuda"):
+        if kv_heads <= 0 or num_heads <= 0 or num_heads % kv_heads:
+            raise ValueError(f"{num_heads} query heads are not a multiple of {kv_heads} kv heads")
+        self.num_heads, self.kv_heads, self.group_size = num_heads, kv_heads, num_heads // kv_heads
+        g = self.group_size
+        own, wide, narrow = [], [], []
+        rows, self.max_slot, self.max_shared, self.min_shared, slots = 0, -1, 0, None, set()
+        for shared, requests in groups:
+            if shared < 0 or not requests:
+                raise ValueError(f"a group shares {shared} keys and has {len(requests)} requests")
+            first = rows
+            for slot, n in requests:
+                if slot < 0 or n <= 0 or slot in slots:
+                    raise ValueError(f"slot {slot} with {n} rows: every request stands once in a plan, with at least one row")
+                slots.add(slot)
+                own += [(rows * g + a, min(self.OWN_TILE, n * g - a), slot, shared) for a in range(0, n * g, self.OWN_TILE)]
+                rows += n
+            heads = (rows - first) * g
+            for tiles, size in ((wide, self.WIDE_TILE), (narrow, self.OWN_TILE)):
+                tiles += [(first * g + a, min(size, heads - a), requests[0][0], shared) for a in range(0, heads, size)]
+            self.max_shared = max(self.max_shared, shared)
+            self.min_shared = shared if self.min_shared is None else min(self.min_shared, shared)
+        if not rows:
+            raise ValueError("a plan without rows")
+        if max(rows * num_heads, self.max_shared) >= 1 << 30:
+            raise ValueError(f"{rows} rows of {num_heads} heads, {self.max_shared} shared keys: more than a plan takes")
+        self.rows, self.max_slot = rows, max(slots)
+        self.counts = (len(own), len(wide), len(narrow))
+        words = torch.tensor(own + wide + narrow, dtype=torch.int32).to(device)
+        self.own, self.wide, self.narrow = words.split(self.counts)
+        self.device = words.device
+
+
 _planners: Dict[int, AttentionTilePlanner] = {}
 
 

@@ -42,12 +42,13 @@ def _nvcc() -> str:
 
 #: sources compiled once per head size (-DTIS_HD=<hd>) into libraries of their own
 PER_HEAD_SIZE = ("attention_mma.cu", "attention_tc.cu")
+PER_HEAD_SIZE_SHARED = ("shared_attention.cu",)
 #: sources compiled once per (key width, value width) (-DTIS_KD=<kd> -DTIS_VD=<vd>)
 PER_WIDTHS = ("window_attention_mma.cu", "window_attention_tc.cu", "window_attention_decode.cu")
 
 
 def sources():
-    return sorted(f for f in os.listdir(CSRC) if f.endswith(".cu") and f not in PER_HEAD_SIZE + PER_WIDTHS)
+    return sorted(f for f in os.listdir(CSRC) if f.endswith(".cu") and f not in PER_HEAD_SIZE + PER_HEAD_SIZE_SHARED + PER_WIDTHS)
 
 
 def _digest() -> str:
@@ -122,20 +123,21 @@ def attention_library_path(head_dim: int) -> str:
     return os.path.join(_build_root(), f"libtis_attn_hd{head_dim}_{_digest()}.so")
 
 
-def build_attention(head_dim: int) -> str:
-    """The tensor-core attention kernels for one head size (what a model needs is compiled
-    when the model first runs)."""
+def shared_attention_library_path(head_dim: int) -> str:
+    return os.path.join(_build_root(), f"libtis_shared_attn_hd{head_dim}_{_digest()}.so")
+
+
+def _build_head_size(head_dim: int, out: str, files, what: str) -> str:
     if head_dim % 16 or not (16 <= head_dim <= 256):
         raise BuildError(f"head size {head_dim}: the attention kernels take multiples of 16 from 16 to 256")
-    out = attention_library_path(head_dim)
     if os.path.isfile(out):
         return out
     nvcc = _nvcc()
     root = os.path.dirname(out)
     work = tempfile.mkdtemp(prefix="tis_obj_", dir=root)
     try:
-        _say(f"compiling the attention kernels for head size {head_dim} (first call only)")
-        jobs = [(src, os.path.join(work, src[:-3] + ".o"), (f"-DTIS_HD={head_dim}",)) for src in PER_HEAD_SIZE]
+        _say(f"compiling {what} for head size {head_dim} (first call only)")
+        jobs = [(src, os.path.join(work, src[:-3] + ".o"), (f"-DTIS_HD={head_dim}",)) for src in files]
         jobs.append(("errors.cu", os.path.join(work, "errors.o"), ()))
         with ThreadPoolExecutor(max_workers=len(jobs)) as ex:
             list(ex.map(lambda j: _compile_one(nvcc, *j), jobs))
@@ -147,6 +149,17 @@ def build_attention(head_dim: int) -> str:
     finally:
         shutil.rmtree(work, ignore_errors=True)
     return out
+
+
+def build_attention(head_dim: int) -> str:
+    """The tensor-core attention kernels for one head size (what a model needs is compiled
+    when the model first runs)."""
+    return _build_head_size(head_dim, attention_library_path(head_dim), PER_HEAD_SIZE, "the attention kernels")
+
+
+def build_shared_attention(head_dim: int) -> str:
+    """The kernels of attention over a shared prefix for one head size, a library of their own."""
+    return _build_head_size(head_dim, shared_attention_library_path(head_dim), PER_HEAD_SIZE_SHARED, "attention over a shared prefix")
 
 
 def window_attention_library_path(k_dim: int, v_dim: int) -> str:

@@ -981,6 +981,85 @@ def paged_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Tensor, blo
     return out
 
 
+_shared_attn_libs = {}
+
+
+def shared_attention_library(head_dim: int):
+    """The kernels of attention over a shared prefix for one head size, compiled when first needed."""
+    lib = _shared_attn_libs.get(head_dim)
+    if lib is None:
+        library()
+        lib = ctypes.CDLL(_build.build_shared_attention(head_dim))
+        lib.tis_last_error.restype = ctypes.c_char_p
+        lib.tis_shared_attention.argtypes = [_KINDS[c] for c in "iplplppiiippipiiiiiiifpppp"]
+        if lib.tis_shared_attn_head_dim() != head_dim:
+            raise KernelError(f"attention library built for head size {lib.tis_shared_attn_head_dim()}, wanted {head_dim}")
+        _shared_attn_libs[head_dim] = lib
+    return lib
+
+
+def _shared_parts(tiles: int, keys: int, resident: int) -> int:
+    """Parts that the keys of ``tiles`` CTAs are split into: as many as are resident at a time, of at least 64 keys each."""
+    return max(1, min(-(-keys // 64), resident // max(1, tiles), 64))
+
+
+def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor,
+                            plan, fault: torch.Tensor, max_position: Optional[int] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention of rows whose requests share the first keys and values of the cache (``attention_plan.SharedPrefixPlan``):
+    what ``paged_attention`` computes, with the shared keys read once for all rows of a group instead of once a request.
+
+    ``q`` (>= plan.rows, >= H * hd) has the queries first in each row (row stride free); ``out`` is (>= plan.rows, >= H * hd); ``plane``
+    [pages, 2, KVH, page, hd] is the cache plane that ``rope_kv_write`` fills, ``block_table`` (slots, pages of a request) its tables.
+    The tables of a group's requests name the same pages for the shared keys, as far as they fill whole pages: those keys are read
+    through the first request's table, all others through each request's own.  Row r sees the keys up to ``positions[r]``, which lies
+    at or behind the group's shared keys; a row at an earlier one (a padding row: -1) gets zeros.  Rows behind the plan's are left
+    as they were.
+
+    ``max_position`` (no row's position is larger; the tables' width unless given) decides only how the requests' own keys are split.
+    ``scale`` multiplies the scores (1 / sqrt(hd) unless given).  bfloat16 or float32 (all in 32 bits), any page size, hd a
+    multiple of 16 up to 256.  A page that is not there sets ``fault``, as in ``paged_attention``."""
+    if plane.dim() != 5 or plane.shape[1] != 2 or not plane.is_contiguous():
+        raise KernelError(f"shared_prefix_attention: a cache plane [pages, 2, kv heads, page, head size], not {tuple(plane.shape)}")
+    pages, _, kvh, page, hd = plane.shape
+    h, rows = plan.num_heads, plan.rows
+    dtype = q.dtype
+    if dtype is not plane.dtype or dtype is not out.dtype:
+        raise KernelError(f"shared_prefix_attention: queries {dtype}, cache {plane.dtype}, results {out.dtype}")
+    if kvh != plan.kv_heads or pages < 1 or page < 1 or hd % 16 or not 16 <= hd <= 256:
+        raise KernelError(f"shared_prefix_attention: a plan for {plan.kv_heads} kv heads, a cache plane {tuple(plane.shape)}")
+    if q.dim() != 2 or out.dim() != 2 or q.shape[0] < rows or out.shape[0] < rows or q.shape[1] < h * hd or out.shape[1] < h * hd:
+        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)}, results {tuple(out.shape)} for {rows} rows of {h} heads of {hd}")
+    if q.stride(1) != 1 or out.stride(1) != 1 or (dtype is torch.bfloat16 and (q.stride(0) % 8 or q.data_ptr() % 16)) or plane.data_ptr() % 16:
+        raise KernelError("shared_prefix_attention: rows are contiguous; in bfloat16 queries start on 16 bytes")
+    if (positions.dtype is not torch.int32 or positions.numel() < rows or not positions.is_contiguous() or fault.dtype is not torch.int32
+            or fault.numel() < 1 or block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1
+            or block_table.shape[0] <= plan.max_slot or block_table.shape[1] < 1):
+        raise KernelError(f"shared_prefix_attention: positions {positions.dtype} {tuple(positions.shape)} for {rows} rows, tables "
+                          f"{block_table.dtype} {tuple(block_table.shape)} for slots up to {plan.max_slot}")
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    if not 0 < scale < math.inf:
+        raise KernelError(f"shared_prefix_attention: the scores are multiplied by a positive number, not {scale}")
+    code = _dt(q)
+    _on_this_device("shared_prefix_attention", q, out, plane, block_table, positions, plan.own, fault)
+    lib = shared_attention_library(hd)
+    width = block_table.shape[1]
+    n_own, n_wide, n_narrow = plan.counts
+    wide, n_wide = (plan.narrow, n_narrow) if code == 0 else (plan.wide, n_wide)
+    shared = plan.max_shared // page * page
+    own_keys = max(1, (width * page if max_position is None else max_position + 1) - plan.min_shared // page * page)
+    shared_parts = _shared_parts(n_wide * kvh, shared, 2 * 148) if shared else 0
+    own_parts = _shared_parts(n_own * kvh, own_keys, 2 * 148)
+    parts, row_heads = shared_parts + own_parts, rows * h
+    scratch = torch.empty(parts * row_heads * (hd + 2), dtype=torch.float32, device=q.device)
+    calls["shared_prefix_attention"] += 1
+    at = scratch.data_ptr()
+    _check(lib.tis_shared_attention(code, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), plane.data_ptr(), block_table.data_ptr(),
+                                    block_table.stride(0), width, pages, positions.data_ptr(), plan.own.data_ptr(), n_own, wide.data_ptr(),
+                                    n_wide, own_parts, shared_parts, rows, h, kvh, page, scale, at, at + 4 * parts * row_heads * hd,
+                                    fault.data_ptr(), _stream()), lib)
+    return out
+
+
 def swiglu(gu: torch.Tensor, out: torch.Tensor, block: Optional[int] = None, form: GateForm = SILU) -> torch.Tensor:
     """out[r, j] = gated(gate_j, up_j) in the form ``form`` (silu(gate_j) * up_j unless given) where a row of ``gu`` holds
     gate and up columns in alternating blocks of ``block`` (default: the hidden size, i.e. [all gates | all ups])."""
