@@ -272,9 +272,10 @@ def test_plan():
     plan = SharedPrefixPlan([(40, [(3, 1), (5, 7)]), (0, [(0, 2)])], 12, 4, "cpu")
     assert plan.rows == 10 and plan.max_slot == 5 and plan.max_shared == 40 and plan.min_shared == 0
     assert plan.own.tolist() == [[0, 3, 3, 40], [3, 16, 5, 40], [19, 5, 5, 40], [24, 6, 0, 0]]
-    covered = [a + i for a, n, _, _ in plan.wide.tolist() for i in range(n)]
-    assert covered == list(range(30)) and [t[2:] for t in plan.wide.tolist()] == [[3, 40], [0, 0]]
-    assert sorted(a + i for a, n, _, _ in plan.narrow.tolist() for i in range(n)) == list(range(30))
+    for size, tiles in plan.shared.items():
+        assert [a + i for a, n, _, _ in tiles.tolist() for i in range(n)] == list(range(30))
+        assert all(n <= size for _, n, _, _ in tiles.tolist())
+    assert [x[2:] for x in plan.shared[64].tolist()] == [[3, 40], [0, 0]] and plan.most_heads == 24
     for groups, heads, kvh in (([], 4, 2), ([(0, [])], 4, 2), ([(-1, [(0, 1)])], 4, 2), ([(0, [(0, 0)])], 4, 2), ([(0, [(-1, 1)])], 4, 2),
                                ([(0, [(0, 1), (0, 1)])], 4, 2), ([(0, [(0, 1)])], 4, 3), ([(1 << 30, [(0, 1)])], 4, 2)):
         with pytest.raises(ValueError):

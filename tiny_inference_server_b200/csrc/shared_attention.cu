@@ -2,9 +2,12 @@
 // and pages that the tcgen05 kernel does not take; the float32 kernel; and the kernel that joins the parts.
 //
 // The first is bound by the keys' and values' bytes (a request's own keys serve its own few row heads only) or, with few of them, by the
-// chain position -> page -> row -> product.  Rows of the cache come by cp.async, 64 keys a tile, STAGES tiles ahead, into shared
-// memory as they are stored (their permuted chunks are free of bank conflicts for ldmatrix).  Four warps: with at most 16 row heads each
-// takes a quarter of every tile's keys and they merge at the end; with up to 64 each takes 16 row heads and all keys.
+// chain tile -> positions -> pages -> rows.  64 keys a tile come STAGES tiles ahead into shared memory as they are stored, one bulk copy a page
+// and operand, ordered by the lanes of a warp, a lane a page (rows are dense in a page; their permuted chunks are free of bank
+// conflicts for ldmatrix).  Four warps: with at most 16 row heads each takes a quarter of every tile's keys and they merge at the end; shared
+// tiles of up to 64 or 128 row heads give each warp 16 or 32 of them and all keys, so that an operand of keys or values read from shared
+// memory serves 32.
+#include "tc_common.cuh"
 #include "shared_attention.cuh"
 
 #ifndef TIS_HD
@@ -40,6 +43,12 @@ constexpr int CHUNKS = HD / 8;               // 16-byte pieces of a row
 constexpr int TILE_ELEMENTS = KT * HD;       // keys, or values
 constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 ? 3 : 2);
 constexpr int MMA_THREADS = 128;
+constexpr bool QUERIES_STAY = HD <= 128;     // in registers
+
+__device__ __forceinline__ void bulk_copy(void* to, const void* from, int bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(tc::smem_u32(to)), "l"(from), "r"(bytes), "r"(tc::smem_u32(bar)) : "memory");
+}
 
 // A tile's rows: position of row head rh0 + i (-1: beyond the tile, or before the end of the shared keys: it sees nothing)
 __device__ __forceinline__ int position_of(const SharedParams& p, const SharedTile& t, int i) {
@@ -63,210 +72,276 @@ __device__ __forceinline__ void load_queries(const SharedParams& p, const Shared
     }
 }
 
-// OWN: own tiles (rows end at their positions), else shared ones.  WIDE: 64 row heads, 16 a warp; else 16, a quarter of the keys a warp.
-template <bool OWN, bool WIDE>
+// OWN: own tiles (rows end at their positions), else shared ones.  WR warps side by side over the rows, MT sixteens of row heads each; with
+// WR 1 the warps share out the keys.
+template <bool OWN, int WR, int MT>
 __global__ void __launch_bounds__(MMA_THREADS)
 shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int part0) {
+    constexpr int ROWS = 16 * WR * MT, BLOCKS = WR == 1 ? 1 : KT / 16;      // a warp's sixteens of keys in a tile
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    bf16* q_smem = reinterpret_cast<bf16*>(smem_raw);
-    bf16* ring = q_smem + (WIDE ? 64 : 16) * HD;
-    __shared__ int row_pos[64];
+    bf16* ring = reinterpret_cast<bf16*>(smem_raw);
+    bf16* q_smem = ring + STAGES * 2 * TILE_ELEMENTS;
+    __shared__ int row_pos[ROWS];
     __shared__ float merge_m[4][16], merge_l[4][16];
-    pdl_launch_dependents();
+    __shared__ unsigned long long full[STAGES];
+    __shared__ int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int kvh = blockIdx.x % p.KVH, part = blockIdx.x / p.KVH % parts;
-    const SharedTile t = tiles[blockIdx.x / p.KVH / parts];
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) tc::mbar_init(&full[s], 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    pdl_launch_dependents();
+    const SharedTile t = tiles[blockIdx.x / p.KVH / parts];             // (the plan's, from before the batch)
     const int G = p.H / p.KVH;
     pdl_wait();
 
     const int shared = shared_keys(p, t);
-    int last = shared;                                      // keys [.., last) are seen by some row
-    if (threadIdx.x < (WIDE ? 64 : 32)) {
-        const int pos = threadIdx.x < (WIDE ? 64 : 16) ? position_of(p, t, threadIdx.x) : -1;
-        row_pos[threadIdx.x] = pos;
-    }
+    for (int i = threadIdx.x; i < ROWS; i += MMA_THREADS) row_pos[i] = position_of(p, t, i);
     __syncthreads();
-    int least = 0x7fffffff;                                 // the smallest position of a row that sees anything
-    bool any = false;
-    for (int i = 0; i < (WIDE ? 64 : 16); ++i) {
+    volatile int* abort = &abort_flag;
+    int last = shared, least = 0x7fffffff;                  // keys [.., last) are seen by some row; the smallest position of one that sees any
+    for (int i = lane; i < ROWS; i += 32) {
         const int pos = row_pos[i];
-        if (pos >= 0) { any = true; least = min(least, pos); if (OWN) last = max(last, pos + 1); }
+        if (pos >= 0) { least = min(least, pos); if (OWN) last = max(last, pos + 1); }
     }
+    least = __reduce_min_sync(ALL, least);
+    last = __reduce_max_sync(ALL, last);
     const int base = OWN ? shared & ~(KT - 1) : 0;
     Range keys = part_range(OWN ? shared : 0, last, base, part, parts, KT);
-    if (!any) keys.hi = keys.lo;
+    if (least == 0x7fffffff) keys.hi = keys.lo;
     const int kt0 = keys.lo & ~(KT - 1), count = keys.hi > keys.lo ? (keys.hi - kt0 + KT - 1) / KT : 0;
 
-    load_queries(p, t, kvh, WIDE ? 64 : 16, q_smem);
-    // keys and values of tile j: rows in [lo, hi), zero elsewhere
+    // keys and values of tile j: its rows in [lo, hi), a lane a page
     auto stage = [&](int j) {
-        if (j < count) {
-            bf16* to = ring + (size_t)(j % STAGES) * 2 * TILE_ELEMENTS;
-            for (int i = threadIdx.x; i < KT * CHUNKS; i += MMA_THREADS) {
-                const int r = i / CHUNKS, c = i % CHUNKS, key = kt0 + j * KT + r;
-                const bool in = key >= keys.lo && key < keys.hi;
-                size_t at = 0;
-                if (in) at = (((size_t)page_at(p, t.slot, key / p.page) * 2 * p.KVH + kvh) * p.page + key % p.page) * HD + c * 8;
-                const bf16* k = static_cast<const bf16*>(p.plane) + at;
-                const bf16* v = k + (in ? (size_t)p.KVH * p.page * HD : 0);
-                const int bytes = in ? 16 : 0;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
-                             ::"r"((unsigned)__cvta_generic_to_shared(to + r * HD + c * 8)), "l"(k), "r"(bytes) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
-                             ::"r"((unsigned)__cvta_generic_to_shared(to + TILE_ELEMENTS + r * HD + c * 8)), "l"(v), "r"(bytes) : "memory");
-            }
+        if (warp != 0 || j >= count) return;
+        const int from = max(kt0 + j * KT, keys.lo), to = min(kt0 + (j + 1) * KT, keys.hi);
+        bf16* k = ring + (size_t)(j % STAGES) * 2 * TILE_ELEMENTS;
+        if (lane == 0) tc::mbar_arrive_expect_tx(&full[j % STAGES], (to - from) * HD * 4);
+        __syncwarp();
+        for (int index = from / p.page + lane; index * p.page < to; index += 32) {
+            const int a = max(from, index * p.page), b = min(to, (index + 1) * p.page);
+            const size_t at = (((size_t)page_at(p, t.slot, index) * 2 * p.KVH + kvh) * p.page + (a - index * p.page)) * HD;
+            const bf16* src = static_cast<const bf16*>(p.plane) + at;
+            bf16* dst = k + (a - kt0 - j * KT) * HD;
+            bulk_copy(dst, src, (b - a) * HD * 2, &full[j % STAGES]);
+            bulk_copy(dst + TILE_ELEMENTS, src + (size_t)p.KVH * p.page * HD, (b - a) * HD * 2, &full[j % STAGES]);
         }
-        asm volatile("cp.async.commit_group;\n" ::: "memory");
     };
 #pragma unroll
     for (int j = 0; j < STAGES - 1; ++j) stage(j);
+    load_queries(p, t, kvh, ROWS, q_smem);
+    __syncthreads();
 
-    // this lane's two row heads
-    const int i0 = (WIDE ? warp * 16 : 0) + g, i1 = i0 + 8;
-    float o[HD / 8][4];
+    const int r0 = WR == 1 ? 0 : warp * 16 * MT;            // the warp's first row head
+    int pos[MT][2];
+    float o[MT][HD / 8][4], m[MT][2], l[MT][2];
+    unsigned qf[QUERIES_STAY ? MT : 1][QUERIES_STAY ? HD / 16 : 1][4];
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
+    for (int x = 0; x < MT; ++x) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[x][n][e] = 0.f;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            pos[x][y] = row_pos[r0 + x * 16 + y * 8 + g];
+            m[x][y] = -INFINITY;
+            l[x][y] = 0.f;
+        }
+        if (QUERIES_STAY) {
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                const int qr = r0 + x * 16 + (lane & 15);
+                ldmatrix4(qf[QUERIES_STAY ? x : 0][QUERIES_STAY ? k : 0], q_smem + qr * HD + cache_chunk(2 * k + (lane >> 4), qr, CHUNKS) * 8);
+            }
+        }
+    }
+    bool ok = true;
     for (int j = 0; j < count; ++j) {
-        asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
-        __syncthreads();                                    // tile j is here, tile j - 1's place is free
+        ok = tc::mbar_wait(&full[j % STAGES], (j / STAGES) & 1, abort, p.fault, 6);
+        if (__syncthreads_or(!ok)) { ok = false; break; }   // everyone has tile j, and is done with tile j - 1: its place is free
         stage(j + STAGES - 1);
         const bf16* ks = ring + (size_t)(j % STAGES) * 2 * TILE_ELEMENTS;
         bf16* vs = const_cast<bf16*>(ks) + TILE_ELEMENTS;
         const int kt = kt0 + j * KT;
-        const int pos0 = row_pos[i0], pos1 = row_pos[i1];
-        if (OWN && kt + KT - 1 > least) {
-            // Behind the first row's position a key is seen by some rows and not by others, whose probability of 0 does not take away a
-            // value that is not finite: such values go apart, and zeros into the products.  (Uniform in the CTA.)
-            __shared__ int odd[KT];
-            if (threadIdx.x < KT) odd[threadIdx.x] = 0;
-            __syncthreads();
+        if (kt < keys.lo || kt + KT > keys.hi) {
+            // values of rows that were not copied: nothing that a probability of 0 could not take away
             for (int i = threadIdx.x; i < KT * CHUNKS; i += MMA_THREADS) {
-                const int r = i / CHUNKS, key = kt + r;
-                if (key > least && key < keys.hi) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(vs + r * HD + i % CHUNKS * 8);
-                    const unsigned u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if ((u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u) odd[r] = 1;
-                }
+                const int key = kt + i / CHUNKS;
+                if (key < keys.lo || key >= keys.hi) *reinterpret_cast<uint4*>(vs + i * 8) = make_uint4(0u, 0u, 0u, 0u);
             }
-            __syncthreads();
-            for (int r = 0; r < KT; ++r) {
-                if (!odd[r]) continue;
-                // rows that see it have a result that is not finite there, whatever its probability (a positive number, or 0): the
-                // products of a positive probability say so; a row that does not see it is left alone
-                for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int d = n * 8 + t4 * 2 + (e & 1);
-                        const float v = __bfloat162float(vs[r * HD + cache_chunk(d / 8, kt + r, CHUNKS) * 8 + d % 8]);
-                        const bool sees = kt + r <= (e < 2 ? pos0 : pos1) && (WIDE || warp == 0);
-                        if (sees && !(fabsf(v) < INFINITY)) o[n][e] += v;
-                    }
-            }
-            __syncthreads();
-            for (int i = threadIdx.x; i < KT * CHUNKS; i += MMA_THREADS) {
-                if (!odd[i / CHUNKS]) continue;
-                unsigned short* w = reinterpret_cast<unsigned short*>(vs + i * 8);
-                for (int e = 0; e < 8; ++e)
-                    if ((w[e] & 0x7f80u) == 0x7f80u) w[e] = 0;
-            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncthreads();
         }
+        if (OWN && kt + KT - 1 > least && least < keys.hi - 1) {
+            // Behind the first row's position a key is seen by some rows and not by others, whose probability of 0 does not take away a
+            // value that is not finite: such values go apart, and zeros into the products.  (Uniform in the CTA.)
+            int odd = 0;
+            for (int i = threadIdx.x; i < KT * CHUNKS; i += MMA_THREADS) {
+                const int key = kt + i / CHUNKS;
+                if (key > least && key < keys.hi) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vs + i * 8);
+                    const unsigned u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int b = 0; b < (WIDE ? KT / 16 : 1); ++b) {
-            const int kb = (WIDE ? b : warp) * 16;          // 16 keys of the tile
+                    for (int e = 0; e < 4; ++e) odd |= (u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u;
+                }
+            }
+            if (__syncthreads_or(odd)) {
+                // a row that sees such a value has a result that is not finite there, whatever the probability (a positive number, or 0)
+                for (int key = max(least + 1, kt); key < min(keys.hi, kt + KT) && (WR > 1 || warp == 0); ++key)
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int d = n * 8 + t4 * 2 + (e & 1);
+                            const float v = __bfloat162float(vs[(key - kt) * HD + cache_chunk(d / 8, key, CHUNKS) * 8 + d % 8]);
+#pragma unroll
+                            for (int x = 0; x < MT; ++x)
+                                if (key <= pos[x][e >> 1] && !(fabsf(v) < INFINITY)) o[x][n][e] += v;
+                        }
+                __syncthreads();
+                for (int i = threadIdx.x; i < KT * CHUNKS; i += MMA_THREADS) {
+                    const int key = kt + i / CHUNKS;
+                    if (key <= least || key >= keys.hi) continue;
+                    unsigned short* w = reinterpret_cast<unsigned short*>(vs + i * 8);
+                    for (int e = 0; e < 8; ++e)
+                        if ((w[e] & 0x7f80u) == 0x7f80u) w[e] = 0;
+                }
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncthreads();
+            }
+        }
+#pragma unroll 1
+        for (int b = 0; b < BLOCKS; ++b) {
+            const int kb = (WR == 1 ? warp : b) * 16;       // 16 keys of the tile
             if (kt + kb >= keys.hi || kt + kb + 15 < keys.lo) continue;
-            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            float s[MT][2][4];
+#pragma unroll
+            for (int x = 0; x < MT; ++x)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[x][e >> 2][e & 3] = 0.f;
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {
-                unsigned a[4], bk[4];
-                const int qr = (WIDE ? warp * 16 : 0) + (lane & 15);
-                ldmatrix4(a, q_smem + qr * HD + cache_chunk(2 * k + (lane >> 4), qr, CHUNKS) * 8);
+                unsigned bk[4];
                 const int kr = kb + (lane & 7) + (lane >> 4) * 8;
                 ldmatrix4(bk, ks + kr * HD + cache_chunk(2 * k + ((lane >> 3) & 1), kt + kr, CHUNKS) * 8);
-                mma(s[0], a, bk[0], bk[1]);
-                mma(s[1], a, bk[2], bk[3]);
-            }
-            float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+                for (int x = 0; x < MT; ++x) {
+                    unsigned a[4];
+                    if (QUERIES_STAY) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int key = kt + kb + n * 8 + t4 * 2 + e;
-                    const bool in = key >= keys.lo && key < keys.hi;
-                    s[n][e] = in && (OWN ? key <= pos0 : pos0 >= 0) ? s[n][e] * p.scale_log2 : -INFINITY;
-                    s[n][2 + e] = in && (OWN ? key <= pos1 : pos1 >= 0) ? s[n][2 + e] * p.scale_log2 : -INFINITY;
-                    x0 = fmaxf(x0, s[n][e]);
-                    x1 = fmaxf(x1, s[n][2 + e]);
+                        for (int e = 0; e < 4; ++e) a[e] = qf[QUERIES_STAY ? x : 0][QUERIES_STAY ? k : 0][e];
+                    } else {
+                        const int qr = r0 + x * 16 + (lane & 15);
+                        ldmatrix4(a, q_smem + qr * HD + cache_chunk(2 * k + (lane >> 4), qr, CHUNKS) * 8);
+                    }
+                    mma(s[x][0], a, bk[0], bk[1]);
+                    mma(s[x][1], a, bk[2], bk[3]);
                 }
-            x0 = fmaxf(x0, __shfl_xor_sync(ALL, x0, 1)); x0 = fmaxf(x0, __shfl_xor_sync(ALL, x0, 2));
-            x1 = fmaxf(x1, __shfl_xor_sync(ALL, x1, 1)); x1 = fmaxf(x1, __shfl_xor_sync(ALL, x1, 2));
-            if (__any_sync(ALL, x0 > m0 || x1 > m1)) {
-                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-                const float f0 = m0 == -INFINITY ? 0.f : exp2_fast(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - n1);
-                // (a row without a maximum has no sums yet but what is not finite: that stays)
-                const float r0 = m0 == -INFINITY ? 1.f : f0, r1 = m1 == -INFINITY ? 1.f : f1;
-                l0 *= f0; l1 *= f1;
-#pragma unroll
-                for (int n = 0; n < HD / 8; ++n) { o[n][0] *= r0; o[n][1] *= r0; o[n][2] *= r1; o[n][3] *= r1; }
-                m0 = n0; m1 = n1;
             }
-            const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+            const bool whole = kt + kb >= keys.lo && kt + kb + 15 < keys.hi && (!OWN || kt + kb + 15 <= least);
+            unsigned pa[MT][4];
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int x = 0; x < MT; ++x) {
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    s[n][e] = exp2_fast(s[n][e] - b0);
-                    s[n][2 + e] = exp2_fast(s[n][2 + e] - b1);
-                    l0 += s[n][e];
-                    l1 += s[n][2 + e];
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = kt + kb + n * 8 + t4 * 2 + (e & 1), y = e >> 1;
+                        const bool in = (whole || (key >= keys.lo && key < keys.hi && (!OWN || key <= pos[x][y]))) && pos[x][y] >= 0;
+                        s[x][n][e] = in ? s[x][n][e] * p.scale_log2 : -INFINITY;
+                        top[y] = fmaxf(top[y], s[x][n][e]);
+                    }
+                bool raise = false;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    top[y] = fmaxf(top[y], __shfl_xor_sync(ALL, top[y], 1));
+                    top[y] = fmaxf(top[y], __shfl_xor_sync(ALL, top[y], 2));
+                    raise |= top[y] > m[x][y];
                 }
-            // probabilities in bfloat16 (half a step, 2^-9 of each, at random): the tensor cores' operand; their sum stays in 32 bits
-            const unsigned a[4] = {pack(s[0][0], s[0][1]), pack(s[0][2], s[0][3]), pack(s[1][0], s[1][1]), pack(s[1][2], s[1][3])};
+                if (__any_sync(ALL, raise)) {
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const float up = fmaxf(m[x][y], top[y]);
+                        // (a row without a maximum has no sums yet but what is not finite: that stays)
+                        const float f = m[x][y] == -INFINITY ? 1.f : exp2_fast(m[x][y] - up);
+                        l[x][y] *= f;
+#pragma unroll
+                        for (int n = 0; n < HD / 8; ++n) { o[x][n][2 * y] *= f; o[x][n][2 * y + 1] *= f; }
+                        m[x][y] = up;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int y = e >> 1;
+                        s[x][n][e] = exp2_fast(s[x][n][e] - (m[x][y] == -INFINITY ? 0.f : m[x][y]));
+                        l[x][y] += s[x][n][e];
+                    }
+                // probabilities in bfloat16 (half a step, 2^-9 of each, at random): the tensor cores' operand; their sum stays in 32 bits
+                pa[x][0] = pack(s[x][0][0], s[x][0][1]); pa[x][1] = pack(s[x][0][2], s[x][0][3]);
+                pa[x][2] = pack(s[x][1][0], s[x][1][1]); pa[x][3] = pack(s[x][1][2], s[x][1][3]);
+            }
 #pragma unroll
             for (int n = 0; n < HD / 16; ++n) {
                 unsigned bv[4];
                 const int vr = kb + (lane & 15);
                 ldmatrix4_trans(bv, vs + vr * HD + cache_chunk(2 * n + (lane >> 4), kt + vr, CHUNKS) * 8);
-                mma(o[2 * n], a, bv[0], bv[1]);
-                mma(o[2 * n + 1], a, bv[2], bv[3]);
+#pragma unroll
+                for (int x = 0; x < MT; ++x) {
+                    mma(o[x][2 * n], pa[x], bv[0], bv[1]);
+                    mma(o[x][2 * n + 1], pa[x], bv[2], bv[3]);
+                }
             }
         }
     }
-    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-    l0 += __shfl_xor_sync(ALL, l0, 1); l0 += __shfl_xor_sync(ALL, l0, 2);
-    l1 += __shfl_xor_sync(ALL, l1, 1); l1 += __shfl_xor_sync(ALL, l1, 2);
+    if (!ok) {
+        // a wait ran out: copies that may still be on their way get time to land before the shared memory is given up
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+        return;
+    }
+#pragma unroll
+    for (int x = 0; x < MT; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            l[x][y] += __shfl_xor_sync(ALL, l[x][y], 1);
+            l[x][y] += __shfl_xor_sync(ALL, l[x][y], 2);
+        }
 
     auto place = [&](int i) { const int rh = t.rh0 + i; return ((size_t)(part0 + part) * p.rows + rh / G) * p.H + kvh * G + rh % G; };
-    if (WIDE) {
-        if (i0 < t.count) {
-            const size_t at = place(i0);
-            if (t4 == 0) p.part_ml[at] = make_float2(m0, l0);
+    if (WR > 1) {
 #pragma unroll
-            for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(p.part_o + at * HD + n * 8 + t4 * 2) = make_float2(o[n][0], o[n][1]);
-        }
-        if (i1 < t.count) {
-            const size_t at = place(i1);
-            if (t4 == 0) p.part_ml[at] = make_float2(m1, l1);
+        for (int x = 0; x < MT; ++x)
 #pragma unroll
-            for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(p.part_o + at * HD + n * 8 + t4 * 2) = make_float2(o[n][2], o[n][3]);
-        }
+            for (int y = 0; y < 2; ++y) {
+                const int i = r0 + x * 16 + y * 8 + g;
+                if (i >= t.count) continue;
+                const size_t at = place(i);
+                if (t4 == 0) p.part_ml[at] = make_float2(m[x][y], l[x][y]);
+#pragma unroll
+                for (int n = 0; n < HD / 8; ++n)
+                    *reinterpret_cast<float2*>(p.part_o + at * HD + n * 8 + t4 * 2) = make_float2(o[x][n][2 * y], o[x][n][2 * y + 1]);
+            }
     } else {
         // the four warps' shares: sums relative to the largest maximum, added up in the order of the warps
-        if (t4 == 0) { merge_m[warp][g] = m0; merge_m[warp][g + 8] = m1; merge_l[warp][g] = l0; merge_l[warp][g + 8] = l1; }
-        __syncthreads();                                    // (the last tile has been read, too)
-        float* merge_o = reinterpret_cast<float*>(ring);    // [warp][row][HD]
-        const float M0 = fmaxf(fmaxf(merge_m[0][g], merge_m[1][g]), fmaxf(merge_m[2][g], merge_m[3][g]));
-        const float M1 = fmaxf(fmaxf(merge_m[0][g + 8], merge_m[1][g + 8]), fmaxf(merge_m[2][g + 8], merge_m[3][g + 8]));
-        const float w0 = m0 == -INFINITY ? 1.f : exp2_fast(m0 - M0), w1 = m1 == -INFINITY ? 1.f : exp2_fast(m1 - M1);
+        float* merge_o = reinterpret_cast<float*>(ring);    // [warp][row][HD]: every copy has landed, every tile been read
+        if (t4 == 0) {
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n) {
-            *reinterpret_cast<float2*>(merge_o + (size_t)(warp * 16 + g) * HD + n * 8 + t4 * 2) = make_float2(o[n][0] * w0, o[n][1] * w0);
-            *reinterpret_cast<float2*>(merge_o + (size_t)(warp * 16 + g + 8) * HD + n * 8 + t4 * 2) = make_float2(o[n][2] * w1, o[n][3] * w1);
+            for (int y = 0; y < 2; ++y) { merge_m[warp][g + 8 * y] = m[0][y]; merge_l[warp][g + 8 * y] = l[0][y]; }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const int r = g + 8 * y;
+            const float M = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
+            const float f = m[0][y] == -INFINITY ? 1.f : exp2_fast(m[0][y] - M);
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n)
+                *reinterpret_cast<float2*>(merge_o + (size_t)(warp * 16 + r) * HD + n * 8 + t4 * 2) = make_float2(o[0][n][2 * y] * f, o[0][n][2 * y + 1] * f);
         }
         __syncthreads();
         for (int i = threadIdx.x; i < 16 * HD; i += MMA_THREADS) {
@@ -277,10 +352,10 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
         if (threadIdx.x < 16 && (int)threadIdx.x < t.count) {
             const int r = threadIdx.x;
             const float M = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
-            float l = 0.f;
+            float sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) l += merge_m[w][r] == -INFINITY ? merge_l[w][r] : merge_l[w][r] * exp2_fast(merge_m[w][r] - M);
-            p.part_ml[place(r)] = make_float2(M, l);
+            for (int w = 0; w < 4; ++w) sum += merge_m[w][r] == -INFINITY ? merge_l[w][r] : merge_l[w][r] * exp2_fast(merge_m[w][r] - M);
+            p.part_ml[place(r)] = make_float2(M, sum);
         }
     }
 }
@@ -436,26 +511,29 @@ shared_join_kernel(const SharedParams p, T* out, long long ldo, int row_heads, i
         if (lane + e * 32 < HD) dst[lane + e * 32] = from_f32<T>(l == 0.f ? 0.f : o[e] / l);
 }
 
-template <bool OWN, bool WIDE> int launch_mma(const SharedParams& p, const SharedTile* tiles, int count, int parts, int part0, cudaStream_t stream) {
-    const int ring = STAGES * 2 * TILE_ELEMENTS * 2, merge = 4 * 16 * HD * 4;
-    const size_t smem = (size_t)(WIDE ? 64 : 16) * HD * 2 + (ring > merge ? ring : merge);
+template <bool OWN, int WR, int MT> int launch_mma(const SharedParams& p, const SharedTile* tiles, int count, int parts, int part0, cudaStream_t stream) {
+    const size_t smem = (size_t)STAGES * 2 * TILE_ELEMENTS * 2 + (size_t)16 * WR * MT * HD * 2;      // (the ring is larger than four warps' shares)
+    static_assert(STAGES * 2 * TILE_ELEMENTS * 2 >= 4 * 16 * HD * 4, "merge");
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(shared_mma_kernel<OWN, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    if (configured.first() && cudaFuncSetAttribute(shared_mma_kernel<OWN, WR, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return tis_check_launch("shared_prefix_attention (shared memory)");
-    tis_launch(shared_mma_kernel<OWN, WIDE>, dim3((unsigned)(count * parts * p.KVH)), dim3(MMA_THREADS), smem, stream, p, tiles, parts, part0);
+    tis_launch(shared_mma_kernel<OWN, WR, MT>, dim3((unsigned)(count * parts * p.KVH)), dim3(MMA_THREADS), smem, stream, p, tiles, parts, part0);
     return tis_check_launch("shared_prefix_attention");
 }
 
 }  // namespace
 
 TIS_API int tis_shared_attn_head_dim() { return HD; }
+// the most row heads of a shared tile: 128, or 64 where a warp's share of 32 does not fit its registers
+TIS_API int tis_shared_attn_widest() { return HD <= 128 ? 128 : 64; }
 
-// `own`, `wide`: tiles on the device, own ones of up to 16 row heads, shared ones of up to 64 (bfloat16) or 16 (float32) row heads.
+// `own`, `wide`: tiles on the device, own ones of up to 16 row heads, shared ones of up to `wide_rows`: 16, and in bfloat16
+// 64 or 128 (tis_shared_attn_widest).
 // The first `shared_parts` parts of the scratch are the shared tiles', the `own_parts` behind them the own ones'; rows of groups
 // without shared keys have empty ones.  `rows`: the rows of the plan, all of which are written.
 TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* out, long long ldo, const void* plane, const int* table,
                                  int table_stride, int table_width, int num_pages, const int* positions, const void* own, int own_count,
-                                 const void* wide, int wide_count, int own_parts, int shared_parts, int rows, int H, int KVH, int page,
+                                 const void* wide, int wide_count, int wide_rows, int own_parts, int shared_parts, int rows, int H, int KVH, int page,
                                  float scale, float* part_o, void* part_ml, int* fault, cudaStream_t stream) {
     if (rows <= 0) return TIS_OK;
     SharedParams p;
@@ -466,6 +544,10 @@ TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* 
     p.rows = rows; p.H = H; p.KVH = KVH; p.page = page; p.own_parts = own_parts; p.shared_parts = shared_parts;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.fault = fault;
+    if (wide_rows != 16 && (dtype == TIS_F32 || wide_rows > tis_shared_attn_widest() || (wide_rows != 64 && wide_rows != 128))) {
+        tis_set_error("shared_prefix_attention: shared tiles of %d row heads", wide_rows);
+        return TIS_BAD_SIZE;
+    }
     const SharedTile* o = static_cast<const SharedTile*>(own);
     const SharedTile* w = static_cast<const SharedTile*>(wide);
     const int parts = own_parts + shared_parts, row_heads = rows * H;
@@ -480,8 +562,12 @@ TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* 
             status = tis_check_launch("shared_prefix_attention");
         }
     } else if (dtype == TIS_BF16) {
-        if (shared_parts > 0) status = launch_mma<false, true>(p, w, wide_count, shared_parts, 0, stream);
-        if (status == TIS_OK) status = launch_mma<true, false>(p, o, own_count, own_parts, shared_parts, stream);
+        if (shared_parts > 0) {
+            if (wide_rows == 16) status = launch_mma<false, 1, 1>(p, w, wide_count, shared_parts, 0, stream);
+            else if (wide_rows == 64) status = launch_mma<false, 4, 1>(p, w, wide_count, shared_parts, 0, stream);
+            else status = launch_mma<false, 4, HD <= 128 ? 2 : 1>(p, w, wide_count, shared_parts, 0, stream);
+        }
+        if (status == TIS_OK) status = launch_mma<true, 1, 1>(p, o, own_count, own_parts, shared_parts, stream);
     } else {
         tis_set_error("shared_prefix_attention: dtype code %d", dtype);
         return TIS_BAD_DTYPE;

@@ -103,17 +103,18 @@ class SharedPrefixPlan:
     made once for a batch and holds as long as its requests, rows and shared keys do; the rows' positions are not part of it.
 
     Tiles are counted in row heads: (row, query head) of a kv head, the G heads of a row one after another.  ``own``: up to OWN_TILE of one
-    request; ``wide`` (``narrow``): up to WIDE_TILE (OWN_TILE) of one group.  Each is (first row head, row heads, slot, shared keys),
-    int32 on the device; a group's keys are read through the table of its first request."""
+    request; ``shared[size]``: up to ``size`` of one group, for the sizes that the kernels know.  Each is (first row head, row heads, slot,
+    shared keys), int32 on the device; a group's keys are read through the table of its first request."""
 
-    OWN_TILE, WIDE_TILE = 16, 64
+    OWN_TILE, SHARED_TILES = 16, (16, 64, 128)
 
     def __init__(self, groups: Sequence[Tuple[int, Sequence[Tuple[int, int]]]], num_heads: int, kv_heads: int, device="cuda"):
         if kv_heads <= 0 or num_heads <= 0 or num_heads % kv_heads:
             raise ValueError(f"{num_heads} query heads are not a multiple of {kv_heads} kv heads")
         self.num_heads, self.kv_heads, self.group_size = num_heads, kv_heads, num_heads // kv_heads
         g = self.group_size
-        own, wide, narrow = [], [], []
+        own, shared_tiles = [], {size: [] for size in self.SHARED_TILES}
+        self.most_heads = 0                                   # row heads of the largest group
         rows, self.max_slot, self.max_shared, self.min_shared, slots = 0, -1, 0, None, set()
         for shared, requests in groups:
             if shared < 0 or not requests:
@@ -126,7 +127,8 @@ class SharedPrefixPlan:
                 own += [(rows * g + a, min(self.OWN_TILE, n * g - a), slot, shared) for a in range(0, n * g, self.OWN_TILE)]
                 rows += n
             heads = (rows - first) * g
-            for tiles, size in ((wide, self.WIDE_TILE), (narrow, self.OWN_TILE)):
+            self.most_heads = max(self.most_heads, heads)
+            for size, tiles in shared_tiles.items():
                 tiles += [(first * g + a, min(size, heads - a), requests[0][0], shared) for a in range(0, heads, size)]
             self.max_shared = max(self.max_shared, shared)
             self.min_shared = shared if self.min_shared is None else min(self.min_shared, shared)
@@ -135,9 +137,10 @@ class SharedPrefixPlan:
         if max(rows * num_heads, self.max_shared) >= 1 << 30:
             raise ValueError(f"{rows} rows of {num_heads} heads, {self.max_shared} shared keys: more than a plan takes")
         self.rows, self.max_slot = rows, max(slots)
-        self.counts = (len(own), len(wide), len(narrow))
-        words = torch.tensor(own + wide + narrow, dtype=torch.int32).to(device)
-        self.own, self.wide, self.narrow = words.split(self.counts)
+        parts = [own, *shared_tiles.values()]
+        words = torch.tensor(sum(parts, []), dtype=torch.int32).to(device)
+        self.own, *shared_words = words.split([len(p) for p in parts])
+        self.shared = dict(zip(self.SHARED_TILES, shared_words))
         self.device = words.device
 
 

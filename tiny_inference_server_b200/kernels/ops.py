@@ -991,7 +991,8 @@ def shared_attention_library(head_dim: int):
         library()
         lib = ctypes.CDLL(_build.build_shared_attention(head_dim))
         lib.tis_last_error.restype = ctypes.c_char_p
-        lib.tis_shared_attention.argtypes = [_KINDS[c] for c in "iplplppiiippipiiiiiiifpppp"]
+        lib.tis_shared_attention.argtypes = [_KINDS[c] for c in "iplplppiiippipiiiiiiiifpppp"]
+        lib.widest = lib.tis_shared_attn_widest()
         if lib.tis_shared_attn_head_dim() != head_dim:
             raise KernelError(f"attention library built for head size {lib.tis_shared_attn_head_dim()}, wanted {head_dim}")
         _shared_attn_libs[head_dim] = lib
@@ -1043,8 +1044,10 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     _on_this_device("shared_prefix_attention", q, out, plane, block_table, positions, plan.own, fault)
     lib = shared_attention_library(hd)
     width = block_table.shape[1]
-    n_own, n_wide, n_narrow = plan.counts
-    wide, n_wide = (plan.narrow, n_narrow) if code == 0 else (plan.wide, n_wide)
+    # shared tiles of the row heads that the groups have, as far as the kernels go
+    wide_rows = 16 if code == 0 or plan.most_heads <= 16 else (64 if plan.most_heads <= 64 else lib.widest)
+    wide = plan.shared[wide_rows]
+    n_own, n_wide = plan.own.shape[0], wide.shape[0]
     shared = plan.max_shared // page * page
     own_keys = max(1, (width * page if max_position is None else max_position + 1) - plan.min_shared // page * page)
     shared_parts = _shared_parts(n_wide * kvh, shared, 2 * 148) if shared else 0
@@ -1055,7 +1058,7 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     at = scratch.data_ptr()
     _check(lib.tis_shared_attention(code, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), plane.data_ptr(), block_table.data_ptr(),
                                     block_table.stride(0), width, pages, positions.data_ptr(), plan.own.data_ptr(), n_own, wide.data_ptr(),
-                                    n_wide, own_parts, shared_parts, rows, h, kvh, page, scale, at, at + 4 * parts * row_heads * hd,
+                                    n_wide, wide_rows, own_parts, shared_parts, rows, h, kvh, page, scale, at, at + 4 * parts * row_heads * hd,
                                     fault.data_ptr(), _stream()), lib)
     return out
 
