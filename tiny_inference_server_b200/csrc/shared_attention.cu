@@ -20,6 +20,7 @@ using namespace shared_attention;
 
 constexpr int HD = TIS_HD;
 constexpr unsigned ALL = 0xffffffffu;
+constexpr int MAX_PARTS = 128;
 
 __device__ __forceinline__ void ldmatrix4(unsigned (&r)[4], const void* smem) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
@@ -80,7 +81,8 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
     constexpr int ROWS = 16 * WR * MT, BLOCKS = WR == 1 ? 1 : KT / 16;      // a warp's sixteens of keys in a tile
     extern __shared__ __align__(128) unsigned char smem_raw[];
     bf16* ring = reinterpret_cast<bf16*>(smem_raw);
-    bf16* q_smem = ring + STAGES * 2 * TILE_ELEMENTS;
+    // the queries lie where the last stage's first tile comes to, where they only pass through
+    bf16* q_smem = ring + (QUERIES_STAY ? STAGES - 1 : STAGES) * 2 * TILE_ELEMENTS;
     __shared__ int row_pos[ROWS];
     __shared__ float merge_m[4][16], merge_l[4][16];
     __shared__ unsigned long long full[STAGES];
@@ -158,6 +160,7 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
             }
         }
     }
+    if (QUERIES_STAY) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     bool ok = true;
     for (int j = 0; j < count; ++j) {
         ok = tc::mbar_wait(&full[j % STAGES], (j / STAGES) & 1, abort, p.fault, 6);
@@ -480,40 +483,79 @@ shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
     }
 }
 
-// ---- the parts of a row head joined: a warp each -------------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(256)
+// ---- the parts of a row head joined ------------------------------------------------------------------------------------------
+// W warps a row head share the parts out and meet in shared memory; each has the loads of several parts on their way.
+constexpr int JOIN_THREADS = 128, JOIN_AHEAD = 8;
+template <typename T, int W>
+__global__ void __launch_bounds__(JOIN_THREADS)
 shared_join_kernel(const SharedParams p, T* out, long long ldo, int row_heads, int parts) {
+    constexpr int HEADS = JOIN_THREADS / 32 / W;            // row heads of a CTA
+    __shared__ float2 ml[HEADS][MAX_PARTS];
+    __shared__ float shares[HEADS][W][HD + 1];
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const int i = blockIdx.x * 8 + (threadIdx.x >> 5);      // row, head
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp / W, w = warp % W;
+    const int i = min((int)blockIdx.x * HEADS + mine, row_heads - 1);      // row, head (the last one again beyond the end)
     pdl_wait();
-    if (i >= row_heads) return;
-    const int row = i / p.H, head = i % p.H;
+    for (int q = w * 32 + lane; q < parts; q += W * 32) ml[mine][q] = p.part_ml[(size_t)q * row_heads + i];
+    __syncthreads();
     float M = -INFINITY;
-    for (int q = 0; q < parts; ++q) M = fmaxf(M, p.part_ml[(size_t)q * row_heads + i].x);
+    for (int q = lane; q < parts; q += 32) M = fmaxf(M, ml[mine][q].x);
+#pragma unroll
+    for (int e = 16; e > 0; e >>= 1) M = fmaxf(M, __shfl_xor_sync(ALL, M, e));
     float l = 0.f, o[F32_LANES];
 #pragma unroll
     for (int e = 0; e < F32_LANES; ++e) o[e] = 0.f;
-    for (int q = 0; q < parts; ++q) {
-        const float2 ml = p.part_ml[(size_t)q * row_heads + i];
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;     // no keys
-        const float f = ml.x == -INFINITY ? 1.f : exp2f(ml.x - M);
-        l += ml.y * f;
-        const float* src = p.part_o + ((size_t)q * row_heads + i) * HD;
+    for (int q0 = w; q0 < parts; q0 += W * JOIN_AHEAD) {
+        float x[JOIN_AHEAD][F32_LANES], f[JOIN_AHEAD];
+#pragma unroll
+        for (int a = 0; a < JOIN_AHEAD; ++a) {
+            const int q = q0 + a * W;
+            const float2 v = q < parts ? ml[mine][q] : make_float2(-INFINITY, 0.f);
+            const bool some = !(v.x == -INFINITY && v.y == 0.f);        // (else no keys: nothing was left there)
+            f[a] = v.x == -INFINITY ? 1.f : exp2f(v.x - M);
+            l += v.y * f[a];
+            const float* src = p.part_o + ((size_t)q * row_heads + i) * HD;
+#pragma unroll
+            for (int e = 0; e < F32_LANES; ++e) x[a][e] = some && lane + e * 32 < HD ? src[lane + e * 32] : 0.f;
+        }
+#pragma unroll
+        for (int a = 0; a < JOIN_AHEAD; ++a)
+#pragma unroll
+            for (int e = 0; e < F32_LANES; ++e) o[e] = fmaf(x[a][e], f[a], o[e]);
+    }
+    if (W > 1) {
 #pragma unroll
         for (int e = 0; e < F32_LANES; ++e)
-            if (lane + e * 32 < HD) o[e] = fmaf(src[lane + e * 32], f, o[e]);
+            if (lane + e * 32 < HD) shares[mine][w][lane + e * 32] = o[e];
+        if (lane == 0) shares[mine][w][HD] = l;
+        __syncthreads();
+        if (w != 0) return;
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < F32_LANES; ++e) o[e] = 0.f;
+        for (int a = 0; a < W; ++a) {
+            l += shares[mine][a][HD];
+#pragma unroll
+            for (int e = 0; e < F32_LANES; ++e)
+                if (lane + e * 32 < HD) o[e] += shares[mine][a][lane + e * 32];
+        }
     }
-    T* dst = out + (long long)row * ldo + head * HD;
+    if ((int)blockIdx.x * HEADS + mine >= row_heads) return;
+    T* dst = out + (long long)(i / p.H) * ldo + i % p.H * HD;
 #pragma unroll
     for (int e = 0; e < F32_LANES; ++e)
         if (lane + e * 32 < HD) dst[lane + e * 32] = from_f32<T>(l == 0.f ? 0.f : o[e] / l);
 }
+template <typename T> int launch_join(const SharedParams& p, void* out, long long ldo, int row_heads, int parts, cudaStream_t stream) {
+    if (parts > 4) tis_launch(shared_join_kernel<T, 4>, dim3((unsigned)row_heads), dim3(JOIN_THREADS), 0, stream, p, static_cast<T*>(out), ldo, row_heads, parts);
+    else tis_launch(shared_join_kernel<T, 1>, dim3((unsigned)((row_heads + 3) / 4)), dim3(JOIN_THREADS), 0, stream, p, static_cast<T*>(out), ldo, row_heads, parts);
+    return tis_check_launch("shared_prefix_attention (join)");
+}
 
 template <bool OWN, int WR, int MT> int launch_mma(const SharedParams& p, const SharedTile* tiles, int count, int parts, int part0, cudaStream_t stream) {
-    const size_t smem = (size_t)STAGES * 2 * TILE_ELEMENTS * 2 + (size_t)16 * WR * MT * HD * 2;      // (the ring is larger than four warps' shares)
-    static_assert(STAGES * 2 * TILE_ELEMENTS * 2 >= 4 * 16 * HD * 4, "merge");
+    const size_t smem = (size_t)STAGES * 2 * TILE_ELEMENTS * 2 + (QUERIES_STAY ? 0 : (size_t)16 * WR * MT * HD * 2);
+    static_assert(STAGES * 2 * TILE_ELEMENTS * 2 >= 4 * 16 * HD * 4, "four warps' shares fit the ring");
+    static_assert(2 * TILE_ELEMENTS >= 16 * WR * MT * HD, "the queries fit a stage");
     static DeviceOnce configured;
     if (configured.first() && cudaFuncSetAttribute(shared_mma_kernel<OWN, WR, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return tis_check_launch("shared_prefix_attention (shared memory)");
@@ -523,17 +565,22 @@ template <bool OWN, int WR, int MT> int launch_mma(const SharedParams& p, const 
 
 }  // namespace
 
+// shared_attention_tc.cu
+bool shared_tc_takes(int page);
+int shared_tc_launch(const SharedParams& p, const SharedTile* tiles, int count, int parts, cudaStream_t stream);
+
 TIS_API int tis_shared_attn_head_dim() { return HD; }
 // the most row heads of a shared tile: 128, or 64 where a warp's share of 32 does not fit its registers
 TIS_API int tis_shared_attn_widest() { return HD <= 128 ? 128 : 64; }
 
 // `own`, `wide`: tiles on the device, own ones of up to 16 row heads, shared ones of up to `wide_rows`: 16, and in bfloat16
-// 64 or 128 (tis_shared_attn_widest).
+// 64 or 128 (tis_shared_attn_widest); `tensor`: shared tiles by the tcgen05 kernel, which takes up to 128.
 // The first `shared_parts` parts of the scratch are the shared tiles', the `own_parts` behind them the own ones'; rows of groups
 // without shared keys have empty ones.  `rows`: the rows of the plan, all of which are written.
+TIS_API int tis_shared_attn_tensor(int page) { return shared_tc_takes(page); }
 TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* out, long long ldo, const void* plane, const int* table,
                                  int table_stride, int table_width, int num_pages, const int* positions, const void* own, int own_count,
-                                 const void* wide, int wide_count, int wide_rows, int own_parts, int shared_parts, int rows, int H, int KVH, int page,
+                                 const void* wide, int wide_count, int wide_rows, int tensor, int own_parts, int shared_parts, int rows, int H, int KVH, int page,
                                  float scale, float* part_o, void* part_ml, int* fault, cudaStream_t stream) {
     if (rows <= 0) return TIS_OK;
     SharedParams p;
@@ -546,6 +593,10 @@ TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* 
     p.fault = fault;
     if (wide_rows != 16 && (dtype == TIS_F32 || wide_rows > tis_shared_attn_widest() || (wide_rows != 64 && wide_rows != 128))) {
         tis_set_error("shared_prefix_attention: shared tiles of %d row heads", wide_rows);
+        return TIS_BAD_SIZE;
+    }
+    if (own_parts < 1 || shared_parts < 0 || own_parts + shared_parts > MAX_PARTS || (tensor && !(dtype == TIS_BF16 && shared_tc_takes(page) && 2ll * num_pages * KVH * page < 1ll << 31))) {
+        tis_set_error("shared_prefix_attention: %d and %d parts, pages of %d", own_parts, shared_parts, page);
         return TIS_BAD_SIZE;
     }
     const SharedTile* o = static_cast<const SharedTile*>(own);
@@ -563,7 +614,8 @@ TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* 
         }
     } else if (dtype == TIS_BF16) {
         if (shared_parts > 0) {
-            if (wide_rows == 16) status = launch_mma<false, 1, 1>(p, w, wide_count, shared_parts, 0, stream);
+            if (tensor) status = shared_tc_launch(p, w, wide_count, shared_parts, stream);
+            else if (wide_rows == 16) status = launch_mma<false, 1, 1>(p, w, wide_count, shared_parts, 0, stream);
             else if (wide_rows == 64) status = launch_mma<false, 4, 1>(p, w, wide_count, shared_parts, 0, stream);
             else status = launch_mma<false, 4, HD <= 128 ? 2 : 1>(p, w, wide_count, shared_parts, 0, stream);
         }
@@ -573,7 +625,5 @@ TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* 
         return TIS_BAD_DTYPE;
     }
     if (status != TIS_OK) return status;
-    if (dtype == TIS_F32) tis_launch(shared_join_kernel<float>, dim3((unsigned)((row_heads + 7) / 8)), dim3(256), 0, stream, p, static_cast<float*>(out), ldo, row_heads, parts);
-    else tis_launch(shared_join_kernel<bf16>, dim3((unsigned)((row_heads + 7) / 8)), dim3(256), 0, stream, p, static_cast<bf16*>(out), ldo, row_heads, parts);
-    return tis_check_launch("shared_prefix_attention");
+    return dtype == TIS_F32 ? launch_join<float>(p, out, ldo, row_heads, parts, stream) : launch_join<bf16>(p, out, ldo, row_heads, parts, stream);
 }

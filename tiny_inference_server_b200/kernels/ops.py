@@ -991,7 +991,7 @@ def shared_attention_library(head_dim: int):
         library()
         lib = ctypes.CDLL(_build.build_shared_attention(head_dim))
         lib.tis_last_error.restype = ctypes.c_char_p
-        lib.tis_shared_attention.argtypes = [_KINDS[c] for c in "iplplppiiippipiiiiiiiifpppp"]
+        lib.tis_shared_attention.argtypes = [_KINDS[c] for c in "iplplppiiippipiiiiiiiiifpppp"]
         lib.widest = lib.tis_shared_attn_widest()
         if lib.tis_shared_attn_head_dim() != head_dim:
             raise KernelError(f"attention library built for head size {lib.tis_shared_attn_head_dim()}, wanted {head_dim}")
@@ -1002,6 +1002,20 @@ def shared_attention_library(head_dim: int):
 def _shared_parts(tiles: int, keys: int, resident: int) -> int:
     """Parts that the keys of ``tiles`` CTAs are split into: as many as are resident at a time, of at least 64 keys each."""
     return max(1, min(-(-keys // 64), resident // max(1, tiles), 64))
+
+
+def _split_parts(items: int, tiles: int, resident: int) -> int:
+    """Parts of the shared keys' ``tiles``, for ``items`` (row heads, kv head) of CTAs of which ``resident`` run at a time: the fewest rounds
+    of the longest part, a CTA costing four tiles to start and finish and a part a tenth of one to join."""
+    best, cost = 1, None
+    for parts in range(1, min(tiles, 64) + 1):
+        per = -(-tiles // parts)
+        if -(-tiles // per) != parts:
+            continue
+        c = -(-items * parts // resident) * (per + 4) + 0.1 * parts
+        if cost is None or c < cost - 1e-9:
+            best, cost = parts, c
+    return best
 
 
 def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor,
@@ -1045,12 +1059,13 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     lib = shared_attention_library(hd)
     width = block_table.shape[1]
     # shared tiles of the row heads that the groups have, as far as the kernels go
-    wide_rows = 16 if code == 0 or plan.most_heads <= 16 else (64 if plan.most_heads <= 64 else lib.widest)
+    tensor = int(code == 1 and TC_ATTENTION and lib.tis_shared_attn_tensor(page) and 2 * pages * kvh * page < 1 << 31)
+    wide_rows = 128 if tensor else (16 if code == 0 or plan.most_heads <= 16 else (64 if plan.most_heads <= 64 else lib.widest))
     wide = plan.shared[wide_rows]
     n_own, n_wide = plan.own.shape[0], wide.shape[0]
     shared = plan.max_shared // page * page
     own_keys = max(1, (width * page if max_position is None else max_position + 1) - plan.min_shared // page * page)
-    shared_parts = _shared_parts(n_wide * kvh, shared, 2 * 148) if shared else 0
+    shared_parts = (_split_parts(n_wide * kvh, -(-shared // 128), 148) if tensor else _shared_parts(n_wide * kvh, shared, 2 * 148)) if shared else 0
     own_parts = _shared_parts(n_own * kvh, own_keys, 2 * 148)
     parts, row_heads = shared_parts + own_parts, rows * h
     scratch = torch.empty(parts * row_heads * (hd + 2), dtype=torch.float32, device=q.device)
@@ -1058,7 +1073,7 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     at = scratch.data_ptr()
     _check(lib.tis_shared_attention(code, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), plane.data_ptr(), block_table.data_ptr(),
                                     block_table.stride(0), width, pages, positions.data_ptr(), plan.own.data_ptr(), n_own, wide.data_ptr(),
-                                    n_wide, wide_rows, own_parts, shared_parts, rows, h, kvh, page, scale, at, at + 4 * parts * row_heads * hd,
+                                    n_wide, wide_rows, tensor, own_parts, shared_parts, rows, h, kvh, page, scale, at, at + 4 * parts * row_heads * hd,
                                     fault.data_ptr(), _stream()), lib)
     return out
 
