@@ -42,8 +42,8 @@ __device__ __forceinline__ unsigned pack(float a, float b) {
 constexpr int KT = 64;                       // keys of a tile
 constexpr int CHUNKS = HD / 8;               // 16-byte pieces of a row
 constexpr int TILE_ELEMENTS = KT * HD;       // keys, or values
-constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 ? 3 : 2);
-constexpr int MMA_THREADS = 128;
+constexpr int STAGES = HD <= 64 ? 4 : (HD <= 96 ? 3 : 2);
+constexpr int MMA_THREADS = 128, LOAD_THREADS = 32;      // four warps compute, one orders copies
 constexpr bool QUERIES_STAY = HD <= 128;     // in registers
 
 __device__ __forceinline__ void bulk_copy(void* to, const void* from, int bytes, unsigned long long* bar) {
@@ -58,84 +58,117 @@ __device__ __forceinline__ int position_of(const SharedParams& p, const SharedTi
     return pos >= t.prefix ? pos : -1;
 }
 
-// Q row heads rh0 .. rh0 + n - 1 of kv head `kvh` into shared memory, rows of HD, chunk c of row i at c XOR / + i as a cache row
-// of position i; zero beyond the tile.
-__device__ __forceinline__ void load_queries(const SharedParams& p, const SharedTile& t, int kvh, int n, bf16* to) {
-    const int G = p.H / p.KVH;
-    for (int j = threadIdx.x; j < n * CHUNKS; j += MMA_THREADS) {
-        const int i = j / CHUNKS, c = j % CHUNKS;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (i < t.count) {
-            const int rh = t.rh0 + i, row = rh / G;
-            v = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + (long long)row * p.ldq + (kvh * G + rh % G) * HD + c * 8);
-        }
-        *reinterpret_cast<uint4*>(to + i * HD + cache_chunk(c, i, CHUNKS) * 8) = v;
-    }
-}
+// What the loading warp tells the others of an item (a tile, a kv head and a part).
+struct Item { int rh0, count, kvh, part, lo, hi, least; };
 
 // OWN: own tiles (rows end at their positions), else shared ones.  WR warps side by side over the rows, MT sixteens of row heads each; with
-// WR 1 the warps share out the keys.
+// WR 1 the warps share out the keys.  A CTA goes through the items blockIdx.x, + gridDim.x, ..; the loading warp is ahead by the
+// ring, and by an item's queries and positions, so that the next item's chain of loads runs under this one's work.
 template <bool OWN, int WR, int MT>
-__global__ void __launch_bounds__(MMA_THREADS)
-shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int part0) {
+__global__ void __launch_bounds__(MMA_THREADS + LOAD_THREADS)
+shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int parts, int part0, int beside) {
     constexpr int ROWS = 16 * WR * MT, BLOCKS = WR == 1 ? 1 : KT / 16;      // a warp's sixteens of keys in a tile
+    constexpr int SLOTS = WR == 1 ? 2 : 1;                  // items whose queries are here
     extern __shared__ __align__(128) unsigned char smem_raw[];
     bf16* ring = reinterpret_cast<bf16*>(smem_raw);
-    // the queries lie where the last stage's first tile comes to, where they only pass through
-    bf16* q_smem = ring + (QUERIES_STAY ? STAGES - 1 : STAGES) * 2 * TILE_ELEMENTS;
-    __shared__ int row_pos[ROWS];
+    bf16* q_smem = ring + STAGES * 2 * TILE_ELEMENTS;       // [slot][row head][HD], dense
+    float* merge_o = reinterpret_cast<float*>(q_smem + SLOTS * ROWS * HD);      // WR 1: [two warps][row head][HD]
+    __shared__ int row_pos[SLOTS][ROWS];
+    __shared__ Item item_of[SLOTS];
     __shared__ float merge_m[4][16], merge_l[4][16];
-    __shared__ unsigned long long full[STAGES];
+    __shared__ unsigned long long full[STAGES], empty[STAGES], q_full[SLOTS], q_empty[SLOTS];
     __shared__ int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int kvh = blockIdx.x % p.KVH, part = blockIdx.x / p.KVH % parts;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) tc::mbar_init(&full[s], 1);
+        for (int s = 0; s < STAGES; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 4); }
+        for (int s = 0; s < SLOTS; ++s) { tc::mbar_init(&q_full[s], 1); tc::mbar_init(&q_empty[s], 4); }
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    pdl_launch_dependents();
-    const SharedTile t = tiles[blockIdx.x / p.KVH / parts];             // (the plan's, from before the batch)
-    const int G = p.H / p.KVH;
-    pdl_wait();
-
-    const int shared = shared_keys(p, t);
-    for (int i = threadIdx.x; i < ROWS; i += MMA_THREADS) row_pos[i] = position_of(p, t, i);
     __syncthreads();
     volatile int* abort = &abort_flag;
-    int last = shared, least = 0x7fffffff;                  // keys [.., last) are seen by some row; the smallest position of one that sees any
-    for (int i = lane; i < ROWS; i += 32) {
-        const int pos = row_pos[i];
-        if (pos >= 0) { least = min(least, pos); if (OWN) last = max(last, pos + 1); }
-    }
-    least = __reduce_min_sync(ALL, least);
-    last = __reduce_max_sync(ALL, last);
-    const int base = OWN ? shared & ~(KT - 1) : 0;
-    Range keys = part_range(OWN ? shared : 0, last, base, part, parts, KT);
-    if (least == 0x7fffffff) keys.hi = keys.lo;
-    const int kt0 = keys.lo & ~(KT - 1), count = keys.hi > keys.lo ? (keys.hi - kt0 + KT - 1) / KT : 0;
+    const int G = p.H / p.KVH;
+    // `beside`: the kernel before is that of the shared tiles, which has let this one go when all it reads was complete, and which it waits
+    // for at its end instead, so that the join behind this one finds both done.  Every shared kernel waits first and then lets the next go.
+    if (!beside) pdl_wait();
+    pdl_launch_dependents();
 
-    // keys and values of tile j: its rows in [lo, hi), a lane a page
-    auto stage = [&](int j) {
-        if (warp != 0 || j >= count) return;
-        const int from = max(kt0 + j * KT, keys.lo), to = min(kt0 + (j + 1) * KT, keys.hi);
-        bf16* k = ring + (size_t)(j % STAGES) * 2 * TILE_ELEMENTS;
-        if (lane == 0) tc::mbar_arrive_expect_tx(&full[j % STAGES], (to - from) * HD * 4);
-        __syncwarp();
-        for (int index = from / p.page + lane; index * p.page < to; index += 32) {
-            const int a = max(from, index * p.page), b = min(to, (index + 1) * p.page);
-            const size_t at = (((size_t)page_at(p, t.slot, index) * 2 * p.KVH + kvh) * p.page + (a - index * p.page)) * HD;
-            const bf16* src = static_cast<const bf16*>(p.plane) + at;
-            bf16* dst = k + (a - kt0 - j * KT) * HD;
-            bulk_copy(dst, src, (b - a) * HD * 2, &full[j % STAGES]);
-            bulk_copy(dst + TILE_ELEMENTS, src + (size_t)p.KVH * p.page * HD, (b - a) * HD * 2, &full[j % STAGES]);
-        }
-    };
+    if (warp == 4) {
+        int stage = 0, n = 0;                               // tiles and items so far
+        bool ok = true;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++n) {
+            const int kvh = item % p.KVH, part = item / p.KVH % parts, slot = n % SLOTS;
+            const SharedTile t = tiles[item / p.KVH / parts];
+            const int shared = shared_keys(p, t);
+            int last = shared, least = 0x7fffffff;          // keys [.., last) are seen by some row; the smallest position of one that sees any
+            int pos[ROWS / 32 + 1];
 #pragma unroll
-    for (int j = 0; j < STAGES - 1; ++j) stage(j);
-    load_queries(p, t, kvh, ROWS, q_smem);
-    __syncthreads();
+            for (int i = 0; i < (ROWS + 31) / 32; ++i) {
+                pos[i] = lane + i * 32 < ROWS ? position_of(p, t, lane + i * 32) : -1;
+                if (pos[i] >= 0) { least = min(least, pos[i]); if (OWN) last = max(last, pos[i] + 1); }
+            }
+            least = __reduce_min_sync(ALL, least);
+            last = __reduce_max_sync(ALL, last);
+            Range keys = part_range(OWN ? shared : 0, last, OWN ? shared & ~(KT - 1) : 0, part, parts, KT);
+            if (least == 0x7fffffff) keys.hi = keys.lo;
+            const int kt0 = keys.lo & ~(KT - 1), count = keys.hi > keys.lo ? (keys.hi - kt0 + KT - 1) / KT : 0;
+            // pages are looked up a tile ahead, a lane a page
+            auto first_page = [&](int j) { return max(kt0 + j * KT, keys.lo) / p.page; };
+            auto page_of = [&](int j) {
+                const int index = j < count ? first_page(j) + lane : 0;
+                return j < count && index * p.page < min(kt0 + (j + 1) * KT, keys.hi) ? page_at(p, t.slot, index) : 0;
+            };
+            int page = page_of(0);
+            // ---- positions, queries (a copy a row's heads) and what the item is ----
+            ok = __all_sync(ALL, tc::mbar_wait(&q_empty[slot], ((n / SLOTS) & 1) ^ 1, abort, p.fault, 6));
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < (ROWS + 31) / 32; ++i)
+                if (lane + i * 32 < ROWS) row_pos[slot][lane + i * 32] = pos[i];
+            if (lane == 0) item_of[slot] = Item{t.rh0, t.count, kvh, part, keys.lo, keys.hi, least};
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive_expect_tx(&q_full[slot], t.count * HD * 2);
+            __syncwarp();
+            for (int row = t.rh0 / G + lane; row * G < t.rh0 + t.count; row += 32) {
+                const int a = max(t.rh0, row * G), b = min(t.rh0 + t.count, (row + 1) * G);
+                bulk_copy(q_smem + (slot * ROWS + a - t.rh0) * HD, static_cast<const bf16*>(p.q) + (long long)row * p.ldq + (kvh * G + a - row * G) * HD,
+                          (b - a) * HD * 2, &q_full[slot]);
+            }
+            // ---- keys and values of tile j: its rows in [lo, hi) ----
+            for (int j = 0; j < count; ++j, ++stage) {
+                const int next = page_of(j + 1), s = stage % STAGES;
+                ok = __all_sync(ALL, tc::mbar_wait(&empty[s], ((stage / STAGES) & 1) ^ 1, abort, p.fault, 6));
+                if (!ok) break;
+                const int from = max(kt0 + j * KT, keys.lo), to = min(kt0 + (j + 1) * KT, keys.hi);
+                bf16* k = ring + (size_t)s * 2 * TILE_ELEMENTS;
+                if (lane == 0) tc::mbar_arrive_expect_tx(&full[s], (to - from) * HD * 4);
+                __syncwarp();
+                for (int index = first_page(j) + lane, turn = 0; index * p.page < to; index += 32, ++turn) {
+                    if (turn > 0) page = page_at(p, t.slot, index);         // (pages of one row: more than a lane has looked up)
+                    const int a = max(from, index * p.page), b = min(to, (index + 1) * p.page);
+                    const bf16* src = static_cast<const bf16*>(p.plane) + (((size_t)page * 2 * p.KVH + kvh) * p.page + (a - index * p.page)) * HD;
+                    bf16* dst = k + (a - kt0 - j * KT) * HD;
+                    bulk_copy(dst, src, (b - a) * HD * 2, &full[s]);
+                    bulk_copy(dst + TILE_ELEMENTS, src + (size_t)p.KVH * p.page * HD, (b - a) * HD * 2, &full[s]);
+                }
+                page = next;
+            }
+        }
+        if (*abort)
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);   // copies that may still be on their way get time to land
+        if (beside) pdl_wait();
+        return;
+    }
 
+    // (A wait that ran out ends no loop over the items: the warps meet at barriers in each.)
+    bool slept = false;
+    for (int item = blockIdx.x, n = 0, stage = 0; item < items; item += gridDim.x, ++n) {
+    const int slot = n % SLOTS;
+    bool ok = __all_sync(ALL, !*abort && tc::mbar_wait(&q_full[slot], (n / SLOTS) & 1, abort, p.fault, 6));
+    const Item keys = item_of[slot];
+    const int least = keys.least, kvh = keys.kvh, part = keys.part;
+    const int kt0 = keys.lo & ~(KT - 1), count = ok && keys.hi > keys.lo ? (keys.hi - kt0 + KT - 1) / KT : 0;
+    const bf16* qs = q_smem + slot * ROWS * HD;
     const int r0 = WR == 1 ? 0 : warp * 16 * MT;            // the warp's first row head
     int pos[MT][2];
     float o[MT][HD / 8][4], m[MT][2], l[MT][2];
@@ -148,7 +181,7 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
             for (int e = 0; e < 4; ++e) o[x][n][e] = 0.f;
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-            pos[x][y] = row_pos[r0 + x * 16 + y * 8 + g];
+            pos[x][y] = row_pos[slot][r0 + x * 16 + y * 8 + g];
             m[x][y] = -INFINITY;
             l[x][y] = 0.f;
         }
@@ -156,44 +189,47 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {
                 const int qr = r0 + x * 16 + (lane & 15);
-                ldmatrix4(qf[QUERIES_STAY ? x : 0][QUERIES_STAY ? k : 0], q_smem + qr * HD + cache_chunk(2 * k + (lane >> 4), qr, CHUNKS) * 8);
+                ldmatrix4(qf[QUERIES_STAY ? x : 0][QUERIES_STAY ? k : 0], qs + qr * HD + (2 * k + (lane >> 4)) * 8);
             }
         }
     }
-    if (QUERIES_STAY) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    bool ok = true;
-    for (int j = 0; j < count; ++j) {
-        ok = tc::mbar_wait(&full[j % STAGES], (j / STAGES) & 1, abort, p.fault, 6);
-        if (__syncthreads_or(!ok)) { ok = false; break; }   // everyone has tile j, and is done with tile j - 1: its place is free
-        stage(j + STAGES - 1);
-        const bf16* ks = ring + (size_t)(j % STAGES) * 2 * TILE_ELEMENTS;
+    for (int j = 0; j < count; ++j, ++stage) {
+        ok = __all_sync(ALL, tc::mbar_wait(&full[stage % STAGES], (stage / STAGES) & 1, abort, p.fault, 6));
+        if (!ok) break;
+        const bf16* ks = ring + (size_t)(stage % STAGES) * 2 * TILE_ELEMENTS;
         bf16* vs = const_cast<bf16*>(ks) + TILE_ELEMENTS;
         const int kt = kt0 + j * KT;
-        if (kt < keys.lo || kt + KT > keys.hi) {
-            // values of rows that were not copied: nothing that a probability of 0 could not take away
-            for (int i = threadIdx.x; i < KT * CHUNKS; i += MMA_THREADS) {
-                const int key = kt + i / CHUNKS;
-                if (key < keys.lo || key >= keys.hi) *reinterpret_cast<uint4*>(vs + i * 8) = make_uint4(0u, 0u, 0u, 0u);
-            }
+        // a warp's keys of the tile (WR 1: a sixteen of its own; else all of them: every warp writes the same zeros and waits for none)
+        const int mine0 = WR == 1 ? warp * 16 : 0, mine = WR == 1 ? 16 : KT;
+        auto meet = [&]() {
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            __syncthreads();
+            __syncwarp();
+        };
+        if (kt + mine0 < keys.lo || kt + mine0 + mine > keys.hi) {
+            // values of rows that were not copied: nothing that a probability of 0 could not take away
+            for (int i = lane; i < mine * CHUNKS; i += 32) {
+                const int key = kt + mine0 + i / CHUNKS;
+                if (key < keys.lo || key >= keys.hi) *reinterpret_cast<uint4*>(vs + mine0 * HD + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            meet();
         }
-        if (OWN && kt + KT - 1 > least && least < keys.hi - 1) {
+        if (OWN && kt + mine0 + mine - 1 > least && least < keys.hi - 1) {
             // Behind the first row's position a key is seen by some rows and not by others, whose probability of 0 does not take away a
-            // value that is not finite: such values go apart, and zeros into the products.  (Uniform in the CTA.)
-            int odd = 0;
-            for (int i = threadIdx.x; i < KT * CHUNKS; i += MMA_THREADS) {
-                const int key = kt + i / CHUNKS;
+            // value that is not finite: such values go apart, and zeros into the products.  (OWN: a warp's keys are its own.)
+            static_assert(!OWN || WR == 1, "own tiles share out their keys");
+            bool odd = false;
+            for (int i = lane; i < mine * CHUNKS; i += 32) {
+                const int key = kt + mine0 + i / CHUNKS;
                 if (key > least && key < keys.hi) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(vs + i * 8);
+                    const uint4 w = *reinterpret_cast<const uint4*>(vs + mine0 * HD + i * 8);
                     const unsigned u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) odd |= (u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u;
                 }
             }
-            if (__syncthreads_or(odd)) {
+            if (__any_sync(ALL, odd)) {
                 // a row that sees such a value has a result that is not finite there, whatever the probability (a positive number, or 0)
-                for (int key = max(least + 1, kt); key < min(keys.hi, kt + KT) && (WR > 1 || warp == 0); ++key)
+                for (int key = max(least + 1, kt + mine0); key < min(keys.hi, kt + mine0 + mine); ++key)
 #pragma unroll
                     for (int n = 0; n < HD / 8; ++n)
 #pragma unroll
@@ -204,16 +240,15 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
                             for (int x = 0; x < MT; ++x)
                                 if (key <= pos[x][e >> 1] && !(fabsf(v) < INFINITY)) o[x][n][e] += v;
                         }
-                __syncthreads();
-                for (int i = threadIdx.x; i < KT * CHUNKS; i += MMA_THREADS) {
-                    const int key = kt + i / CHUNKS;
+                __syncwarp();
+                for (int i = lane; i < mine * CHUNKS; i += 32) {
+                    const int key = kt + mine0 + i / CHUNKS;
                     if (key <= least || key >= keys.hi) continue;
-                    unsigned short* w = reinterpret_cast<unsigned short*>(vs + i * 8);
+                    unsigned short* w = reinterpret_cast<unsigned short*>(vs + mine0 * HD + i * 8);
                     for (int e = 0; e < 8; ++e)
                         if ((w[e] & 0x7f80u) == 0x7f80u) w[e] = 0;
                 }
-                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                __syncthreads();
+                meet();
             }
         }
 #pragma unroll 1
@@ -238,7 +273,7 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
                         for (int e = 0; e < 4; ++e) a[e] = qf[QUERIES_STAY ? x : 0][QUERIES_STAY ? k : 0][e];
                     } else {
                         const int qr = r0 + x * 16 + (lane & 15);
-                        ldmatrix4(a, q_smem + qr * HD + cache_chunk(2 * k + (lane >> 4), qr, CHUNKS) * 8);
+                        ldmatrix4(a, qs + qr * HD + (2 * k + (lane >> 4)) * 8);
                     }
                     mma(s[x][0], a, bk[0], bk[1]);
                     mma(s[x][1], a, bk[2], bk[3]);
@@ -301,12 +336,16 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
                 }
             }
         }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&empty[stage % STAGES]);
     }
-    if (!ok) {
-        // a wait ran out: copies that may still be on their way get time to land before the shared memory is given up
+    if (!ok && !slept) {                                    // a wait ran out: copies that may still be on their way get time to land
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-        return;
+        slept = true;
     }
+    // the item's queries have been read, its place is free
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&q_empty[slot]);
 #pragma unroll
     for (int x = 0; x < MT; ++x)
 #pragma unroll
@@ -315,14 +354,14 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
             l[x][y] += __shfl_xor_sync(ALL, l[x][y], 2);
         }
 
-    auto place = [&](int i) { const int rh = t.rh0 + i; return ((size_t)(part0 + part) * p.rows + rh / G) * p.H + kvh * G + rh % G; };
+    auto place = [&](int i) { const int rh = keys.rh0 + i; return ((size_t)(part0 + part) * p.rows + rh / G) * p.H + kvh * G + rh % G; };
     if (WR > 1) {
 #pragma unroll
         for (int x = 0; x < MT; ++x)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 const int i = r0 + x * 16 + y * 8 + g;
-                if (i >= t.count) continue;
+                if (i >= keys.count || !ok) continue;
                 const size_t at = place(i);
                 if (t4 == 0) p.part_ml[at] = make_float2(m[x][y], l[x][y]);
 #pragma unroll
@@ -330,37 +369,56 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
                     *reinterpret_cast<float2*>(p.part_o + at * HD + n * 8 + t4 * 2) = make_float2(o[x][n][2 * y], o[x][n][2 * y + 1]);
             }
     } else {
-        // the four warps' shares: sums relative to the largest maximum, added up in the order of the warps
-        float* merge_o = reinterpret_cast<float*>(ring);    // [warp][row][HD]: every copy has landed, every tile been read
+        // the four warps' shares, sums relative to the largest maximum: warps 2 and 3 to 0 and 1, then 1 to 0
         if (t4 == 0) {
 #pragma unroll
             for (int y = 0; y < 2; ++y) { merge_m[warp][g + 8 * y] = m[0][y]; merge_l[warp][g + 8 * y] = l[0][y]; }
         }
-        __syncthreads();
+        asm volatile("bar.sync 1, 128;\n" ::: "memory");
+        float M[2], sum[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             const int r = g + 8 * y;
-            const float M = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
-            const float f = m[0][y] == -INFINITY ? 1.f : exp2_fast(m[0][y] - M);
+            M[y] = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
+            sum[y] = 0.f;
 #pragma unroll
-            for (int n = 0; n < HD / 8; ++n)
-                *reinterpret_cast<float2*>(merge_o + (size_t)(warp * 16 + r) * HD + n * 8 + t4 * 2) = make_float2(o[0][n][2 * y] * f, o[0][n][2 * y + 1] * f);
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * HD; i += MMA_THREADS) {
-            const int r = i / HD;
-            if (r >= t.count) break;
-            p.part_o[place(r) * HD + i % HD] = ((merge_o[i] + merge_o[16 * HD + i]) + merge_o[32 * HD + i]) + merge_o[48 * HD + i];
-        }
-        if (threadIdx.x < 16 && (int)threadIdx.x < t.count) {
-            const int r = threadIdx.x;
-            const float M = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
-            float sum = 0.f;
+            for (int w = 0; w < 4; ++w) sum[y] += merge_m[w][r] == -INFINITY ? merge_l[w][r] : merge_l[w][r] * exp2_fast(merge_m[w][r] - M[y]);
+            const float f = m[0][y] == -INFINITY ? 1.f : exp2_fast(m[0][y] - M[y]);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) sum += merge_m[w][r] == -INFINITY ? merge_l[w][r] : merge_l[w][r] * exp2_fast(merge_m[w][r] - M);
-            p.part_ml[place(r)] = make_float2(M, sum);
+            for (int n8 = 0; n8 < HD / 8; ++n8) { o[0][n8][2 * y] *= f; o[0][n8][2 * y + 1] *= f; }
+        }
+#pragma unroll
+        for (int from = 2; from > 0; from >>= 1) {          // warps [from, 2 from) give, warps [0, from) take: each lane's sums, in its own order
+            if (warp >= from && warp < 2 * from) {
+#pragma unroll
+                for (int n8 = 0; n8 < HD / 8; ++n8)
+                    *reinterpret_cast<float4*>(merge_o + (((warp - from) * (HD / 8) + n8) * 32 + lane) * 4) = make_float4(o[0][n8][0], o[0][n8][1], o[0][n8][2], o[0][n8][3]);
+            }
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");
+            if (warp < from) {
+#pragma unroll
+                for (int n8 = 0; n8 < HD / 8; ++n8) {
+                    const float4 v = *reinterpret_cast<const float4*>(merge_o + ((warp * (HD / 8) + n8) * 32 + lane) * 4);
+                    o[0][n8][0] += v.x; o[0][n8][1] += v.y; o[0][n8][2] += v.z; o[0][n8][3] += v.w;
+                }
+            }
+            if (from > 1) asm volatile("bar.sync 1, 128;\n" ::: "memory");     // (read before it is written again; behind the last round the next
+        }                                                                       // item's first barrier is between)
+        if (warp == 0 && ok) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int i = g + 8 * y;
+                if (i >= keys.count) continue;
+                const size_t at = place(i);
+                if (t4 == 0) p.part_ml[at] = make_float2(M[y], sum[y]);
+#pragma unroll
+                for (int n8 = 0; n8 < HD / 8; ++n8)
+                    *reinterpret_cast<float2*>(p.part_o + at * HD + n8 * 8 + t4 * 2) = make_float2(o[0][n8][2 * y], o[0][n8][2 * y + 1]);
+            }
         }
     }
+    }
+    if (beside) pdl_wait();
 }
 
 // ---- float32: dot products on the CUDA cores, everything in 32 bits ---------------------------------------------------------
@@ -552,14 +610,14 @@ template <typename T> int launch_join(const SharedParams& p, void* out, long lon
     return tis_check_launch("shared_prefix_attention (join)");
 }
 
-template <bool OWN, int WR, int MT> int launch_mma(const SharedParams& p, const SharedTile* tiles, int count, int parts, int part0, cudaStream_t stream) {
-    const size_t smem = (size_t)STAGES * 2 * TILE_ELEMENTS * 2 + (QUERIES_STAY ? 0 : (size_t)16 * WR * MT * HD * 2);
-    static_assert(STAGES * 2 * TILE_ELEMENTS * 2 >= 4 * 16 * HD * 4, "four warps' shares fit the ring");
-    static_assert(2 * TILE_ELEMENTS >= 16 * WR * MT * HD, "the queries fit a stage");
+template <bool OWN, int WR, int MT> int launch_mma(const SharedParams& p, const SharedTile* tiles, int count, int parts, int part0, int beside, cudaStream_t stream) {
+    constexpr int ROWS = 16 * WR * MT;
+    const size_t smem = (size_t)STAGES * 2 * TILE_ELEMENTS * 2 + (size_t)(WR == 1 ? 2 : 1) * ROWS * HD * 2 + (WR == 1 ? 2 * 16 * HD * 4 : 0);
+    const int items = count * parts * p.KVH, ctas = WR == 1 ? (HD <= 128 ? 2 : 1) * tc::sm_count() : items;
     static DeviceOnce configured;
     if (configured.first() && cudaFuncSetAttribute(shared_mma_kernel<OWN, WR, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return tis_check_launch("shared_prefix_attention (shared memory)");
-    tis_launch(shared_mma_kernel<OWN, WR, MT>, dim3((unsigned)(count * parts * p.KVH)), dim3(MMA_THREADS), smem, stream, p, tiles, parts, part0);
+    tis_launch(shared_mma_kernel<OWN, WR, MT>, dim3((unsigned)(items < ctas ? items : ctas)), dim3(MMA_THREADS + LOAD_THREADS), smem, stream, p, tiles, items, parts, part0, beside);
     return tis_check_launch("shared_prefix_attention");
 }
 
@@ -615,11 +673,11 @@ TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* 
     } else if (dtype == TIS_BF16) {
         if (shared_parts > 0) {
             if (tensor) status = shared_tc_launch(p, w, wide_count, shared_parts, stream);
-            else if (wide_rows == 16) status = launch_mma<false, 1, 1>(p, w, wide_count, shared_parts, 0, stream);
-            else if (wide_rows == 64) status = launch_mma<false, 4, 1>(p, w, wide_count, shared_parts, 0, stream);
-            else status = launch_mma<false, 4, HD <= 128 ? 2 : 1>(p, w, wide_count, shared_parts, 0, stream);
+            else if (wide_rows == 16) status = launch_mma<false, 1, 1>(p, w, wide_count, shared_parts, 0, 0, stream);
+            else if (wide_rows == 64) status = launch_mma<false, 4, 1>(p, w, wide_count, shared_parts, 0, 0, stream);
+            else status = launch_mma<false, 4, HD <= 128 ? 2 : 1>(p, w, wide_count, shared_parts, 0, 0, stream);
         }
-        if (status == TIS_OK) status = launch_mma<true, 1, 1>(p, o, own_count, own_parts, shared_parts, stream);
+        if (status == TIS_OK) status = launch_mma<true, 1, 1>(p, o, own_count, own_parts, shared_parts, shared_parts > 0, stream);
     } else {
         tis_set_error("shared_prefix_attention: dtype code %d", dtype);
         return TIS_BAD_DTYPE;

@@ -55,7 +55,6 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const SharedParams 
     __shared__ int abort_flag;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_launch_dependents();
     const int kvh = blockIdx.x % p.KVH, part = blockIdx.x / p.KVH % parts;
     const SharedTile t = tiles[blockIdx.x / p.KVH / parts];             // (the plan's, from before the batch)
     const int G = p.H / p.KVH;
@@ -64,6 +63,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const SharedParams 
     auto place = [&](int i) { const int rh = t.rh0 + i; return ((size_t)part * p.rows + rh / G) * p.H + kvh * G + rh % G; };
     if (T == 0) {                                           // nothing of this group in this part: the whole CTA leaves together
         pdl_wait();
+        pdl_launch_dependents();
         if ((int)threadIdx.x < t.count) p.part_ml[place(threadIdx.x)] = make_float2(-INFINITY, 0.f);
         return;
     }
@@ -90,6 +90,9 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const SharedParams 
     const unsigned tmem_base = tmem_base_slot;
     volatile int* abort = &abort_flag;
     pdl_wait();                                             // queries, tables and the cache's rows come from the kernels before
+    // Only now: the kernel of the requests' own keys starts beside this one, when all CTAs of this one are here, and waits for it at its
+    // end; what both read is complete by then.
+    pdl_launch_dependents();
 
     // 512 threads are launched with 128 registers each, 65536 in all: 256 x 40 + 256 x 216
     if (warp < 4 || warp >= 12) {

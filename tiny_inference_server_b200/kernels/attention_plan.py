@@ -142,6 +142,7 @@ class SharedPrefixPlan:
         self.own, *shared_words = words.split([len(p) for p in parts])
         self.shared = dict(zip(self.SHARED_TILES, shared_words))
         self.device = words.device
+        self.splits: Dict[tuple, tuple] = {}                  # how the kernels split the keys (kernels.ops)
 
 
 _planners: Dict[int, AttentionTilePlanner] = {}

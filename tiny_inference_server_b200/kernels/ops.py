@@ -999,20 +999,15 @@ def shared_attention_library(head_dim: int):
     return lib
 
 
-def _shared_parts(tiles: int, keys: int, resident: int) -> int:
-    """Parts that the keys of ``tiles`` CTAs are split into: as many as are resident at a time, of at least 64 keys each."""
-    return max(1, min(-(-keys // 64), resident // max(1, tiles), 64))
-
-
-def _split_parts(items: int, tiles: int, resident: int) -> int:
-    """Parts of the shared keys' ``tiles``, for ``items`` (row heads, kv head) of CTAs of which ``resident`` run at a time: the fewest rounds
-    of the longest part, a CTA costing four tiles to start and finish and a part a tenth of one to join."""
+def _split_parts(items: int, tiles: int, resident: int, start: float, most: int = 64) -> int:
+    """Parts that ``tiles`` of keys are split into, for ``items`` (row heads, kv head) of which ``resident`` are worked on at a time: the
+    fewest rounds of the longest part, an item costing ``start`` tiles beside its own and a part a tenth of one to join."""
     best, cost = 1, None
-    for parts in range(1, min(tiles, 64) + 1):
+    for parts in range(1, min(tiles, most) + 1):
         per = -(-tiles // parts)
         if -(-tiles // per) != parts:
             continue
-        c = -(-items * parts // resident) * (per + 4) + 0.1 * parts
+        c = -(-items * parts // resident) * (per + start) + 0.1 * parts
         if cost is None or c < cost - 1e-9:
             best, cost = parts, c
     return best
@@ -1058,15 +1053,29 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     _on_this_device("shared_prefix_attention", q, out, plane, block_table, positions, plan.own, fault)
     lib = shared_attention_library(hd)
     width = block_table.shape[1]
-    # shared tiles of the row heads that the groups have, as far as the kernels go
-    tensor = int(code == 1 and TC_ATTENTION and lib.tis_shared_attn_tensor(page) and 2 * pages * kvh * page < 1 << 31)
-    wide_rows = 128 if tensor else (16 if code == 0 or plan.most_heads <= 16 else (64 if plan.most_heads <= 64 else lib.widest))
-    wide = plan.shared[wide_rows]
-    n_own, n_wide = plan.own.shape[0], wide.shape[0]
+    n_own = plan.own.shape[0]
     shared = plan.max_shared // page * page
-    own_keys = max(1, (width * page if max_position is None else max_position + 1) - plan.min_shared // page * page)
-    shared_parts = (_split_parts(n_wide * kvh, -(-shared // 128), 148) if tensor else _shared_parts(n_wide * kvh, shared, 2 * 148)) if shared else 0
-    own_parts = _shared_parts(n_own * kvh, own_keys, 2 * 148)
+    own_tiles = max(1, -(-((width * page if max_position is None else max_position + 1) - plan.min_shared // page * page) // 64))
+    # how the keys are split: found once for a plan and as long as the own keys stay within the same 64
+    tensor = code == 1 and TC_ATTENTION and 2 * pages * kvh * page < 1 << 31
+    key = (hd, page, code, tensor, own_tiles)
+    split = plan.splits.get(key)
+    if split is None:
+        tensor = int(tensor and lib.tis_shared_attn_tensor(page))
+        # shared tiles of the row heads that the groups have, as far as the kernels go
+        wide_rows = 128 if tensor else (16 if code == 0 or plan.most_heads <= 16 else (64 if plan.most_heads <= 64 else lib.widest))
+        n_wide = plan.shared[wide_rows].shape[0]
+        if not shared:
+            shared_parts = 0
+        elif tensor:
+            shared_parts = _split_parts(n_wide * kvh, -(-shared // 128), 148, 4)
+        else:
+            shared_parts = _split_parts(n_wide * kvh, -(-shared // 64), 2 * 148, 4)
+        own_parts = _split_parts(n_own * kvh, own_tiles, (2 if hd <= 128 else 1) * 148, 1)
+        if len(plan.splits) > 256:
+            plan.splits.clear()
+        split = plan.splits[key] = (tensor, wide_rows, plan.shared[wide_rows], n_wide, shared_parts, own_parts)
+    tensor, wide_rows, wide, n_wide, shared_parts, own_parts = split
     parts, row_heads = shared_parts + own_parts, rows * h
     scratch = torch.empty(parts * row_heads * (hd + 2), dtype=torch.float32, device=q.device)
     calls["shared_prefix_attention"] += 1
