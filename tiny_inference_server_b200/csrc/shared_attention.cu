@@ -58,8 +58,20 @@ __device__ __forceinline__ int position_of(const SharedParams& p, const SharedTi
     return pos >= t.prefix ? pos : -1;
 }
 
+// Chunk c of the cache row of a position (common.cuh: cache_chunk), the position's part worked out once.
+struct RowChunks {
+    int base;
+    __device__ __forceinline__ explicit RowChunks(int position) : base(CHUNKS % 8 == 0 ? position & 7 : position % CHUNKS) {}
+    __device__ __forceinline__ int operator()(int c) const {
+        if (CHUNKS % 8 == 0) return c ^ base;
+        return base + c - (base + c >= CHUNKS ? CHUNKS : 0);
+    }
+};
+// the running maximum is raised when a row's scores leave it behind by more than this (in units of log2: sums stay below 2^8 a key)
+constexpr float RAISE_STEP = 8.f;
+
 // What the loading warp tells the others of an item (a tile, a kv head and a part).
-struct Item { int rh0, count, kvh, part, lo, hi, least; };
+struct Item { int rh0, count, kvh, part, lo, hi, least; bool all; };     // all: every row head sees keys (what rows behind them hold stays there)
 
 // OWN: own tiles (rows end at their positions), else shared ones.  WR warps side by side over the rows, MT sixteens of row heads each; with
 // WR 1 the warps share out the keys.  A CTA goes through the items blockIdx.x, + gridDim.x, ..; the loading warp is ahead by the
@@ -109,6 +121,10 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
             }
             least = __reduce_min_sync(ALL, least);
             last = __reduce_max_sync(ALL, last);
+            bool all = true;
+#pragma unroll
+            for (int i = 0; i < (ROWS + 31) / 32; ++i) all = all && (pos[i] >= 0 || lane + i * 32 >= t.count);
+            all = __all_sync(ALL, all);
             Range keys = part_range(OWN ? shared : 0, last, OWN ? shared & ~(KT - 1) : 0, part, parts, KT);
             if (least == 0x7fffffff) keys.hi = keys.lo;
             const int kt0 = keys.lo & ~(KT - 1), count = keys.hi > keys.lo ? (keys.hi - kt0 + KT - 1) / KT : 0;
@@ -125,7 +141,7 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
 #pragma unroll
             for (int i = 0; i < (ROWS + 31) / 32; ++i)
                 if (lane + i * 32 < ROWS) row_pos[slot][lane + i * 32] = pos[i];
-            if (lane == 0) item_of[slot] = Item{t.rh0, t.count, kvh, part, keys.lo, keys.hi, least};
+            if (lane == 0) item_of[slot] = Item{t.rh0, t.count, kvh, part, keys.lo, keys.hi, least, all};
             __syncwarp();
             if (lane == 0) tc::mbar_arrive_expect_tx(&q_full[slot], t.count * HD * 2);
             __syncwarp();
@@ -260,11 +276,13 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
             for (int x = 0; x < MT; ++x)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[x][e >> 2][e & 3] = 0.f;
+            const int kr = kb + (lane & 7) + (lane >> 4) * 8, kc = (lane >> 3) & 1;
+            const bf16* krow = ks + kr * HD;
+            const RowChunks kchunk(kt + kr);
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {
                 unsigned bk[4];
-                const int kr = kb + (lane & 7) + (lane >> 4) * 8;
-                ldmatrix4(bk, ks + kr * HD + cache_chunk(2 * k + ((lane >> 3) & 1), kt + kr, CHUNKS) * 8);
+                ldmatrix4(bk, krow + kchunk(2 * k + kc) * 8);
 #pragma unroll
                 for (int x = 0; x < MT; ++x) {
                     unsigned a[4];
@@ -279,26 +297,29 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
                     mma(s[x][1], a, bk[2], bk[3]);
                 }
             }
-            const bool whole = kt + kb >= keys.lo && kt + kb + 15 < keys.hi && (!OWN || kt + kb + 15 <= least);
+            // every key is there, and every row sees it
+            const bool whole = kt + kb >= keys.lo && kt + kb + 15 < keys.hi && (!OWN || kt + kb + 15 <= least) && keys.all;
             unsigned pa[MT][4];
 #pragma unroll
             for (int x = 0; x < MT; ++x) {
-                float top[2] = {-INFINITY, -INFINITY};
+                if (!whole) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = kt + kb + n * 8 + t4 * 2 + (e & 1), y = e >> 1;
-                        const bool in = (whole || (key >= keys.lo && key < keys.hi && (!OWN || key <= pos[x][y]))) && pos[x][y] >= 0;
-                        s[x][n][e] = in ? s[x][n][e] * p.scale_log2 : -INFINITY;
-                        top[y] = fmaxf(top[y], s[x][n][e]);
-                    }
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = kt + kb + n * 8 + t4 * 2 + (e & 1), y = e >> 1;
+                            const bool in = key >= keys.lo && key < keys.hi && (!OWN || key <= pos[x][y]) && pos[x][y] >= 0;
+                            s[x][n][e] = in ? s[x][n][e] : -INFINITY;
+                        }
+                }
+                float top[2];
                 bool raise = false;
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
+                    top[y] = fmaxf(fmaxf(s[x][0][2 * y], s[x][0][2 * y + 1]), fmaxf(s[x][1][2 * y], s[x][1][2 * y + 1]));
                     top[y] = fmaxf(top[y], __shfl_xor_sync(ALL, top[y], 1));
-                    top[y] = fmaxf(top[y], __shfl_xor_sync(ALL, top[y], 2));
-                    raise |= top[y] > m[x][y];
+                    top[y] = fmaxf(top[y], __shfl_xor_sync(ALL, top[y], 2)) * p.scale_log2;     // (the scale is positive)
+                    raise |= top[y] > m[x][y] + RAISE_STEP || (m[x][y] == -INFINITY && top[y] > -INFINITY);
                 }
                 if (__any_sync(ALL, raise)) {
 #pragma unroll
@@ -312,23 +333,25 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
                         m[x][y] = up;
                     }
                 }
+                const float neg[2] = {m[x][0] == -INFINITY ? 0.f : -m[x][0], m[x][1] == -INFINITY ? 0.f : -m[x][1]};
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int y = e >> 1;
-                        s[x][n][e] = exp2_fast(s[x][n][e] - (m[x][y] == -INFINITY ? 0.f : m[x][y]));
-                        l[x][y] += s[x][n][e];
+                        s[x][n][e] = exp2_fast(fmaf(s[x][n][e], p.scale_log2, neg[e >> 1]));
+                        l[x][e >> 1] += s[x][n][e];
                     }
                 // probabilities in bfloat16 (half a step, 2^-9 of each, at random): the tensor cores' operand; their sum stays in 32 bits
                 pa[x][0] = pack(s[x][0][0], s[x][0][1]); pa[x][1] = pack(s[x][0][2], s[x][0][3]);
                 pa[x][2] = pack(s[x][1][0], s[x][1][1]); pa[x][3] = pack(s[x][1][2], s[x][1][3]);
             }
+            const int vr = kb + (lane & 15), vc = lane >> 4;
+            const bf16* vrow = vs + vr * HD;
+            const RowChunks vchunk(kt + vr);
 #pragma unroll
             for (int n = 0; n < HD / 16; ++n) {
                 unsigned bv[4];
-                const int vr = kb + (lane & 15);
-                ldmatrix4_trans(bv, vs + vr * HD + cache_chunk(2 * n + (lane >> 4), kt + vr, CHUNKS) * 8);
+                ldmatrix4_trans(bv, vrow + vchunk(2 * n + vc) * 8);
 #pragma unroll
                 for (int x = 0; x < MT; ++x) {
                     mma(o[x][2 * n], pa[x], bv[0], bv[1]);
