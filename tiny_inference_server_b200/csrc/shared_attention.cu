@@ -70,6 +70,55 @@ struct RowChunks {
 // the running maximum is raised when a row's scores leave it behind by more than this (in units of log2: sums stay below 2^8 a key)
 constexpr float RAISE_STEP = 8.f;
 
+// The result of row head rh of a kv head from its own part (m, l, o in shared memory) and the shared ones: an eighth of its columns.
+__device__ __forceinline__ void join_row(const SharedParams& p, float m, float l, const float* o, int rh, int kvh, int eighth) {
+    constexpr int COLS = HD / 8, AHEAD = 4;
+    const int G = p.H / p.KVH, row = rh / G, head = kvh * G + rh % G;
+    const size_t at = (size_t)row * p.H + head, step = (size_t)p.rows * p.H;
+    float M = m;
+    for (int q0 = 0; q0 < p.shared_parts; q0 += 8) {
+        float x8[8];
+#pragma unroll
+        for (int a = 0; a < 8; ++a) x8[a] = p.part_ml[at + min(q0 + a, p.shared_parts - 1) * step].x;
+#pragma unroll
+        for (int a = 0; a < 8; ++a) M = fmaxf(M, x8[a]);
+    }
+    float f = m == -INFINITY ? 1.f : exp2_fast(m - M), sum = l * f, x[COLS];
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) x[c] = o[eighth * COLS + c] * f;
+    for (int q0 = 0; q0 < p.shared_parts; q0 += AHEAD) {
+        float2 v[AHEAD][COLS / 2], ml[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            ml[a] = q0 + a < p.shared_parts ? p.part_ml[at + (q0 + a) * step] : make_float2(-INFINITY, 0.f);
+            const bool some = !(ml[a].x == -INFINITY && ml[a].y == 0.f);             // (else no keys: nothing was left there)
+            const float2* src = reinterpret_cast<const float2*>(p.part_o + (at + (q0 + a) * step) * HD + eighth * COLS);
+#pragma unroll
+            for (int c = 0; c < COLS / 2; ++c) v[a][c] = some ? src[c] : make_float2(0.f, 0.f);
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            f = ml[a].x == -INFINITY ? 1.f : exp2_fast(ml[a].x - M);
+            sum += ml[a].y * f;
+#pragma unroll
+            for (int c = 0; c < COLS / 2; ++c) {
+                x[2 * c] = fmaf(v[a][c].x, f, x[2 * c]);
+                x[2 * c + 1] = fmaf(v[a][c].y, f, x[2 * c + 1]);
+            }
+        }
+    }
+    bf16* dst = static_cast<bf16*>(p.out) + (long long)row * p.ldo + head * HD + eighth * COLS;
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) x[c] = sum == 0.f ? 0.f : x[c] / sum;
+    if (p.out_vectors && COLS % 8 == 0) {
+#pragma unroll
+        for (int c = 0; c < COLS / 8; ++c) tc::store8(dst + c * 8, x + c * 8);
+    } else {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) dst[c] = __float2bfloat16_rn(x[c]);
+    }
+}
+
 // What the loading warp tells the others of an item (a tile, a kv head and a part).
 struct Item { int rh0, count, kvh, part, lo, hi, least; bool all; };     // all: every row head sees keys (what rows behind them hold stays there)
 
@@ -427,17 +476,36 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
             }
             if (from > 1) asm volatile("bar.sync 1, 128;\n" ::: "memory");     // (read before it is written again; behind the last round the next
         }                                                                       // item's first barrier is between)
-        if (warp == 0 && ok) {
+        if (!OWN || p.own_parts > 1) {
+            if (warp == 0 && ok) {
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const int i = g + 8 * y;
-                if (i >= keys.count) continue;
-                const size_t at = place(i);
-                if (t4 == 0) p.part_ml[at] = make_float2(M[y], sum[y]);
+                for (int y = 0; y < 2; ++y) {
+                    const int i = g + 8 * y;
+                    if (i >= keys.count) continue;
+                    const size_t at = place(i);
+                    if (t4 == 0) p.part_ml[at] = make_float2(M[y], sum[y]);
 #pragma unroll
-                for (int n8 = 0; n8 < HD / 8; ++n8)
-                    *reinterpret_cast<float2*>(p.part_o + at * HD + n8 * 8 + t4 * 2) = make_float2(o[0][n8][2 * y], o[0][n8][2 * y + 1]);
+                    for (int n8 = 0; n8 < HD / 8; ++n8)
+                        *reinterpret_cast<float2*>(p.part_o + at * HD + n8 * 8 + t4 * 2) = make_float2(o[0][n8][2 * y], o[0][n8][2 * y + 1]);
+                }
             }
+        } else {
+            // ---- the only own part: joined with the shared ones here, eight threads a row head.  The kernel of the shared tiles is waited for
+            // only now. ----
+            if (warp == 0) {
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    if (t4 == 0) { merge_m[0][g + 8 * y] = M[y]; merge_l[0][g + 8 * y] = sum[y]; }
+#pragma unroll
+                    for (int n8 = 0; n8 < HD / 8; ++n8)
+                        *reinterpret_cast<float2*>(merge_o + (g + 8 * y) * HD + n8 * 8 + t4 * 2) = make_float2(o[0][n8][2 * y], o[0][n8][2 * y + 1]);
+                }
+            }
+            if (beside) pdl_wait();
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");
+            const int i = threadIdx.x >> 3;
+            if (i < keys.count && ok) join_row(p, merge_m[0][i], merge_l[0][i], merge_o + i * HD, keys.rh0 + i, kvh, threadIdx.x & 7);
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");         // (read before the next item writes it)
         }
     }
     }
@@ -670,6 +738,7 @@ TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* 
     p.positions = positions;
     p.part_o = part_o; p.part_ml = static_cast<float2*>(part_ml);
     p.rows = rows; p.H = H; p.KVH = KVH; p.page = page; p.own_parts = own_parts; p.shared_parts = shared_parts;
+    p.out = out; p.ldo = ldo; p.out_vectors = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo % 8 == 0;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.fault = fault;
     if (wide_rows != 16 && (dtype == TIS_F32 || wide_rows > tis_shared_attn_widest() || (wide_rows != 64 && wide_rows != 128))) {
@@ -705,6 +774,6 @@ TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* 
         tis_set_error("shared_prefix_attention: dtype code %d", dtype);
         return TIS_BAD_DTYPE;
     }
-    if (status != TIS_OK) return status;
+    if (status != TIS_OK || (dtype == TIS_BF16 && own_parts == 1)) return status;       // (the own tiles have joined theirs)
     return dtype == TIS_F32 ? launch_join<float>(p, out, ldo, row_heads, parts, stream) : launch_join<bf16>(p, out, ldo, row_heads, parts, stream);
 }

@@ -21,6 +21,7 @@ struct SharedParams {
     float* part_o;                                // [parts][rows][H][hd]
     float2* part_ml;                              // [parts][rows][H]
     int rows, H, KVH, page, own_parts, shared_parts;
+    void* out; long long ldo; bool out_vectors;   // results; whether their rows start on 16 bytes
     float scale_log2;
     int* fault;
 };

@@ -188,15 +188,22 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const SharedParams 
         const int g = warp >= 8 ? 1 : 0;                  // warps 4-7 and 8-11
         const int quarter = warp & 3;                     // the lanes of tensor memory this warp may touch
         const int r = quarter * 32 + lane;
-        // the queries, a 16-byte piece a thread: rows of 128 swizzled bytes, zero beyond the tile
-        for (int i = threadIdx.x - 128; i < BM * HD / 8; i += 256) {
-            const int row = i / (HD / 8), c = i % (HD / 8);
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        // the queries, 16-byte pieces, all loads of a thread on their way at once: rows of 128 swizzled bytes, zero beyond the tile
+        constexpr int PIECES = BM * HD / 8 / 256;
+        uint4 piece[PIECES];
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) {
+            const int i = threadIdx.x - 128 + n * 256, row = i / (HD / 8), c = i % (HD / 8);
+            piece[n] = make_uint4(0u, 0u, 0u, 0u);
             if (row < t.count) {
                 const int rh = t.rh0 + row;
-                v = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + (long long)(rh / G) * p.ldq + (kvh * G + rh % G) * HD + c * 8);
+                piece[n] = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + (long long)(rh / G) * p.ldq + (kvh * G + rh % G) * HD + c * 8);
             }
-            *reinterpret_cast<uint4*>(q_smem + (c >> 3) * HALF_BYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+        }
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) {
+            const int i = threadIdx.x - 128 + n * 256, row = i / (HD / 8), c = i % (HD / 8);
+            *reinterpret_cast<uint4*>(q_smem + (c >> 3) * HALF_BYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = piece[n];
         }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         __syncwarp();

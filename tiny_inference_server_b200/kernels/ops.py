@@ -999,15 +999,16 @@ def shared_attention_library(head_dim: int):
     return lib
 
 
-def _split_parts(items: int, tiles: int, resident: int, start: float, most: int = 64) -> int:
+def _split_parts(items: int, tiles: int, resident: int, start: float, join: float = 0.0, most: int = 64) -> int:
     """Parts that ``tiles`` of keys are split into, for ``items`` (row heads, kv head) of which ``resident`` are worked on at a time: the
-    fewest rounds of the longest part, an item costing ``start`` tiles beside its own and a part a tenth of one to join."""
+    fewest rounds of the longest part, an item costing ``start`` tiles beside its own, a part a tenth of one to join, and more than one part
+    ``join`` of them."""
     best, cost = 1, None
     for parts in range(1, min(tiles, most) + 1):
         per = -(-tiles // parts)
         if -(-tiles // per) != parts:
             continue
-        c = -(-items * parts // resident) * (per + start) + 0.1 * parts
+        c = -(-items * parts // resident) * (per + start) + 0.1 * parts + (join if parts > 1 else 0.0)
         if cost is None or c < cost - 1e-9:
             best, cost = parts, c
     return best
@@ -1071,7 +1072,7 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
             shared_parts = _split_parts(n_wide * kvh, -(-shared // 128), 148, 4)
         else:
             shared_parts = _split_parts(n_wide * kvh, -(-shared // 64), 2 * 148, 4)
-        own_parts = _split_parts(n_own * kvh, own_tiles, (2 if hd <= 128 else 1) * 148, 1)
+        own_parts = _split_parts(n_own * kvh, own_tiles, (2 if hd <= 128 else 1) * 148, 1, 8 if code else 0)
         if len(plan.splits) > 256:
             plan.splits.clear()
         split = plan.splits[key] = (tensor, wide_rows, plan.shared[wide_rows], n_wide, shared_parts, own_parts)
