@@ -321,22 +321,27 @@ template <int NT, int SP, int AHEAD> int w4_forms(const W4Params& p, int slabs, 
 }  // namespace
 
 // out (rows, N) = x (rows, K) times the packed weights; dtype is that of x and out, rows of both contiguous, row strides free.
-TIS_API int tis_gemm_w4(int dtype, const void* x, long long ldx, const void* words, const void* scales, const void* zeros, void* out,
-                        long long ldo, int rows, int K, int N, int group, cudaStream_t stream) {
+struct W4Args { long long dtype, x, ldx, words, scales, zeros, out, ldo, rows, K, N, group, stream; };
+TIS_API int tis_gemm_w4(const W4Args* a) {
+    if (a->K <= 0 || a->K > (1 << 30) || a->N > (1 << 30) || a->rows > (1 << 30) || a->group < 32 || a->group > (1 << 30) ||
+        (a->group & (a->group - 1)) != 0 || a->K * a->N > (1ll << 36)) {
+        tis_set_error("gemm_w4: %lld rows, %lld x %lld in groups of %lld", a->rows, a->K, a->N, a->group);
+        return TIS_BAD_SIZE;
+    }
+    const int dtype = (int)a->dtype, rows = (int)a->rows, K = (int)a->K, N = (int)a->N, group = (int)a->group;
+    const void* x = reinterpret_cast<const void*>(a->x);
+    const long long ldx = a->ldx;
+    const cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
     if (rows <= 0 || N <= 0) return TIS_OK;
     if (dtype != TIS_F32 && dtype != TIS_BF16) {
         tis_set_error("gemm_w4: dtype code %d", dtype);
         return TIS_BAD_DTYPE;
     }
-    if (K <= 0 || K > (1 << 30) || N > (1 << 30) || group < 32 || (group & (group - 1)) != 0) {
-        tis_set_error("gemm_w4: %d x %d in groups of %d", K, N, group);
-        return TIS_BAD_SIZE;
-    }
     W4Params p = {};
-    p.words = static_cast<const uint4*>(words);
-    p.scales = static_cast<const unsigned*>(scales);
-    p.zeros = static_cast<const unsigned short*>(zeros);
-    p.x = x; p.ldx = ldx; p.out = out; p.ldo = ldo;
+    p.words = reinterpret_cast<const uint4*>(a->words);
+    p.scales = reinterpret_cast<const unsigned*>(a->scales);
+    p.zeros = reinterpret_cast<const unsigned short*>(a->zeros);
+    p.x = x; p.ldx = ldx; p.out = reinterpret_cast<void*>(a->out); p.ldo = a->ldo;
     p.rows = rows; p.K = K; p.N = N;
     p.chunks = (K + W4_CHUNK - 1) / W4_CHUNK;
     p.strips = (N + W4_STRIP - 1) / W4_STRIP;

@@ -727,20 +727,34 @@ TIS_API int tis_shared_attn_widest() { return HD <= 128 ? 128 : 64; }
 // The first `shared_parts` parts of the scratch are the shared tiles', the `own_parts` behind them the own ones'; rows of groups
 // without shared keys have empty ones.  `rows`: the rows of the plan, all of which are written.
 TIS_API int tis_shared_attn_tensor(int page) { return shared_tc_takes(page); }
-TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* out, long long ldo, const void* plane, const int* table,
-                                 int table_stride, int table_width, int num_pages, const int* positions, const void* own, int own_count,
-                                 const void* wide, int wide_count, int wide_rows, int tensor, int own_parts, int shared_parts, int rows, int H, int KVH, int page,
-                                 float scale, float* part_o, void* part_ml, int* fault, cudaStream_t stream) {
-    if (rows <= 0) return TIS_OK;
+struct SharedArgs {
+    long long dtype, q, ldq, out, ldo, plane, table, table_stride, table_width, num_pages, positions, own, own_count, wide, wide_count, wide_rows,
+        tensor, own_parts, shared_parts, rows, H, KVH, page, part_o, part_ml, fault, stream, unused;
+    double scale;
+};
+TIS_API int tis_shared_attention(const SharedArgs* a) {
+    if (a->rows <= 0) return TIS_OK;
+    const long long most = 1ll << 30;
+    if (a->table_stride > most || a->table_width > most || a->num_pages > most || a->page > most || a->rows * a->H > most ||
+        a->own_count * a->own_parts * a->KVH > most || a->wide_count * a->shared_parts * a->KVH > most) {
+        tis_set_error("shared_prefix_attention: %lld rows of %lld heads, %lld pages of %lld, tables of %lld", a->rows, a->H, a->num_pages, a->page, a->table_width);
+        return TIS_BAD_SIZE;
+    }
+    const int dtype = (int)a->dtype, rows = (int)a->rows, H = (int)a->H, KVH = (int)a->KVH, page = (int)a->page, num_pages = (int)a->num_pages;
+    const int own_count = (int)a->own_count, wide_count = (int)a->wide_count, wide_rows = (int)a->wide_rows, tensor = (int)a->tensor;
+    const int own_parts = (int)a->own_parts, shared_parts = (int)a->shared_parts;
+    void* out = reinterpret_cast<void*>(a->out);
+    const long long ldo = a->ldo;
+    const cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
     SharedParams p;
-    p.q = q; p.ldq = ldq; p.plane = plane;
-    p.table = table; p.table_stride = table_stride; p.table_width = table_width; p.num_pages = num_pages;
-    p.positions = positions;
-    p.part_o = part_o; p.part_ml = static_cast<float2*>(part_ml);
+    p.q = reinterpret_cast<const void*>(a->q); p.ldq = a->ldq; p.plane = reinterpret_cast<const void*>(a->plane);
+    p.table = reinterpret_cast<const int*>(a->table); p.table_stride = (int)a->table_stride; p.table_width = (int)a->table_width; p.num_pages = num_pages;
+    p.positions = reinterpret_cast<const int*>(a->positions);
+    p.part_o = reinterpret_cast<float*>(a->part_o); p.part_ml = reinterpret_cast<float2*>(a->part_ml);
     p.rows = rows; p.H = H; p.KVH = KVH; p.page = page; p.own_parts = own_parts; p.shared_parts = shared_parts;
     p.out = out; p.ldo = ldo; p.out_vectors = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo % 8 == 0;
-    p.scale_log2 = scale * 1.4426950408889634f;
-    p.fault = fault;
+    p.scale_log2 = (float)(a->scale * 1.4426950408889634);
+    p.fault = reinterpret_cast<int*>(a->fault);
     if (wide_rows != 16 && (dtype == TIS_F32 || wide_rows > tis_shared_attn_widest() || (wide_rows != 64 && wide_rows != 128))) {
         tis_set_error("shared_prefix_attention: shared tiles of %d row heads", wide_rows);
         return TIS_BAD_SIZE;
@@ -749,8 +763,8 @@ TIS_API int tis_shared_attention(int dtype, const void* q, long long ldq, void* 
         tis_set_error("shared_prefix_attention: %d and %d parts, pages of %d", own_parts, shared_parts, page);
         return TIS_BAD_SIZE;
     }
-    const SharedTile* o = static_cast<const SharedTile*>(own);
-    const SharedTile* w = static_cast<const SharedTile*>(wide);
+    const SharedTile* o = reinterpret_cast<const SharedTile*>(a->own);
+    const SharedTile* w = reinterpret_cast<const SharedTile*>(a->wide);
     const int parts = own_parts + shared_parts, row_heads = rows * H;
     int status = TIS_OK;
     if (dtype == TIS_F32) {

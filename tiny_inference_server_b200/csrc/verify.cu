@@ -298,11 +298,18 @@ template <int N> int verify_launch(const cudaLaunchConfig_t& cfg, const VerifyPa
 
 // n requests of up to k drafts over V tokens.  p: rows p + b p_request + i p_row (i <= k) of V floats; q likewise (i < k; null: none);
 // drafts [n][k], u [n][k + 1], lens [n] (null: k each); tokens [n][k + 1]: the kept drafts, the drawn token (-1: no mass), -1 behind.
-TIS_API int tis_verify_drafts(const float* p, long long p_request, long long p_row, const float* q, long long q_request,
-                              long long q_row, const int* drafts, const float* u, const int* lens, int* tokens, int* accepted,
-                              int n, int k, int V, cudaStream_t stream) {
+struct VerifyArgs { long long p, p_request, p_row, q, q_request, q_row, drafts, u, lens, tokens, accepted, n, k, V, stream; };
+TIS_API int tis_verify_drafts(const VerifyArgs* a) {
+    const float* p = reinterpret_cast<const float*>(a->p);
+    const float* q = reinterpret_cast<const float*>(a->q);
+    const cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
+    if (a->V > (1 << 30) || a->n > (1 << 30) || a->k > VERIFY_MAX_DRAFTS) {
+        tis_set_error("verify_drafts: %lld requests of %lld drafts, vocabulary of %lld", a->n, a->k, a->V);
+        return TIS_BAD_SIZE;
+    }
+    const int n = (int)a->n, k = (int)a->k, V = (int)a->V;
     if (n <= 0) return TIS_OK;
-    if (k < 0 || k > VERIFY_MAX_DRAFTS || V <= 0 || V > (1 << 30)) {
+    if (k < 0 || V <= 0) {
         tis_set_error("verify_drafts: %d drafts, vocabulary of %d", k, V);
         return TIS_BAD_SIZE;
     }
@@ -316,7 +323,9 @@ TIS_API int tis_verify_drafts(const float* p, long long p_request, long long p_r
         return TIS_BAD_SIZE;
     }
     const long long runs = (long long)ranks * VERIFY_WARPS, run = (V + runs - 1) / runs;
-    VerifyParams v{p, p_request, p_row, q, q_request, q_row, drafts, u, lens, tokens, accepted, k, V};
+    VerifyParams v{p, a->p_request, a->p_row, q, a->q_request, a->q_row, reinterpret_cast<const int*>(a->drafts),
+                   reinterpret_cast<const float*>(a->u), reinterpret_cast<const int*>(a->lens), reinterpret_cast<int*>(a->tokens),
+                   reinterpret_cast<int*>(a->accepted), k, V};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n * ranks));
     cfg.blockDim = dim3(VERIFY_THREADS);

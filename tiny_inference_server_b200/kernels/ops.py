@@ -12,6 +12,7 @@ import collections
 import ctypes
 import math
 import os
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -31,9 +32,11 @@ class KernelError(RuntimeError):
     pass
 
 
-#: argument kinds of launchers whose pointers are passed as plain numbers: p a pointer, i an int, l a 64-bit int, f a float
-_ARGUMENTS = {"tis_verify_drafts": "pllpllpppppiiip", "tis_gemm_w4": "iplppppliiiip"}
-_KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+#: layouts of the arguments of launchers that take them as one block of 64-bit values (q: whole, d: floating point): a call with
+#: twenty arguments costs ctypes 2.5 us, the same packed 0.9
+_VERIFY_ARGS = struct.Struct("15q")
+_W4_ARGS = struct.Struct("13q")
+_SHARED_ARGS = struct.Struct("28qd")
 
 
 def library():
@@ -52,8 +55,7 @@ def library():
     lib.tis_last_error.restype = ctypes.c_char_p
     lib.tis_abi_version.restype = ctypes.c_int
     lib.tis_chunked_recurrence_floats.restype = ctypes.c_size_t
-    for name, kinds in _ARGUMENTS.items():
-        getattr(lib, name).argtypes = [_KINDS[c] for c in kinds]
+    lib.tis_verify_drafts.argtypes = lib.tis_gemm_w4.argtypes = [ctypes.c_char_p]
     if lib.tis_abi_version() != ABI_VERSION:
         raise KernelError(f"{path}: launcher interface {lib.tis_abi_version()}, expected {ABI_VERSION}")
     _lib = lib
@@ -96,21 +98,21 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _stream_number(device: int) -> int:
+    """torch's current CUDA stream of a device as a number, for packed arguments."""
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def _f(x: float):
     return ctypes.c_float(x)
 
 
-def _on_this_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """A launch goes to the current device: raise for a tensor that lies elsewhere."""
-    device = -1
-    for t in tensors:
-        if t is not None:
-            if not t.is_cuda:
-                raise KernelError(f"{what}: a tensor on {t.device}; the kernels take CUDA tensors")
-            if device < 0:
-                device = _current_device()
-            if t.get_device() != device:
-                raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{device}")
+def _elsewhere(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raise for tensors that do not all lie on the current device, where a launch goes to."""
+    places = sorted({str(t.device) for t in tensors if t is not None})
+    if any(t is not None and not t.is_cuda for t in tensors):
+        raise KernelError(f"{what}: tensors on {', '.join(places)}; the kernels take CUDA tensors")
+    raise KernelError(f"{what}: tensors on {', '.join(places)}, the current device is cuda:{_current_device()}")
 
 
 # ---------------------------------------------------------------------------------------
@@ -663,23 +665,32 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
 
     For few rows: the weights are streamed once for up to 64 rows of bfloat16 and 21 of float32, and again for as many more.  (A prompt's rows
     are better off with ``weights.w4.unpack_w4`` and ``gemm``.)"""
-    words = w.words
-    n, k = a.shape
     dtype = a.dtype
-    if k != w.k or (dtype is not torch.bfloat16 and dtype is not torch.float32) or (k > 1 and a.stride(1) != 1):
-        raise KernelError(f"gemm_w4: rows {dtype} {tuple(a.shape)} (bfloat16 or float32, contiguous) for weights {w.k} x {w.n}")
+    if (dtype is not torch.bfloat16 and dtype is not torch.float32) or a.ndim != 2:
+        raise KernelError(f"gemm_w4: rows {dtype} {tuple(a.shape)}; bfloat16 or float32 are taken")
+    n, k = a.shape
+    lda, unit = a.stride()
+    if k != w.k or (unit != 1 and k > 1):
+        raise KernelError(f"gemm_w4: rows {tuple(a.shape)}, strides {a.stride()}, for weights {w.k} x {w.n}")
+    cols = w.n
     if out is None:
-        out = torch.empty((n, w.n), dtype=dtype, device=a.device)
-    elif out.dtype is not dtype or out.shape != (n, w.n) or (w.n > 1 and out.stride(1) != 1):
-        raise KernelError(f"gemm_w4: result {out.dtype} {tuple(out.shape)} for {n} rows of {dtype} and weights {w.k} x {w.n}")
-    _on_this_device("gemm_w4", a, out, words)
+        out, ldo = torch.empty((n, cols), dtype=dtype, device=a.device), cols
+    else:
+        if out.dtype is not dtype or out.shape != (n, cols):
+            raise KernelError(f"gemm_w4: result {out.dtype} {tuple(out.shape)} for {n} rows of {dtype} and weights {w.k} x {cols}")
+        ldo, unit = out.stride()
+        if unit != 1 and cols > 1:
+            raise KernelError("gemm_w4: a row of the result is contiguous")
+    device = a.get_device()
+    if device < 0 or out.get_device() != device or w.place != device or _current_device() != device:
+        _elsewhere("gemm_w4", a, out, w.words)
     if n == 0:
         return out
-    lib = library()
+    lib = _lib or library()
     calls["gemm_w4"] += 1
-    _check(lib.tis_gemm_w4(_dt(a), a.data_ptr(), a.stride(0), words.data_ptr(), w.scales.data_ptr(),
-                           None if w.zeros is None else w.zeros.data_ptr(), out.data_ptr(), out.stride(0), n, k, w.n, w.group,
-                           _stream()), lib)
+    words, scales, zeros = w.pointers
+    _check(lib.tis_gemm_w4(_W4_ARGS.pack(1 if dtype is torch.bfloat16 else 0, a.data_ptr(), lda, words, scales, zeros, out.data_ptr(), ldo, n, k,
+                                         cols, w.group, _stream_number(device))), lib)
     return out
 
 
@@ -991,7 +1002,7 @@ def shared_attention_library(head_dim: int):
         library()
         lib = ctypes.CDLL(_build.build_shared_attention(head_dim))
         lib.tis_last_error.restype = ctypes.c_char_p
-        lib.tis_shared_attention.argtypes = [_KINDS[c] for c in "iplplppiiippipiiiiiiiiifpppp"]
+        lib.tis_shared_attention.argtypes = [ctypes.c_char_p]
         lib.widest = lib.tis_shared_attn_widest()
         if lib.tis_shared_attn_head_dim() != head_dim:
             raise KernelError(f"attention library built for head size {lib.tis_shared_attn_head_dim()}, wanted {head_dim}")
@@ -1029,39 +1040,48 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     ``max_position`` (no row's position is larger; the tables' width unless given) decides only how the requests' own keys are split.
     ``scale`` multiplies the scores (1 / sqrt(hd) unless given).  bfloat16 or float32 (all in 32 bits), any page size, hd a
     multiple of 16 up to 256.  A page that is not there sets ``fault``, as in ``paged_attention``."""
-    if plane.dim() != 5 or plane.shape[1] != 2 or not plane.is_contiguous():
-        raise KernelError(f"shared_prefix_attention: a cache plane [pages, 2, kv heads, page, head size], not {tuple(plane.shape)}")
-    pages, _, kvh, page, hd = plane.shape
-    h, rows = plan.num_heads, plan.rows
     dtype = q.dtype
-    if dtype is not plane.dtype or dtype is not out.dtype:
-        raise KernelError(f"shared_prefix_attention: queries {dtype}, cache {plane.dtype}, results {out.dtype}")
-    if kvh != plan.kv_heads or pages < 1 or page < 1 or hd % 16 or not 16 <= hd <= 256:
-        raise KernelError(f"shared_prefix_attention: a plan for {plan.kv_heads} kv heads, a cache plane {tuple(plane.shape)}")
-    if q.dim() != 2 or out.dim() != 2 or q.shape[0] < rows or out.shape[0] < rows or q.shape[1] < h * hd or out.shape[1] < h * hd:
-        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)}, results {tuple(out.shape)} for {rows} rows of {h} heads of {hd}")
-    if q.stride(1) != 1 or out.stride(1) != 1 or (dtype is torch.bfloat16 and (q.stride(0) % 8 or q.data_ptr() % 16)) or plane.data_ptr() % 16:
-        raise KernelError("shared_prefix_attention: rows are contiguous; in bfloat16 queries start on 16 bytes")
-    if (positions.dtype is not torch.int32 or positions.numel() < rows or not positions.is_contiguous() or fault.dtype is not torch.int32
-            or fault.numel() < 1 or block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1
-            or block_table.shape[0] <= plan.max_slot or block_table.shape[1] < 1):
+    if plane.ndim != 5 or q.ndim != 2 or out.ndim != 2 or block_table.ndim != 2 or plane.dtype is not dtype or out.dtype is not dtype:
+        raise KernelError(f"shared_prefix_attention: queries {dtype} {tuple(q.shape)}, results {out.dtype} {tuple(out.shape)}, cache {plane.dtype} "
+                          f"{tuple(plane.shape)}: matrices, and a plane [pages, 2, kv heads, page, head size], of one type")
+    pages, two, kvh, page, hd = plane.shape
+    h, rows = plan.num_heads, plan.rows
+    if two != 2 or kvh != plan.kv_heads or pages < 1 or page < 1 or hd % 16 or not 16 <= hd <= 256 or not plane.is_contiguous():
+        raise KernelError(f"shared_prefix_attention: a plan for {plan.kv_heads} kv heads, a cache plane {tuple(plane.shape)} (contiguous; head "
+                          "sizes that are multiples of 16 up to 256)")
+    n, width = q.shape
+    ldq, unit = q.stride()
+    n_out, width_out = out.shape
+    ldo, unit_out = out.stride()
+    if n < rows or n_out < rows or width < h * hd or width_out < h * hd or unit != 1 or unit_out != 1:
+        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)}, results {tuple(out.shape)} (rows contiguous) for {rows} rows of {h} "
+                          f"heads of {hd}")
+    q_at, plane_at = q.data_ptr(), plane.data_ptr()
+    code = 1 if dtype is torch.bfloat16 else 0
+    if (plane_at | (q_at | 2 * ldq if code else 0)) % 16 or (not code and dtype is not torch.float32):
+        raise KernelError(f"shared_prefix_attention: bfloat16 or float32, not {dtype}; the cache and in bfloat16 the rows of queries start on 16 bytes")
+    slots, width = block_table.shape
+    table_stride, unit = block_table.stride()
+    i32 = torch.int32
+    if (positions.dtype is not i32 or block_table.dtype is not i32 or fault.dtype is not i32 or positions.numel() < rows or fault.numel() < 1
+            or unit != 1 or slots <= plan.max_slot or width < 1 or not positions.is_contiguous()):
         raise KernelError(f"shared_prefix_attention: positions {positions.dtype} {tuple(positions.shape)} for {rows} rows, tables "
-                          f"{block_table.dtype} {tuple(block_table.shape)} for slots up to {plan.max_slot}")
-    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+                          f"{block_table.dtype} {tuple(block_table.shape)} for slots up to {plan.max_slot}, fault {fault.dtype}: int32, contiguous")
+    scale = hd ** -0.5 if scale is None else float(scale)
     if not 0 < scale < math.inf:
         raise KernelError(f"shared_prefix_attention: the scores are multiplied by a positive number, not {scale}")
-    code = _dt(q)
-    _on_this_device("shared_prefix_attention", q, out, plane, block_table, positions, plan.own, fault)
-    lib = shared_attention_library(hd)
-    width = block_table.shape[1]
-    n_own = plan.own.shape[0]
-    shared = plan.max_shared // page * page
+    device = q.get_device()
+    if (device < 0 or out.get_device() != device or plane.get_device() != device or block_table.get_device() != device
+            or positions.get_device() != device or plan.place != device or fault.get_device() != device or _current_device() != device):
+        _elsewhere("shared_prefix_attention", q, out, plane, block_table, positions, plan.own, fault)
+    lib = _shared_attn_libs.get(hd) or shared_attention_library(hd)
     own_tiles = max(1, -(-((width * page if max_position is None else max_position + 1) - plan.min_shared // page * page) // 64))
     # how the keys are split: found once for a plan and as long as the own keys stay within the same 64
     tensor = code == 1 and TC_ATTENTION and 2 * pages * kvh * page < 1 << 31
     key = (hd, page, code, tensor, own_tiles)
     split = plan.splits.get(key)
     if split is None:
+        n_own, shared = plan.own.shape[0], plan.max_shared // page * page
         tensor = int(tensor and lib.tis_shared_attn_tensor(page))
         # shared tiles of the row heads that the groups have, as far as the kernels go
         wide_rows = 128 if tensor else (16 if code == 0 or plan.most_heads <= 16 else (64 if plan.most_heads <= 64 else lib.widest))
@@ -1075,16 +1095,15 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
         own_parts = _split_parts(n_own * kvh, own_tiles, (2 if hd <= 128 else 1) * 148, 1, 8 if code else 0)
         if len(plan.splits) > 256:
             plan.splits.clear()
-        split = plan.splits[key] = (tensor, wide_rows, plan.shared[wide_rows], n_wide, shared_parts, own_parts)
-    tensor, wide_rows, wide, n_wide, shared_parts, own_parts = split
-    parts, row_heads = shared_parts + own_parts, rows * h
-    scratch = torch.empty(parts * row_heads * (hd + 2), dtype=torch.float32, device=q.device)
+        split = plan.splits[key] = ((shared_parts + own_parts) * rows * h, plan.own.data_ptr(), n_own, plan.shared[wide_rows].data_ptr(), n_wide,
+                                    wide_rows, tensor, own_parts, shared_parts)
+    part_rows = split[0]
+    scratch = torch.empty(part_rows * (hd + 2), dtype=torch.float32, device=q.device)
     calls["shared_prefix_attention"] += 1
     at = scratch.data_ptr()
-    _check(lib.tis_shared_attention(code, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), plane.data_ptr(), block_table.data_ptr(),
-                                    block_table.stride(0), width, pages, positions.data_ptr(), plan.own.data_ptr(), n_own, wide.data_ptr(),
-                                    n_wide, wide_rows, tensor, own_parts, shared_parts, rows, h, kvh, page, scale, at, at + 4 * parts * row_heads * hd,
-                                    fault.data_ptr(), _stream()), lib)
+    _check(lib.tis_shared_attention(_SHARED_ARGS.pack(code, q_at, ldq, out.data_ptr(), ldo, plane_at, block_table.data_ptr(), table_stride, width,
+                                                      pages, positions.data_ptr(), *split[1:], rows, h, kvh, page, at, at + 4 * part_rows * hd,
+                                                      fault.data_ptr(), _stream_number(device), 0, scale)), lib)
     return out
 
 
@@ -2025,42 +2044,50 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
     nothing is left of the difference; without a distribution ``q_i`` is one at the draft) and over the target's row behind the last
     draft.  Entries that are not positive numbers have no mass; a row without mass gives the token -1.  A draft outside the
     vocabulary is not kept.  Computed in 64 bits: the tokens do not depend on how the work is shared out."""
+    f32, i32 = torch.float32, torch.int32
+    if target_probs.dtype is not f32 or uniforms.dtype is not f32 or drafts.dtype is not i32 or target_probs.ndim != 3:
+        raise KernelError(f"verify_drafts: float32 probabilities (n, k + 1, V) and numbers and int32 drafts are taken, not "
+                          f"{target_probs.dtype} {tuple(target_probs.shape)}, {uniforms.dtype}, {drafts.dtype}")
     n, k1, v = target_probs.shape
     k = k1 - 1
-    f32, i32 = torch.float32, torch.int32
-    if target_probs.dtype != f32 or uniforms.dtype != f32 or drafts.dtype != i32 or k1 < 1 or v < 1 or k > VERIFY_MAX_DRAFTS:
-        raise KernelError(f"verify_drafts: float32 probabilities and numbers, int32 drafts, up to {VERIFY_MAX_DRAFTS} drafts, not "
-                          f"{target_probs.dtype} {tuple(target_probs.shape)}, {uniforms.dtype}, {drafts.dtype}")
-    if drafts.shape != (n, k) or uniforms.shape != (n, k1) or (draft_lens is not None and draft_lens.shape != (n,)):
-        raise KernelError(f"verify_drafts: drafts {tuple(drafts.shape)}, numbers {tuple(uniforms.shape)} for probabilities "
-                          f"{tuple(target_probs.shape)}")
-    if target_probs.stride(2) != 1 and v > 1:
+    if k < 0 or v < 1 or k > VERIFY_MAX_DRAFTS or drafts.shape != (n, k) or uniforms.shape != (n, k1):
+        raise KernelError(f"verify_drafts: up to {VERIFY_MAX_DRAFTS} drafts; drafts {tuple(drafts.shape)}, numbers {tuple(uniforms.shape)} for "
+                          f"probabilities {tuple(target_probs.shape)}")
+    p_request, p_row, unit = target_probs.stride()
+    q = q_request = q_row = 0
+    if draft_probs is not None:
+        if draft_probs.dtype is not f32 or draft_probs.shape != (n, k, v):
+            raise KernelError(f"verify_drafts: draft probabilities {draft_probs.dtype} {tuple(draft_probs.shape)} for {tuple(target_probs.shape)}")
+        q_request, q_row, q_unit = draft_probs.stride()
+        unit = unit if q_unit == 1 or k == 0 else q_unit
+        q = draft_probs.data_ptr() if k else 0
+    if unit != 1 and v > 1:
         raise KernelError("verify_drafts: a row of probabilities is contiguous")
-    if draft_probs is not None and (draft_probs.dtype != f32 or draft_probs.shape != (n, k, v) or (draft_probs.stride(2) != 1 and v > 1)):
-        raise KernelError(f"verify_drafts: draft probabilities {draft_probs.dtype} {tuple(draft_probs.shape)} for {tuple(target_probs.shape)}")
-    device = target_probs.device
+    device = target_probs.get_device()
     if tokens is None:
-        tokens = torch.empty((n, k1), dtype=i32, device=device)
+        tokens = torch.empty((n, k1), dtype=i32, device=target_probs.device)
     if accepted is None:
-        accepted = torch.empty(n, dtype=i32, device=device)
-    if tokens.shape != (n, k1) or accepted.shape != (n,) or tokens.dtype != i32 or accepted.dtype != i32:
+        accepted = torch.empty(n, dtype=i32, device=target_probs.device)
+    if tokens.dtype is not i32 or accepted.dtype is not i32 or tokens.shape != (n, k1) or accepted.shape != (n,):
         raise KernelError(f"verify_drafts: results {tuple(tokens.shape)} {tokens.dtype}, {tuple(accepted.shape)} {accepted.dtype}")
     if not (drafts.is_contiguous() and uniforms.is_contiguous() and tokens.is_contiguous() and accepted.is_contiguous()):
         raise KernelError("verify_drafts: drafts, numbers and results are contiguous")
-    if draft_lens is not None and (draft_lens.dtype != i32 or not draft_lens.is_contiguous()):
-        raise KernelError("verify_drafts: numbers of drafts are contiguous int32")
-    _on_this_device("verify_drafts", target_probs, draft_probs, drafts, uniforms, draft_lens, tokens, accepted)
+    lens = 0
+    if draft_lens is not None:
+        if draft_lens.dtype is not i32 or draft_lens.shape != (n,) or not draft_lens.is_contiguous():
+            raise KernelError(f"verify_drafts: numbers of drafts {draft_lens.dtype} {tuple(draft_lens.shape)}; contiguous int32 ({n},) is taken")
+        lens = draft_lens.data_ptr()
+    if (device < 0 or drafts.get_device() != device or uniforms.get_device() != device or tokens.get_device() != device
+            or accepted.get_device() != device or _current_device() != device or (lens and draft_lens.get_device() != device)
+            or (q and draft_probs.get_device() != device)):
+        _elsewhere("verify_drafts", target_probs, draft_probs, drafts, uniforms, draft_lens, tokens, accepted)
     if n == 0:
         return tokens, accepted
-    lib = library()
-    if draft_probs is not None and k:
-        q, q_request, q_row = draft_probs.data_ptr(), draft_probs.stride(0), draft_probs.stride(1)
-    else:
-        q, q_request, q_row = None, 0, 0
+    lib = _lib or library()
     calls["verify_drafts"] += 1
-    _check(lib.tis_verify_drafts(target_probs.data_ptr(), target_probs.stride(0), target_probs.stride(1), q, q_request, q_row,
-                                 drafts.data_ptr(), uniforms.data_ptr(), draft_lens.data_ptr() if draft_lens is not None else None,
-                                 tokens.data_ptr(), accepted.data_ptr(), n, k, v, _stream()), lib)
+    _check(lib.tis_verify_drafts(_VERIFY_ARGS.pack(target_probs.data_ptr(), p_request, p_row, q, q_request, q_row, drafts.data_ptr(),
+                                                   uniforms.data_ptr(), lens, tokens.data_ptr(), accepted.data_ptr(), n, k, v,
+                                                   _stream_number(device))), lib)
     return tokens, accepted
 
 

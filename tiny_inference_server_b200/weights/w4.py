@@ -32,6 +32,11 @@ class W4Weights:
     n: int
     group: int
 
+    def __post_init__(self):
+        # what a launch takes, found once: the weights stay where they are
+        object.__setattr__(self, "place", self.words.get_device())
+        object.__setattr__(self, "pointers", (self.words.data_ptr(), self.scales.data_ptr(), 0 if self.zeros is None else self.zeros.data_ptr()))
+
     @property
     def shape(self) -> Tuple[int, int]:
         return self.k, self.n
