@@ -54,8 +54,8 @@ def test_words_of_a_lane():
     codes, scales, _ = make(128, 48, 64, False)
     w = pack_w4(codes, scales, None, 64)
     for strip, chunk, lane, word in ((0, 0, 0, 0), (1, 1, 13, 3), (2, 0, 31, 2), (2, 1, 6, 1)):
-        g, t, h, j = lane // 4, lane % 4, word // 2, word % 2
-        k0, c = 64 * chunk + 32 * h + 8 * t + 4 * j, 16 * strip + g
+        g, t = lane // 4, lane % 4
+        k0, c = 64 * chunk + 16 * word + 4 * t, 16 * strip + g
         want = [codes[k0, c], codes[k0, c + 8], codes[k0 + 2, c], codes[k0 + 2, c + 8],
                 codes[k0 + 1, c], codes[k0 + 1, c + 8], codes[k0 + 3, c], codes[k0 + 3, c + 8]]
         v = int(w.words[strip, chunk, lane, word])

@@ -12,26 +12,16 @@
 //
 // A CTA of eight warps takes a few strips of 16 columns; its warps share them out (`ws` of them side by side) and the chunks of
 // 64 entries of the sum (`wk` of them take turns), and add up in shared memory, in a fixed order.  x waits in shared memory, whole or in
-// stages; its rows lie 64 bytes off a multiple of 128 apart, so that the eight rows x four pieces of 16 bytes that a warp reads at a time
+// stages; its rows lie 32 bytes off a multiple of 128 apart, so that the four rows x four pieces of 8 bytes that half a warp reads at a time
 // are free of bank conflicts.
-#include "common.cuh"
+#include "gemm_w4.cuh"
 
 namespace {
 
 constexpr int W4_THREADS = 256, W4_WARPS = 8;
-constexpr int W4_STRIP = 16, W4_CHUNK = 64;
-constexpr int W4_PAD = 32;                  // elements behind a staged row
+constexpr int W4_PAD = 16;                  // elements behind a staged row
 constexpr int W4_ROWS = 64;                 // rows of a slab in bfloat16
 constexpr int W4_ROWS_F32 = 21;             // and in float32, three numbers each
-
-struct W4Params {
-    const uint4* words; const unsigned* scales; const unsigned short* zeros;
-    const void* x; long long ldx;
-    void* out; long long ldo;
-    int rows, slab, K, N, chunks, strips, groups, group_shift;      // group_shift: log2 of the halves of a chunk in a group
-    int ws, wk, stage_chunks, stages;
-    bool f32, vectors;
-};
 
 __device__ __forceinline__ uint4 load_stream(const uint4* p) {
     uint4 v;
@@ -42,12 +32,6 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const unsigned (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// two codes (bits 0-3 and 16-19 of w) less their zero point; `base` is 128 + zero in both halves
-__device__ __forceinline__ unsigned weight_pair(unsigned w, unsigned base) {
-    const unsigned v = (w & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&base));
-    return *reinterpret_cast<const unsigned*>(&d);
 }
 __device__ __forceinline__ float low_half(unsigned v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high_half(unsigned v) { return __uint_as_float(v & 0xffff0000u); }
@@ -196,7 +180,7 @@ w4_kernel(const W4Params p) {
                 }
                 staged = p.stages == 1;
             }
-            const bf16* x_lane = x_smem + now * buffer + (size_t)g * stride + t * 8 + turn * W4_CHUNK;
+            const bf16* x_lane = x_smem + now * buffer + (size_t)g * stride + t * 4 + turn * W4_CHUNK;
             // (chunks of the stage: per_stage of this warp's, in steps of AHEAD, per_stage being a multiple of that where there are several stages)
             for (int i = stage * per_stage; i < min(mine, (stage + 1) * per_stage); i += AHEAD) {
 #pragma unroll
@@ -208,9 +192,11 @@ w4_kernel(const W4Params p) {
                     float sum[SP][NT][4];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        uint4 x[NT];
+                        uint2 x[NT][2];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) x[n] = *reinterpret_cast<const uint4*>(xc + (size_t)n * 8 * stride + 32 * h);
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) x[n][j] = *reinterpret_cast<const uint2*>(xc + (size_t)n * 8 * stride + 32 * h + 16 * j);
                         if (h == 0 || HALVES) {
 #pragma unroll
                             for (int s = 0; s < SP; ++s)
@@ -227,10 +213,10 @@ w4_kernel(const W4Params p) {
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
                                 const unsigned w = h ? (j ? it.w[s].w : it.w[s].z) : (j ? it.w[s].y : it.w[s].x);
-                                const unsigned a[4] = {weight_pair(w, low), weight_pair(w >> 4, high),
-                                                       weight_pair(w >> 8, low), weight_pair(w >> 12, high)};
+                                const unsigned a[4] = {w4_pair(w, low), w4_pair(w >> 4, high),
+                                                       w4_pair(w >> 8, low), w4_pair(w >> 12, high)};
 #pragma unroll
-                                for (int n = 0; n < NT; ++n) mma_bf16(sum[s][n], a, j ? x[n].z : x[n].x, j ? x[n].w : x[n].y);
+                                for (int n = 0; n < NT; ++n) mma_bf16(sum[s][n], a, x[n][j].x, x[n][j].y);
                             }
                             if (h == 1 || HALVES) {
                                 const unsigned sc = it.s[s][HALVES ? h : 0];
@@ -321,7 +307,7 @@ template <int NT, int SP, int AHEAD> int w4_forms(const W4Params& p, int slabs, 
 }  // namespace
 
 // out (rows, N) = x (rows, K) times the packed weights; dtype is that of x and out, rows of both contiguous, row strides free.
-struct W4Args { long long dtype, x, ldx, words, scales, zeros, out, ldo, rows, K, N, group, stream; };
+struct W4Args { long long dtype, x, ldx, words, scales, zeros, out, ldo, rows, K, N, group, tensor, fault, stream; };
 TIS_API int tis_gemm_w4(const W4Args* a) {
     if (a->K <= 0 || a->K > (1 << 30) || a->N > (1 << 30) || a->rows > (1 << 30) || a->group < 32 || a->group > (1 << 30) ||
         (a->group & (a->group - 1)) != 0 || a->K * a->N > (1ll << 36)) {
@@ -349,6 +335,13 @@ TIS_API int tis_gemm_w4(const W4Args* a) {
     for (int h = group / 32; h > 1; h >>= 1) ++p.group_shift;
     p.f32 = dtype == TIS_F32;
     p.vectors = K % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (p.f32 ? 4 : 8) == 0;
+    if (a->tensor) {
+        if (p.f32 || rows > W4_ROWS || !p.vectors) {
+            tis_set_error("gemm_w4: %d rows, %s, are not for the tcgen05 kernel", rows, p.f32 ? "float32" : "bfloat16");
+            return TIS_BAD_SIZE;
+        }
+        return w4_tc_launch(p, x, rows, ldx, reinterpret_cast<int*>(a->fault), stream);
+    }
     // rows in slabs of about the same size
     const int most = p.f32 ? W4_ROWS_F32 : W4_ROWS;
     const int slabs = (rows + most - 1) / most;

@@ -35,7 +35,7 @@ class KernelError(RuntimeError):
 #: layouts of the arguments of launchers that take them as one block of 64-bit values (q: whole, d: floating point): a call with
 #: twenty arguments costs ctypes 2.5 us, the same packed 0.9
 _VERIFY_ARGS = struct.Struct("15q")
-_W4_ARGS = struct.Struct("13q")
+_W4_ARGS = struct.Struct("15q")
 _SHARED_ARGS = struct.Struct("28qd")
 
 
@@ -659,6 +659,9 @@ def gemm_f32_out(a: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
 # row-wise kernels
 # ---------------------------------------------------------------------------------------
 
+W4_TENSOR = os.environ.get("W4T", "1") != "0"
+
+
 def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a (n, K) @ w (K, N)`` for weights of four bits (``weights.w4.pack_w4``), a and the result in bfloat16 or float32; row strides
     free.  Every weight is taken as it is, (code - zero) * scale, and a sum is rounded once, when it is stored.
@@ -689,8 +692,9 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
     lib = _lib or library()
     calls["gemm_w4"] += 1
     words, scales, zeros = w.pointers
+    tensor = W4_TENSOR and dtype is torch.bfloat16 and n <= 64 and not (k % 8 or lda % 8 or a.data_ptr() % 16) and lda >= k
     _check(lib.tis_gemm_w4(_W4_ARGS.pack(1 if dtype is torch.bfloat16 else 0, a.data_ptr(), lda, words, scales, zeros, out.data_ptr(), ldo, n, k,
-                                         cols, w.group, _stream_number(device))), lib)
+                                         cols, w.group, tensor, tc_fault().data_ptr() if tensor else 0, _stream_number(device))), lib)
     return out
 
 

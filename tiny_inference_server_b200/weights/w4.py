@@ -5,11 +5,11 @@ kept).  ``quantize_w4`` finds codes by rounding to nearest, ``pack_w4`` lays cod
 them, ``unpack_w4`` gives the matrix back (for products of many rows).
 
 Layout.  16 columns ("strip") by 64 entries of the sum ("chunk") are 512 bytes in a row: 16 bytes of each lane of a warp, which are
-that lane's parts of four 16 x 16 operands of ``mma.sync`` (columns as rows).  Lane (g, t) = (lane // 4, lane % 4) holds columns g
-and g + 8; its word 2 h + j the entries 32 h + 8 t + 4 j + (0..3) of the chunk: bits 0-3 and 16-19 the first two of column g, 4-7 and
-20-23 those of column g + 8, 8-11 and 24-27 the last two of column g, 12-15 and 28-31 those of column g + 8.  So a shift and
-a mask give two neighbouring entries in the halves of a register, and the entries that a lane needs of a row of activations are
-16 contiguous bytes.  Scales and zero points lie as pairs (column g, column g + 8) by strip and group.
+that lane's parts of four 16 x 16 operands of the tensor cores (columns as rows).  Lane (g, t) = (lane // 4, lane % 4) holds columns g
+and g + 8; its word s the entries 16 s + 4 t + (0..3) of the chunk: bits 0-3 and 16-19 the first two of column g, 4-7 and 20-23 those
+of column g + 8, 8-11 and 24-27 the last two of column g, 12-15 and 28-31 those of column g + 8.  So a shift and a mask give two
+neighbouring entries in the halves of a register, and a lane's registers are what ``mma.sync`` takes and, in another order, what a
+store of 16 lanes by 256 bits into tensor memory takes.  Scales and zero points lie as pairs (column g, column g + 8) by strip and group.
 """
 from __future__ import annotations
 
@@ -104,10 +104,10 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Ten
         x = torch.zeros((chunks * CHUNK, (b - a) * STRIP), dtype=torch.uint8, device=codes.device)
         part = codes[:, a * STRIP:b * STRIP]
         x[:k, : part.shape[1]] = part
-        # chunk, half h, t, word j, pair i, entry e of the pair; strip, column half c, g
-        x = x.reshape(chunks, 2, 4, 2, 2, 2, b - a, 2, 8)
-        # strip, chunk, g, t, h, j, e, i, c: nibble 4 e + 2 i + c
-        x = x.permute(6, 0, 8, 2, 1, 3, 5, 4, 7).reshape(b - a, chunks, 32, 4, 4, 2)
+        # chunk, word s, t, pair i, entry e of the pair; strip, column half c, g
+        x = x.reshape(chunks, 4, 4, 2, 2, b - a, 2, 8)
+        # strip, chunk, g, t, s, e, i, c: nibble 4 e + 2 i + c
+        x = x.permute(5, 0, 7, 2, 1, 4, 3, 6).reshape(b - a, chunks, 32, 4, 4, 2)
         x = x[..., 0] | (x[..., 1] << 4)                      # bytes, the low nibble first
         words[a:b] = x.contiguous().view(torch.int32).squeeze(-1)
     return W4Weights(words, _pairs(scales), None if zeros is None else _pairs(zeros), k, n, group)
@@ -116,9 +116,9 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Ten
 def unpack_w4(w: W4Weights, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The (K, N) matrix of packed weights: every weight worked out in 32 bits and rounded to ``dtype`` once."""
     strips, chunks = w.words.shape[:2]
-    x = w.words.contiguous().view(torch.uint8).reshape(strips, chunks, 8, 4, 2, 2, 4)
-    x = torch.stack([x & 15, x >> 4], -1).reshape(strips, chunks, 8, 4, 2, 2, 2, 2, 2)          # strip, chunk, g, t, h, j, e, i, c
-    codes = x.permute(1, 4, 3, 5, 7, 6, 0, 8, 2).reshape(chunks * CHUNK, strips * STRIP)[: w.k, : w.n]
+    x = w.words.contiguous().view(torch.uint8).reshape(strips, chunks, 8, 4, 4, 4)
+    x = torch.stack([x & 15, x >> 4], -1).reshape(strips, chunks, 8, 4, 4, 2, 2, 2)             # strip, chunk, g, t, s, e, i, c
+    codes = x.permute(1, 4, 3, 6, 5, 0, 7, 2).reshape(chunks * CHUNK, strips * STRIP)[: w.k, : w.n]
 
     def rows(pairs):
         y = pairs.permute(1, 0, 3, 2).reshape(pairs.shape[1], strips * STRIP)[:, : w.n]
