@@ -45,20 +45,20 @@ def check(x, codes, scales, zeros, group, out=None):
 def test_pack_and_back(k, n, group, zeros):
     codes, scales, z = make(k, n, group, zeros)
     w = pack_w4(codes, scales, z, group)
-    assert w.shape == (k, n) and w.words.numel() * 8 == -(-k // 64) * 64 * -(-n // 16) * 16
+    assert w.shape == (k, n) and w.words.numel() * 8 == -(-k // 64) * 64 * -(-n // 128) * 128
     assert torch.equal(unpack_w4(w, torch.float32).double(), dense(codes, scales, z, group))
 
 
 def test_words_of_a_lane():
     """The documented place of every code."""
-    codes, scales, _ = make(128, 48, 64, False)
+    codes, scales, _ = make(128, 176, 64, False)
     w = pack_w4(codes, scales, None, 64)
-    for strip, chunk, lane, word in ((0, 0, 0, 0), (1, 1, 13, 3), (2, 0, 31, 2), (2, 1, 6, 1)):
+    for strip, chunk, lane, word in ((0, 0, 0, 0), (1, 1, 13, 3), (2, 0, 31, 2), (10, 1, 6, 1)):
         g, t = lane // 4, lane % 4
         k0, c = 64 * chunk + 16 * word + 4 * t, 16 * strip + g
         want = [codes[k0, c], codes[k0, c + 8], codes[k0 + 2, c], codes[k0 + 2, c + 8],
                 codes[k0 + 1, c], codes[k0 + 1, c + 8], codes[k0 + 3, c], codes[k0 + 3, c + 8]]
-        v = int(w.words[strip, chunk, lane, word])
+        v = int(w.words[strip // 8, chunk, strip % 8, lane, word])
         assert [(v >> (4 * i)) & 15 for i in range(8)] == [int(x) for x in want]
 
 

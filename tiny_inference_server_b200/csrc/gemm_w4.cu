@@ -109,7 +109,7 @@ w4_kernel(const W4Params p) {
 #pragma unroll
         for (int s = 0; s < SP; ++s) {
             const unsigned strip = (unsigned)min(load_tile * strips_of_tile + side * SP + s, p.strips - 1);
-            words[s] = (strip * (unsigned)p.chunks + turn) * 32 + lane;
+            words[s] = ((strip / 8 * (unsigned)p.chunks + turn) * 8 + strip % 8) * 32 + lane;
             groups[s] = strip * (unsigned)p.groups * 8 + g;
         }
     };
@@ -119,7 +119,7 @@ w4_kernel(const W4Params p) {
 #pragma unroll
             for (int s = 0; s < SP; ++s) {
                 it.w[s] = load_stream(p.words + words[s]);
-                words[s] += p.wk * 32;
+                words[s] += p.wk * (8 * 32);
 #pragma unroll
                 for (int h = 0; h < GROUPS; ++h) {
                     const unsigned a = groups[s] + 8 * (HALVES ? min(2 * c + h, p.groups - 1) : (2 * c) >> p.group_shift);

@@ -21,9 +21,9 @@ using namespace tc;
 
 constexpr int TILE = 128, TILE_STRIPS = TILE / W4_STRIP;
 constexpr int STAGE_CHUNKS = 2, STAGE_WORDS = TILE_STRIPS * STAGE_CHUNKS * 512;          // bytes of codes of a stage
-constexpr int A_STAGES = 4, A_COLS = 32;    // tensor memory: operands of 64 entries, two a column
+constexpr int A_STAGES = 2, A_COLS = 32;    // tensor memory: operands of a stage of the ring, a chunk's 64 entries in 32 columns
 constexpr unsigned COL_D = 0, COL_A = 128, TMEM_COLS = 256;
-constexpr int NTH = 384;                    // warps 0-3 unpack, 4-7 add up, 8 orders copies, 9 issues products, 10 and 11 fill the group
+constexpr int NTH = 512;                    // warps 0-7 unpack, 8-11 add up, 12 orders copies, 13 issues products, 14 and 15 fill the group
 
 template <int NB> struct Ring {
     static constexpr int X_BYTES = NB * 128 * STAGE_CHUNKS, BYTES = STAGE_WORDS + X_BYTES;
@@ -66,12 +66,13 @@ __device__ __forceinline__ float load_rank(const float* local, unsigned rank) {
     return v;
 }
 
-// NB: rows of x in the product (16, 32, 48, 64).  HALVES: groups of 32, two a chunk.  F32: the rows of x are three parts of a float's each, one
+// NB: rows of x in the product (16, 32, 48, 64).  SPAN: entries of a group, 128 for all from there on.  F32: the rows of x are three parts of a float's each, one
 // after another, and out is in float32.
-template <int NB, bool HALVES, bool F32>
+template <int NB, int SPAN, bool F32>
 __global__ void __launch_bounds__(NTH, 2)
 w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
     constexpr int STAGES = Ring<NB>::STAGES, BYTES = Ring<NB>::BYTES;
+    constexpr bool HALVES = SPAN == 32;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     __shared__ unsigned long long full[STAGES], empty[STAGES], a_full[A_STAGES], a_empty[A_STAGES], d_full[2], d_empty[2];
@@ -85,8 +86,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
     const int c0 = (int)rank * p.slice, c1 = min(c0 + p.slice, p.chunks);               // (no rank is without chunks)
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 5); }
-        for (int s = 0; s < A_STAGES; ++s) { mbar_init(&a_full[s], 4); mbar_init(&a_empty[s], 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 8); }
+        for (int s = 0; s < A_STAGES; ++s) { mbar_init(&a_full[s], 8); mbar_init(&a_empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(&d_full[s], 1); mbar_init(&d_empty[s], 4); }
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -95,156 +96,175 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
     __syncthreads();
     volatile int* abort = &abort_flag;
     unsigned tmem = 0;
-    if (warp != 8) {
+    if (warp != 12) {
         // Tensor memory only when the kernel before is done: one that has begun to let this one in may still have to ask for its own.
-        if (warp == 9) {
+        if (warp == 13) {
             pdl_wait();
             tmem_alloc(&tmem_base_slot, TMEM_COLS);
             pdl_launch_dependents();
         }
         fence_before();
-        asm volatile("bar.sync 1, 352;\n" ::: "memory");
+        asm volatile("bar.sync 1, 480;\n" ::: "memory");
         fence_after();
         tmem = tmem_base_slot;
     }
 
-    // 384 threads are launched with 80 registers each at the least, 30720 in all: 128 x 104 + 128 x 104 + 128 x 32
-    if (warp >= 8) {
+    // 512 threads are launched with 64 registers each, 32768 in all: 256 x 64 + 128 x 96 + 128 x 32
+    if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 32;\n" ::);
-        if (warp == 8) {
-            // ---- codes (eight copies a stage, a lane a strip) and x (a box a chunk); weights do not come from the kernel before, x does ----
-            int stage = 0;
-            bool waited = false, ok = true;
-            for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
-                const int strip = min(tile * TILE_STRIPS + (lane & 7), p.strips - 1);
-                const unsigned char* src = p.words + (size_t)strip * p.chunks * 512;
-                for (int c = c0; c < c1; c += STAGE_CHUNKS, ++stage) {
-                    const int s = stage % STAGES, n = min(STAGE_CHUNKS, c1 - c);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((stage / STAGES) & 1) ^ 1, abort, p.fault, 6));
-                    if (!ok) break;
-                    unsigned char* at = ring + (size_t)s * BYTES;
-                    if (lane == 0) mbar_arrive_expect_tx(&full[s], n * (TILE_STRIPS * 512 + NB * 128));
-                    __syncwarp();
-                    if (lane < TILE_STRIPS) bulk_copy(at + lane * (STAGE_CHUNKS * 512), src + (size_t)c * 512, n * 512, &full[s]);
-                    if (!waited) { pdl_wait(); waited = true; }
-                    if (lane < n) tma_load_2d(at + STAGE_WORDS + lane * (NB * 128), &map_x, (c + lane) * W4_CHUNK, 0, &full[s]);
+        if (warp == 12) {
+            // ---- codes (a copy a stage) and x (a box a chunk), by one thread; weights do not come from the kernel before, x does ----
+            if (elect_one()) {
+                int stage = 0;
+                bool waited = false, ok = true;
+                for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
+                    const unsigned char* src = p.words + (size_t)tile * p.chunks * (TILE_STRIPS * 512);
+                    for (int c = c0; c < c1; c += STAGE_CHUNKS, ++stage) {
+                        const int s = stage % STAGES, n = min(STAGE_CHUNKS, c1 - c);
+                        ok = mbar_wait(&empty[s], ((stage / STAGES) & 1) ^ 1, abort, p.fault, 6);
+                        if (!ok) break;
+                        unsigned char* at = ring + (size_t)s * BYTES;
+                        mbar_arrive_expect_tx(&full[s], n * (TILE_STRIPS * 512 + NB * 128));
+                        bulk_copy(at, src + (size_t)c * (TILE_STRIPS * 512), n * (TILE_STRIPS * 512), &full[s]);
+                        if (!waited) { pdl_wait(); waited = true; }
+                        for (int u = 0; u < n; ++u) tma_load_2d(at + STAGE_WORDS + u * (NB * 128), &map_x, (c + u) * W4_CHUNK, 0, &full[s]);
+                    }
                 }
+                if (!waited) pdl_wait();
             }
-            if (!waited) pdl_wait();
-        } else if (warp == 9) {
-            // ---- products: a chunk is four steps of 16 entries; a group's first step starts its sum ----
+            __syncwarp();
+        } else if (warp == 13) {
+            // ---- products: a chunk is four steps of 16 entries; a group's first step starts its sum.  One hand-over a stage; that its rows of x
+            // have landed the unpacking warps have seen.  (The warp walks together and one lane issues what a stage has in one go, so that
+            // operands come from uniform registers: alone in its branch a thread takes 100 cycles a product, this way 25.) ----
             constexpr unsigned IDESC = instr_desc(TILE, NB, false);
+            constexpr int SUMS = SPAN == 128 ? 1 : 128 / SPAN / (HALVES ? 2 : 1);       // groups that a round begins: of a stage, or of a chunk
             const unsigned long long x_desc0 = smem_desc(smem_u32(ring + STAGE_WORDS), 16, 1024);
-            int stage = 0, a = 0, d = 0;                    // stages, operands and sums so far
+            int stage = 0, d = 0;                           // stages and sums so far
             bool ok = true;
             for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
-                bool open = false;                          // a group's sum has begun
+                bool open = false;                          // a group's sum has begun (SPAN 128: it may go over several stages)
                 for (int c = c0; c < c1 && ok; c += STAGE_CHUNKS, ++stage) {
-                    const int s = stage % STAGES, n = min(STAGE_CHUNKS, c1 - c);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (stage / STAGES) & 1, abort, p.fault, 6));
-                    for (int u = 0; u < n && ok; ++u, ++a) {
-                        const int as = a % A_STAGES;
-                        ok = __all_sync(0xffffffffu, mbar_wait(&a_full[as], (a / A_STAGES) & 1, abort, p.fault, 6));
-                        if (!ok) break;
-                        const bool ends = ((2 * (c + u)) >> p.group_shift) != ((2 * (c + u + 1)) >> p.group_shift) || c + u + 1 == c1;
-                        const unsigned long long xd = x_desc0 + (unsigned long long)((s * BYTES + u * NB * 128) >> 4);
+                    const int s = stage % STAGES, as = stage % A_STAGES, n = min(STAGE_CHUNKS, c1 - c);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&a_full[as], (stage / A_STAGES) & 1, abort, p.fault, 6));
+                    if (!ok) break;
+                    const bool ends = SPAN != 128 || c + n == c1 || ((2 * c) >> p.group_shift) != ((2 * (c + n)) >> p.group_shift);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (!open) {
-                                ok = ok && __all_sync(0xffffffffu, mbar_wait(&d_empty[d & 1], ((d >> 1) & 1) ^ 1, abort, p.fault, 6));
-                                if (!ok) break;
-                            }
-                            fence_after();
-                            if (elect_one()) {
-                                const unsigned dst = tmem + COL_D + (d & 1) * 64;
-#pragma unroll
-                                for (int j = 0; j < 2; ++j) {
-                                    const int k = 2 * h + j;
-                                    umma_ts(dst, tmem + COL_A + as * A_COLS + k * 8, xd + (unsigned long long)(k * 2), IDESC, open || j > 0);
-                                }
-                                if (h == 1) umma_commit(&a_empty[as]);
-                                if (h == 1 && u == n - 1) umma_commit(&empty[s]);
-                                if (HALVES || (h == 1 && ends)) umma_commit(&d_full[d & 1]);
-                            }
-                            __syncwarp();
-                            open = true;
-                            if (HALVES || (h == 1 && ends)) { open = false; ++d; }
+                    for (int round = 0; round < (HALVES ? 2 : 1); ++round) {
+                        if (HALVES && round == 1 && n == 1) break;
+                        const int sums = SPAN == 64 ? n : SUMS;
+                        if (!open) {
+                            for (int q = 0; q < sums; ++q)
+                                ok = ok && __all_sync(0xffffffffu, mbar_wait(&d_empty[(d + q) & 1], (((d + q) >> 1) & 1) ^ 1, abort, p.fault, 6));
+                            if (!ok) break;
                         }
+                        fence_after();
+                        if (elect_one()) {
+                            const unsigned a0 = tmem + COL_A + as * (STAGE_CHUNKS * A_COLS);
+                            const unsigned long long x0 = x_desc0 + (unsigned long long)((s * BYTES) >> 4);
+#pragma unroll
+                            for (int u = HALVES ? round : 0; u < (HALVES ? round + 1 : STAGE_CHUNKS); ++u) {
+                                if (u == 1 && n == 1) break;
+                                // the place of this chunk's sum (SPAN 32: of its halves')
+                                const int at = SPAN == 64 ? d + u : d;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const unsigned dst = tmem + COL_D + ((at + (HALVES ? k / 2 : 0)) & 1) * 64;
+                                    const unsigned going = SPAN == 128 ? (open || u > 0 || k > 0) : (SPAN == 64 ? k > 0 : (k & 1));
+                                    umma_ts(dst, a0 + u * A_COLS + k * 8, x0 + (unsigned long long)((u * NB * 128 + k * 32) >> 4), IDESC, going);
+                                    if (HALVES && (k & 1)) umma_commit(&d_full[(at + k / 2) & 1]);
+                                }
+                                if (SPAN == 64) umma_commit(&d_full[at & 1]);
+                            }
+                            if (SPAN == 128 && ends) umma_commit(&d_full[d & 1]);
+                            if (!HALVES || round == 1 || n == 1) umma_commit(&a_empty[as]);
+                        }
+                        __syncwarp();
+                        if (SPAN == 128) { open = !ends; d += ends; }
+                        else d += sums;
                     }
                 }
             }
         }
-    } else if (warp < 4) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::);
-        // ---- codes to bfloat16: a warp has two strips, 32 lanes of tensor memory ----
-        int stage = 0, a = 0;
+    } else if (warp < 8) {
+        // ---- codes to bfloat16: a warp has two strips, 32 lanes of tensor memory, of every other chunk: the two of a stage are two warps' ----
+        static_assert(STAGE_CHUNKS == 2, "a chunk of a stage each");
+        const int quarter = warp & 3, u = warp >> 2;
+        int stage = 0, stored = -1;                         // stages so far, the operand whose store is under way
         bool ok = true;
         const int g = lane >> 2;
+        auto finish = [&]() {                               // the store is done: over to the products
+            if (stored >= 0) {
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&a_full[stored]);
+                stored = -1;
+            }
+        };
         for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
             const unsigned short* zeros[2];
             int seen = -1;                                  // the group whose zero points are here
             unsigned low[2] = {0x43084308u, 0x43084308u}, high[2] = {0x43084308u, 0x43084308u};     // 128 + zero of the columns g and g + 8
-            unsigned next[2] = {0u, 0u};                    // and those of the group behind it
 #pragma unroll
             for (int q = 0; q < 2; ++q)
-                zeros[q] = p.zeros + (size_t)min(tile * TILE_STRIPS + warp * 2 + q, p.strips - 1) * p.groups * 8 + g;
-            if (p.zeros != nullptr) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q) next[q] = __ldg(zeros[q] + ((2 * c0) >> p.group_shift) * 8);
-            }
+                zeros[q] = p.zeros + (size_t)min(tile * TILE_STRIPS + quarter * 2 + q, p.strips - 1) * p.groups * 8 + g;
             for (int c = c0; c < c1 && ok; c += STAGE_CHUNKS, ++stage) {
                 const int s = stage % STAGES, n = min(STAGE_CHUNKS, c1 - c);
+                // zero points are asked for before the codes are waited for
+                unsigned short z[2][2] = {{0, 0}, {0, 0}};
+                const int group = min((2 * (c + u)) >> p.group_shift, p.groups - 1);
+                const bool fresh = p.zeros != nullptr && group != seen;         // (uniform in the warp)
+                if (fresh) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        z[q][0] = __ldg(zeros[q] + group * 8);
+                        if (HALVES) z[q][1] = __ldg(zeros[q] + min(group + 1, p.groups - 1) * 8);
+                    }
+                    seen = group;
+                }
                 ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (stage / STAGES) & 1, abort, p.fault, 6));
                 if (!ok) break;
-                for (int u = 0; u < n; ++u, ++a) {
-                    const int as = a % A_STAGES;
-                    uint4 w[2];
+                const int as = stage % A_STAGES;
+                unsigned r[2][16];
 #pragma unroll
-                    for (int q = 0; q < 2; ++q)
-                        w[q] = *reinterpret_cast<const uint4*>(ring + (size_t)s * BYTES + (warp * 2 + q) * (STAGE_CHUNKS * 512) + u * 512 + lane * 16);
-                    unsigned r[2][16];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (p.zeros != nullptr && (h == 0 || HALVES)) {
-                            const int group = (2 * (c + u) + h) >> p.group_shift;
-                            if (group != seen) {            // (uniform in the CTA)
-                                seen = group;
-#pragma unroll
-                                for (int q = 0; q < 2; ++q) {
-                                    low[q] = 0x43004300u | (next[q] & 0xffu) * 0x00010001u;
-                                    high[q] = 0x43004300u | (next[q] >> 8) * 0x00010001u;
-                                    next[q] = __ldg(zeros[q] + min(group + 1, p.groups - 1) * 8);
-                                }
-                            }
-                        }
-#pragma unroll
-                        for (int q = 0; q < 2; ++q)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const unsigned v = h ? (j ? w[q].w : w[q].z) : (j ? w[q].y : w[q].x);
-                                unsigned* to = r[q] + (2 * h + j) * 4;
-                                to[0] = w4_pair(v, low[q]);
-                                to[2] = w4_pair(v >> 4, high[q]);
-                                to[1] = w4_pair(v >> 8, low[q]);
-                                to[3] = w4_pair(v >> 12, high[q]);
-                            }
+                for (int q = 0; q < 2; ++q) {               // (of a chunk beyond the last: what lies there, for an operand that no product takes)
+                    const uint4 w = *reinterpret_cast<const uint4*>(ring + (size_t)s * BYTES + (u * TILE_STRIPS + quarter * 2 + q) * 512 + lane * 16);
+                    if (fresh) {
+                        low[q] = 0x43004300u | (z[q][0] & 0xffu) * 0x00010001u;
+                        high[q] = 0x43004300u | (unsigned)(z[q][0] >> 8) * 0x00010001u;
                     }
-                    ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[as], ((a / A_STAGES) & 1) ^ 1, abort, p.fault, 6));
-                    if (!ok) break;
-                    fence_after();
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) tmem_st_16x256b_x4(tmem + ((unsigned)(warp * 32 + q * 16) << 16) + COL_A + as * A_COLS, r[q]);
-                    asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&a_full[as]);
+                    for (int k = 0; k < 4; ++k) {
+                        const unsigned v = k == 0 ? w.x : (k == 1 ? w.y : (k == 2 ? w.z : w.w));
+                        unsigned lo = low[q], hi = high[q];
+                        if (HALVES && k >= 2 && p.zeros != nullptr) {
+                            lo = 0x43004300u | (z[q][1] & 0xffu) * 0x00010001u;
+                            hi = 0x43004300u | (unsigned)(z[q][1] >> 8) * 0x00010001u;
+                        }
+                        r[q][4 * k] = w4_pair(v, lo);
+                        r[q][4 * k + 2] = w4_pair(v >> 4, hi);
+                        r[q][4 * k + 1] = w4_pair(v >> 8, lo);
+                        r[q][4 * k + 3] = w4_pair(v >> 12, hi);
+                    }
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[s]);      // the stage's codes have been read
+                finish();                                   // (the store before had the time of the unpacking)
+                ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[as], ((stage / A_STAGES) & 1) ^ 1, abort, p.fault, 6));
+                if (!ok) break;
+                // the products of the stage before the one before are done: its place in the ring is free, codes and rows of x
+                if (stage >= A_STAGES && lane == 0) mbar_arrive(&empty[(stage - A_STAGES) % STAGES]);
+                fence_after();
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    tmem_st_16x256b_x4(tmem + ((unsigned)(quarter * 32 + q * 16) << 16) + COL_A + (as * STAGE_CHUNKS + u) * A_COLS, r[q]);
+                stored = as;
             }
+            // (the tile's last operands are handed over before its sums are waited for elsewhere: nothing behind waits for this warp's next)
+            finish();
         }
+        finish();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;\n" ::);
         // ---- a thread a column: the groups' sums, times their scales, added up ----
         const int quarter = warp & 3, column = quarter * 32 + lane;
         const unsigned from = tmem + ((unsigned)(quarter * 32) << 16) + COL_D;
@@ -309,7 +329,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
     }
     fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 13) {
         fence_after();
         tmem_free(tmem, TMEM_COLS);
     }
@@ -318,8 +338,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
         cluster_reduce::cluster_wait();
         const float* part = reinterpret_cast<const float*>(ring);
         const int n = first_tile * TILE + (int)(threadIdx.x & 127);
-        // rows rank, rank + ranks, ..: three at a time, the ranks' sums in their order
-        for (int r = (int)rank + (int)(threadIdx.x >> 7) * (int)ranks; r < p.rows; r += 3 * (int)ranks) {
+        // rows rank, rank + ranks, ..: four at a time, the ranks' sums in their order
+        for (int r = (int)rank + (int)(threadIdx.x >> 7) * (int)ranks; r < p.rows; r += 4 * (int)ranks) {
             float v[3] = {0.f, 0.f, 0.f};
             for (unsigned q = 0; q < ranks; ++q)
 #pragma unroll
@@ -334,11 +354,12 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
     }
 }
 
-template <int NB, bool HALVES, bool F32> int launch(const CUtensorMap& map, const W4TcParams& p, int ranks, cudaStream_t stream) {
+template <int NB, int SPAN, bool F32> int launch(const CUtensorMap& map, const W4TcParams& p, int ranks, cudaStream_t stream) {
     const int smem = Ring<NB>::STAGES * Ring<NB>::BYTES + 1024;
+    static_assert(Ring<NB>::STAGES > A_STAGES, "the ring is ahead of the operands");
     static_assert(Ring<NB>::STAGES * Ring<NB>::BYTES >= NB * TILE * 4, "a CTA's sums fit the ring");
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(w4_tc_kernel<NB, HALVES, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    if (configured.first() && cudaFuncSetAttribute(w4_tc_kernel<NB, SPAN, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return tis_check_launch("gemm_w4 (shared memory)");
     const int most = 2 * sm_count();
     cudaLaunchConfig_t cfg = {};
@@ -355,12 +376,16 @@ template <int NB, bool HALVES, bool F32> int launch(const CUtensorMap& map, cons
     attrs[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attrs;
     cfg.numAttrs = tis_pdl_enabled() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, w4_tc_kernel<NB, HALVES, F32>, map, p);
+    cudaLaunchKernelEx(&cfg, w4_tc_kernel<NB, SPAN, F32>, map, p);
     return tis_check_launch("gemm_w4");
 }
+template <int NB, bool F32> int launch_span(const CUtensorMap& map, const W4TcParams& p, int ranks, cudaStream_t stream) {
+    if (p.group_shift == 0) return launch<NB, 32, F32>(map, p, ranks, stream);
+    if (p.group_shift == 1) return launch<NB, 64, F32>(map, p, ranks, stream);
+    return launch<NB, 128, F32>(map, p, ranks, stream);
+}
 template <int NB> int launch_form(const CUtensorMap& map, const W4TcParams& p, int ranks, cudaStream_t stream) {
-    if (p.f32) return p.group_shift == 0 ? launch<NB, true, true>(map, p, ranks, stream) : launch<NB, false, true>(map, p, ranks, stream);
-    return p.group_shift == 0 ? launch<NB, true, false>(map, p, ranks, stream) : launch<NB, false, false>(map, p, ranks, stream);
+    return p.f32 ? launch_span<NB, true>(map, p, ranks, stream) : launch_span<NB, false>(map, p, ranks, stream);
 }
 
 }  // namespace
@@ -381,8 +406,10 @@ int w4_tc_launch(const W4Params& w, const void* x, int x_rows, long long ldx, in
     // CTAs of a tile: as many as are all resident, with four chunks each at the least, none of them empty
     int ranks = 1;
     while (ranks < 8 && p.tiles * ranks * 2 <= 2 * sm_count() && p.chunks >= 2 * ranks * 4) ranks *= 2;
-    while (ranks > 1 && ((p.chunks + ranks - 1) / ranks) * (ranks - 1) >= p.chunks) ranks /= 2;
-    p.slice = (p.chunks + ranks - 1) / ranks;
+    // (whole stages each, so that a stage has whole groups)
+    auto slice = [&](int r) { return ((p.chunks + r - 1) / r + STAGE_CHUNKS - 1) / STAGE_CHUNKS * STAGE_CHUNKS; };
+    while (ranks > 1 && slice(ranks) * (ranks - 1) >= p.chunks) ranks /= 2;
+    p.slice = slice(ranks);
     switch (nb) {
         case 16: return launch_form<16>(map, p, ranks, stream);
         case 32: return launch_form<32>(map, p, ranks, stream);

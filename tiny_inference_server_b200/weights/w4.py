@@ -4,7 +4,8 @@ A weight of a (K, N) matrix is ``(code[k, n] - zero[k // group, n]) * scale[k //
 kept).  ``quantize_w4`` finds codes by rounding to nearest, ``pack_w4`` lays codes out once as ``kernels.ops.gemm_w4`` streams
 them, ``unpack_w4`` gives the matrix back (for products of many rows).
 
-Layout.  16 columns ("strip") by 64 entries of the sum ("chunk") are 512 bytes in a row: 16 bytes of each lane of a warp, which are
+Layout.  Eight strips of 16 columns are a tile; the chunks of 64 entries of the sum follow one another in it, each with its strips' 512
+bytes one after another.  A strip's 512 bytes of a chunk are 16 of each lane of a warp, which are
 that lane's parts of four 16 x 16 operands of the tensor cores (columns as rows).  Lane (g, t) = (lane // 4, lane % 4) holds columns g
 and g + 8; its word s the entries 16 s + 4 t + (0..3) of the chunk: bits 0-3 and 16-19 the first two of column g, 4-7 and 20-23 those
 of column g + 8, 8-11 and 24-27 the last two of column g, 12-15 and 28-31 those of column g + 8.  So a shift and a mask give two
@@ -18,12 +19,12 @@ from typing import Optional, Tuple
 
 import torch
 
-STRIP, CHUNK = 16, 64
+STRIP, CHUNK, TILE_STRIPS = 16, 64, 8
 
 
 @dataclass(frozen=True)
 class W4Weights:
-    """Codes in the kernel's layout: ``words`` (strips, chunks, 32, 4) int32, ``scales`` (strips, groups, 8, 2) bfloat16, ``zeros``
+    """Codes in the kernel's layout: ``words`` (tiles, chunks, 8, 32, 4) int32, ``scales`` (strips, groups, 8, 2) bfloat16, ``zeros``
     the same in uint8 (None: 8 everywhere)."""
     words: torch.Tensor
     scales: torch.Tensor
@@ -98,16 +99,17 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Ten
     if int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15):
         raise ValueError("codes and zero points are 0..15")
     strips, chunks = -(-n // STRIP), -(-k // CHUNK)
-    words = torch.empty((strips, chunks, 32, 4), dtype=torch.int32, device=codes.device)
-    for a in range(0, strips, 1024):                          # (in pieces: the working copies are several times the codes)
-        b = min(a + 1024, strips)
-        x = torch.zeros((chunks * CHUNK, (b - a) * STRIP), dtype=torch.uint8, device=codes.device)
-        part = codes[:, a * STRIP:b * STRIP]
+    tiles = -(-strips // TILE_STRIPS)
+    words = torch.empty((tiles, chunks, TILE_STRIPS, 32, 4), dtype=torch.int32, device=codes.device)
+    for a in range(0, tiles, 128):                            # (in pieces: the working copies are several times the codes)
+        b = min(a + 128, tiles)
+        x = torch.zeros((chunks * CHUNK, (b - a) * TILE_STRIPS * STRIP), dtype=torch.uint8, device=codes.device)
+        part = codes[:, a * TILE_STRIPS * STRIP:b * TILE_STRIPS * STRIP]
         x[:k, : part.shape[1]] = part
-        # chunk, word s, t, pair i, entry e of the pair; strip, column half c, g
-        x = x.reshape(chunks, 4, 4, 2, 2, b - a, 2, 8)
-        # strip, chunk, g, t, s, e, i, c: nibble 4 e + 2 i + c
-        x = x.permute(5, 0, 7, 2, 1, 4, 3, 6).reshape(b - a, chunks, 32, 4, 4, 2)
+        # chunk, word s, t, pair i, entry e of the pair; tile, strip, column half c, g
+        x = x.reshape(chunks, 4, 4, 2, 2, b - a, TILE_STRIPS, 2, 8)
+        # tile, chunk, strip, g, t, s, e, i, c: nibble 4 e + 2 i + c
+        x = x.permute(5, 0, 6, 8, 2, 1, 4, 3, 7).reshape(b - a, chunks, TILE_STRIPS, 32, 4, 4, 2)
         x = x[..., 0] | (x[..., 1] << 4)                      # bytes, the low nibble first
         words[a:b] = x.contiguous().view(torch.int32).squeeze(-1)
     return W4Weights(words, _pairs(scales), None if zeros is None else _pairs(zeros), k, n, group)
@@ -115,12 +117,13 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Ten
 
 def unpack_w4(w: W4Weights, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The (K, N) matrix of packed weights: every weight worked out in 32 bits and rounded to ``dtype`` once."""
-    strips, chunks = w.words.shape[:2]
-    x = w.words.contiguous().view(torch.uint8).reshape(strips, chunks, 8, 4, 4, 4)
-    x = torch.stack([x & 15, x >> 4], -1).reshape(strips, chunks, 8, 4, 4, 2, 2, 2)             # strip, chunk, g, t, s, e, i, c
-    codes = x.permute(1, 4, 3, 6, 5, 0, 7, 2).reshape(chunks * CHUNK, strips * STRIP)[: w.k, : w.n]
+    tiles, chunks = w.words.shape[:2]
+    x = w.words.contiguous().view(torch.uint8).reshape(tiles, chunks, TILE_STRIPS, 8, 4, 4, 4)
+    x = torch.stack([x & 15, x >> 4], -1).reshape(tiles, chunks, TILE_STRIPS, 8, 4, 4, 2, 2, 2)         # tile, chunk, strip, g, t, s, e, i, c
+    codes = x.permute(1, 5, 4, 7, 6, 0, 2, 8, 3).reshape(chunks * CHUNK, tiles * TILE_STRIPS * STRIP)[: w.k, : w.n]
 
     def rows(pairs):
+        strips = pairs.shape[0]
         y = pairs.permute(1, 0, 3, 2).reshape(pairs.shape[1], strips * STRIP)[:, : w.n]
         return y.repeat_interleave(w.group, 0)[: w.k].float()
 
