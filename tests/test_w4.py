@@ -104,11 +104,19 @@ SIZES = [(1, 1, 1, 32), (1, 64, 16, 32), (1, 1536, 2304, 128), (8, 1536, 520, 64
          (200, 640, 72, 256), (2, 20000, 16, 64), (7, 4096, 20000, 128), (33, 130, 19000, 32), (60, 8200, 24, 16384)]
 
 
+@pytest.fixture(params=[None, False, True], ids=["chosen", "mma", "tcgen05"])
+def kernel(request, monkeypatch):
+    monkeypatch.setattr(ops, "W4_TENSOR", request.param)
+    yield
+    if torch.cuda.is_available():
+        assert int(ops.tc_fault()[0].item()) == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,k,n,group", SIZES)
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_products(rows, k, n, group, zeros, dtype):
+def test_products(rows, k, n, group, zeros, dtype, kernel):
     codes, scales, z = make(k, n, group, zeros, rows + k + n, "cuda")
     x = torch.randn(rows, k, generator=torch.Generator().manual_seed(rows)).to(dtype).cuda()
     check(x, codes, scales, z, group)
@@ -116,7 +124,7 @@ def test_products(rows, k, n, group, zeros, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_strided_rows_and_what_lies_beside_them(dtype):
+def test_strided_rows_and_what_lies_beside_them(dtype, kernel):
     codes, scales, z = make(512, 80, 64, True, 3, "cuda")
     for offset, extra in ((0, 0), (8, 8), (1, 3), (4, 4)):
         room = torch.full((6, 512 + offset + extra), float("nan"), dtype=dtype, device="cuda")
@@ -132,7 +140,7 @@ def test_strided_rows_and_what_lies_beside_them(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_numbers_far_apart_and_none(dtype):
+def test_numbers_far_apart_and_none(dtype, kernel):
     """Large beside small, infinities and NaN: what is not finite stays in its row."""
     codes, scales, z = make(256, 48, 32, True, 5, "cuda")
     x = torch.randn(6, 256, generator=torch.Generator().manual_seed(1)) * torch.logspace(-18, 18, 256)[None]
@@ -155,7 +163,7 @@ def test_numbers_far_apart_and_none(dtype):
 
 
 @pytest.mark.gpu
-def test_float32_rows_keep_their_bits():
+def test_float32_rows_keep_their_bits(kernel):
     """A float's low bits count: x and the same less its last sixteen bits differ by what they are."""
     codes, scales, z = make(128, 16, 128, False, 6, "cuda")
     codes.fill_(9)
@@ -167,7 +175,7 @@ def test_float32_rows_keep_their_bits():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 8, 24, 48])
-def test_a_row_does_not_depend_on_the_others_and_runs_repeat(rows):
+def test_a_row_does_not_depend_on_the_others_and_runs_repeat(rows, kernel):
     codes, scales, z = make(1024, 400, 64, True, 8, "cuda")
     w = pack_w4(codes, scales, z, 64)
     x = torch.randn(rows, 1024, device="cuda").bfloat16()
@@ -179,7 +187,7 @@ def test_a_row_does_not_depend_on_the_others_and_runs_repeat(rows):
 
 
 @pytest.mark.gpu
-def test_streams_and_graphs():
+def test_streams_and_graphs(kernel):
     codes, scales, z = make(1536, 640, 128, False, 9, "cuda")
     w = pack_w4(codes, scales, z, 128)
     x = torch.randn(4, 1536, device="cuda").bfloat16()

@@ -36,16 +36,6 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const unsigned (&a)[4], 
 __device__ __forceinline__ float low_half(unsigned v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high_half(unsigned v) { return __uint_as_float(v & 0xffff0000u); }
 
-// one float as three bfloat16 numbers that add up to it
-__device__ __forceinline__ void three(float x, unsigned short (&v)[3]) {
-    const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-    const float rest = fabsf(x) < INFINITY ? x - hi : 0.f;
-    const float mid = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
-    v[0] = x != x ? 0x7fc0 : (unsigned short)(__float_as_uint(hi) >> 16);
-    v[1] = (unsigned short)(__float_as_uint(mid) >> 16);
-    v[2] = (unsigned short)(__float_as_uint(rest - mid) >> 16);
-}
-
 // Entries [k0, k0 + count) of the slab's rows of x into shared memory, zero beyond K.  In float32 the rows stand three times, the
 // high parts, the middle ones, the low ones.
 __device__ __forceinline__ void stage_rows(const W4Params& p, bf16* to, int stride, int row0, int rows, int k0, int count) {
@@ -89,8 +79,8 @@ __device__ __forceinline__ void stage_rows(const W4Params& p, bf16* to, int stri
 }
 
 // NT: eights of staged rows; SP: strips of a warp; AHEAD: chunks that it has under way; HALVES: groups of 32, two a chunk.
-template <int NT, int SP, int AHEAD, bool HALVES, bool ZEROS>
-__global__ void __launch_bounds__(W4_THREADS, 2)
+template <int NT, int SP, int AHEAD, int CTAS, bool HALVES, bool ZEROS>
+__global__ void __launch_bounds__(W4_THREADS, CTAS)
 w4_kernel(const W4Params p) {
     extern __shared__ __align__(16) unsigned char w4_smem[];
     pdl_launch_dependents();
@@ -262,9 +252,8 @@ w4_kernel(const W4Params p) {
     }
 }
 
-constexpr int W4_SMEM = 112 * 1024;         // two CTAs an SM
 
-template <int NT, int SP, int AHEAD, bool HALVES, bool ZEROS> int w4_launch(W4Params p, int slabs, cudaStream_t stream) {
+template <int NT, int SP, int AHEAD, int CTAS, bool HALVES, bool ZEROS> int w4_launch(W4Params p, int slabs, cudaStream_t stream) {
     auto bytes = [&](int stage_chunks, int buffers) {
         const size_t count = (size_t)stage_chunks * W4_CHUNK;
         const size_t staged = (size_t)NT * 8 * (count + W4_PAD) * 2 * buffers;
@@ -275,39 +264,39 @@ template <int NT, int SP, int AHEAD, bool HALVES, bool ZEROS> int w4_launch(W4Pa
     p.wk = W4_WARPS;
     p.stages = 1;
     p.stage_chunks = (p.chunks + p.wk - 1) / p.wk * p.wk;
-    if (bytes(p.stage_chunks, 1) > W4_SMEM) {
+    if (bytes(p.stage_chunks, 1) > (224 * 1024 / CTAS)) {
         p.ws = 4;
-        p.wk = 2;
+        p.wk = W4_WARPS / p.ws;
         const int unit = p.wk * AHEAD;
         p.stage_chunks = unit;
-        while (bytes(p.stage_chunks + unit, 2) <= W4_SMEM) p.stage_chunks += unit;
+        while (bytes(p.stage_chunks + unit, 2) <= (224 * 1024 / CTAS)) p.stage_chunks += unit;
         p.stages = (p.chunks + p.stage_chunks - 1) / p.stage_chunks;
     }
     const size_t smem = bytes(p.stage_chunks, p.stages > 1 ? 2 : 1);
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(w4_kernel<NT, SP, AHEAD, HALVES, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
+    if (configured.first() && cudaFuncSetAttribute(w4_kernel<NT, SP, AHEAD, CTAS, HALVES, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
         return tis_check_launch("gemm_w4 (shared memory)");
     if (smem > 227 * 1024) {
         tis_set_error("gemm_w4: %zu bytes of shared memory", smem);
         return TIS_BAD_SIZE;
     }
     const int tiles = (p.strips + p.ws * SP - 1) / (p.ws * SP);
-    const int most = 2 * 148;
-    tis_launch(w4_kernel<NT, SP, AHEAD, HALVES, ZEROS>, dim3((unsigned)(tiles < most ? tiles : most), (unsigned)slabs), dim3(W4_THREADS), smem, stream, p);
+    const int most = CTAS * 148;
+    tis_launch(w4_kernel<NT, SP, AHEAD, CTAS, HALVES, ZEROS>, dim3((unsigned)(tiles < most ? tiles : most), (unsigned)slabs), dim3(W4_THREADS), smem, stream, p);
     return tis_check_launch("gemm_w4");
 }
 
-template <int NT, int SP, int AHEAD, bool HALVES> int w4_zeros(const W4Params& p, int slabs, cudaStream_t stream) {
-    return p.zeros != nullptr ? w4_launch<NT, SP, AHEAD, HALVES, true>(p, slabs, stream) : w4_launch<NT, SP, AHEAD, HALVES, false>(p, slabs, stream);
+template <int NT, int SP, int AHEAD, int CTAS, bool HALVES> int w4_zeros(const W4Params& p, int slabs, cudaStream_t stream) {
+    return p.zeros != nullptr ? w4_launch<NT, SP, AHEAD, CTAS, HALVES, true>(p, slabs, stream) : w4_launch<NT, SP, AHEAD, CTAS, HALVES, false>(p, slabs, stream);
 }
-template <int NT, int SP, int AHEAD> int w4_forms(const W4Params& p, int slabs, cudaStream_t stream) {
-    return p.group_shift == 0 ? w4_zeros<NT, SP, AHEAD, true>(p, slabs, stream) : w4_zeros<NT, SP, AHEAD, false>(p, slabs, stream);
+template <int NT, int SP, int AHEAD, int CTAS> int w4_forms(const W4Params& p, int slabs, cudaStream_t stream) {
+    return p.group_shift == 0 ? w4_zeros<NT, SP, AHEAD, CTAS, true>(p, slabs, stream) : w4_zeros<NT, SP, AHEAD, CTAS, false>(p, slabs, stream);
 }
 
 }  // namespace
 
 // out (rows, N) = x (rows, K) times the packed weights; dtype is that of x and out, rows of both contiguous, row strides free.
-struct W4Args { long long dtype, x, ldx, words, scales, zeros, out, ldo, rows, K, N, group, tensor, fault, stream; };
+struct W4Args { long long dtype, x, ldx, words, scales, zeros, out, ldo, rows, K, N, group, tensor, copy, fault, stream; };
 TIS_API int tis_gemm_w4(const W4Args* a) {
     if (a->K <= 0 || a->K > (1 << 30) || a->N > (1 << 30) || a->rows > (1 << 30) || a->group < 32 || a->group > (1 << 30) ||
         (a->group & (a->group - 1)) != 0 || a->K * a->N > (1ll << 36)) {
@@ -336,11 +325,11 @@ TIS_API int tis_gemm_w4(const W4Args* a) {
     p.f32 = dtype == TIS_F32;
     p.vectors = K % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (p.f32 ? 4 : 8) == 0;
     if (a->tensor) {
-        if (p.f32 || rows > W4_ROWS || !p.vectors) {
-            tis_set_error("gemm_w4: %d rows, %s, are not for the tcgen05 kernel", rows, p.f32 ? "float32" : "bfloat16");
+        if (a->copy == 0 && (p.f32 || !p.vectors)) {
+            tis_set_error("gemm_w4: the tcgen05 kernel takes bfloat16 rows that start on 16 bytes, or room to copy them to");
             return TIS_BAD_SIZE;
         }
-        return w4_tc_launch(p, x, rows, ldx, reinterpret_cast<int*>(a->fault), stream);
+        return w4_tc_launch(p, reinterpret_cast<void*>(a->copy), reinterpret_cast<int*>(a->fault), stream);
     }
     // rows in slabs of about the same size
     const int most = p.f32 ? W4_ROWS_F32 : W4_ROWS;
@@ -352,12 +341,13 @@ TIS_API int tis_gemm_w4(const W4Args* a) {
     p.slab = (rows + slabs - 1) / slabs;
     const int eights = ((p.f32 ? 3 : 1) * p.slab + 7) / 8;
     switch (eights) {
-        case 1: return p.strips <= 2 * 148 ? w4_forms<1, 1, 4>(p, slabs, stream) : w4_forms<1, 2, 4>(p, slabs, stream);
-        case 2: return w4_forms<2, 2, 2>(p, slabs, stream);
-        case 3: return w4_forms<3, 1, 4>(p, slabs, stream);
-        case 4: return w4_forms<4, 1, 4>(p, slabs, stream);
-        case 5: return w4_forms<5, 1, 2>(p, slabs, stream);
-        case 6: return w4_forms<6, 1, 2>(p, slabs, stream);
-        default: return w4_forms<8, 1, 2>(p, slabs, stream);
+        case 1:
+            return p.strips <= 2 * 148 ? w4_forms<1, 1, 4, 2>(p, slabs, stream) : w4_forms<1, 2, 4, 2>(p, slabs, stream);
+        case 2: return w4_forms<2, 2, 2, 2>(p, slabs, stream);
+        case 3: return w4_forms<3, 1, 4, 2>(p, slabs, stream);
+        case 4: return w4_forms<4, 1, 4, 2>(p, slabs, stream);
+        case 5: return w4_forms<5, 1, 2, 2>(p, slabs, stream);
+        case 6: return w4_forms<6, 1, 2, 2>(p, slabs, stream);
+        default: return w4_forms<8, 1, 2, 2>(p, slabs, stream);
     }
 }

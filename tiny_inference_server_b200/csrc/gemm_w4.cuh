@@ -19,5 +19,17 @@ __device__ __forceinline__ unsigned w4_pair(unsigned w, unsigned base) {
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&base));
     return *reinterpret_cast<const unsigned*>(&d);
 }
-// gemm_w4_tc.cu: x in bfloat16 (`x_rows` rows; for float32 three of them, one after another, are a row), rows that start on 16 bytes
-int w4_tc_launch(const W4Params& p, const void* x, int x_rows, long long ldx, int* fault, cudaStream_t stream);
+// one float as three bfloat16 numbers that add up to it
+__device__ __forceinline__ void three(float x, unsigned short (&v)[3]) {
+    const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    const float rest = fabsf(x) < INFINITY ? x - hi : 0.f;
+    const float mid = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+    v[0] = x != x ? 0x7fc0 : (unsigned short)(__float_as_uint(hi) >> 16);
+    v[1] = (unsigned short)(__float_as_uint(mid) >> 16);
+    v[2] = (unsigned short)(__float_as_uint(rest - mid) >> 16);
+}
+
+// gemm_w4_tc.cu.  `copy` (null: x is bfloat16 in rows that start on 16 bytes): room for x's rows in bfloat16, (K + 7) / 8 * 8 entries each, three for
+// one of float32.
+constexpr int W4_TC_ROWS = 64, W4_TC_ROWS_F32 = 21;      // of a launch
+int w4_tc_launch(const W4Params& p, void* copy, int* fault, cudaStream_t stream);

@@ -354,6 +354,25 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
     }
 }
 
+// x's rows as the products take them: bfloat16 in rows that start on 16 bytes; a row of float32 is three, its high, middle and low parts.
+template <typename T>
+__global__ void __launch_bounds__(256) w4_copy_kernel(const T* x, long long ldx, bf16* to, long long ldt, int rows, int K) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int k = blockIdx.x * 256 + threadIdx.x;
+    if (k >= K) return;
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        if (sizeof(T) == 2) {
+            to[r * ldt + k] = *reinterpret_cast<const bf16*>(x + r * ldx + k);
+        } else {
+            unsigned short v[3];
+            three(*reinterpret_cast<const float*>(x + r * ldx + k), v);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) reinterpret_cast<unsigned short*>(to)[(3ll * r + q) * ldt + k] = v[q];
+        }
+    }
+}
+
 template <int NB, int SPAN, bool F32> int launch(const CUtensorMap& map, const W4TcParams& p, int ranks, cudaStream_t stream) {
     const int smem = Ring<NB>::STAGES * Ring<NB>::BYTES + 1024;
     static_assert(Ring<NB>::STAGES > A_STAGES, "the ring is ahead of the operands");
@@ -390,16 +409,25 @@ template <int NB> int launch_form(const CUtensorMap& map, const W4TcParams& p, i
 
 }  // namespace
 
-int w4_tc_launch(const W4Params& w, const void* x, int x_rows, long long ldx, int* fault, cudaStream_t stream) {
-    const int nb = x_rows <= 16 ? 16 : (x_rows <= 32 ? 32 : (x_rows <= 48 ? 48 : 64));
-    CUtensorMap map;
-    if (!tensor_map(x, w.K, x_rows, ldx, nb, true, &map)) return TIS_CUDA_ERROR;
+int w4_tc_launch(const W4Params& w, void* copy, int* fault, cudaStream_t stream) {
+    const bf16* x = static_cast<const bf16*>(w.x);
+    long long ldx = w.ldx;
+    const int times = w.f32 ? 3 : 1;
+    if (copy != nullptr) {
+        ldx = (w.K + 7) / 8 * 8;
+        x = static_cast<const bf16*>(copy);
+        const dim3 grid((unsigned)((w.K + 255) / 256), (unsigned)(w.rows < 65535 ? w.rows : 65535));
+        if (w.f32) tis_launch(w4_copy_kernel<float>, grid, dim3(256), 0, stream, static_cast<const float*>(w.x), w.ldx, static_cast<bf16*>(copy), ldx, w.rows, w.K);
+        else tis_launch(w4_copy_kernel<bf16>, grid, dim3(256), 0, stream, static_cast<const bf16*>(w.x), w.ldx, static_cast<bf16*>(copy), ldx, w.rows, w.K);
+        const int status = tis_check_launch("gemm_w4 (copy)");
+        if (status != TIS_OK) return status;
+    }
     W4TcParams p;
     p.words = reinterpret_cast<const unsigned char*>(w.words);
     p.scales = reinterpret_cast<const unsigned short*>(w.scales);
     p.zeros = w.zeros;
-    p.out = w.out; p.ldo = w.ldo;
-    p.rows = w.rows; p.N = w.N; p.chunks = w.chunks; p.strips = w.strips; p.groups = w.groups; p.group_shift = w.group_shift;
+    p.ldo = w.ldo;
+    p.N = w.N; p.chunks = w.chunks; p.strips = w.strips; p.groups = w.groups; p.group_shift = w.group_shift;
     p.tiles = (w.N + TILE - 1) / TILE;
     p.f32 = w.f32;
     p.fault = fault;
@@ -410,10 +438,17 @@ int w4_tc_launch(const W4Params& w, const void* x, int x_rows, long long ldx, in
     auto slice = [&](int r) { return ((p.chunks + r - 1) / r + STAGE_CHUNKS - 1) / STAGE_CHUNKS * STAGE_CHUNKS; };
     while (ranks > 1 && slice(ranks) * (ranks - 1) >= p.chunks) ranks /= 2;
     p.slice = slice(ranks);
-    switch (nb) {
-        case 16: return launch_form<16>(map, p, ranks, stream);
-        case 32: return launch_form<32>(map, p, ranks, stream);
-        case 48: return launch_form<48>(map, p, ranks, stream);
-        default: return launch_form<64>(map, p, ranks, stream);
+    // rows in slabs of about the same size
+    const int most = w.f32 ? W4_TC_ROWS_F32 : W4_TC_ROWS, slabs = (w.rows + most - 1) / most, slab = (w.rows + slabs - 1) / slabs;
+    for (int row = 0; row < w.rows; row += slab) {
+        p.rows = w.rows - row < slab ? w.rows - row : slab;
+        p.out = static_cast<char*>(w.out) + (long long)row * w.ldo * (w.f32 ? 4 : 2);
+        const int x_rows = times * p.rows, nb = x_rows <= 16 ? 16 : (x_rows <= 32 ? 32 : (x_rows <= 48 ? 48 : 64));
+        CUtensorMap map;
+        if (!tensor_map(x + (long long)times * row * ldx, w.K, x_rows, ldx, nb, true, &map)) return TIS_CUDA_ERROR;
+        const int status = nb == 16 ? launch_form<16>(map, p, ranks, stream) : nb == 32 ? launch_form<32>(map, p, ranks, stream)
+                         : nb == 48 ? launch_form<48>(map, p, ranks, stream) : launch_form<64>(map, p, ranks, stream);
+        if (status != TIS_OK) return status;
     }
+    return TIS_OK;
 }

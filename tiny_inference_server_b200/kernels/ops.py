@@ -35,7 +35,7 @@ class KernelError(RuntimeError):
 #: layouts of the arguments of launchers that take them as one block of 64-bit values (q: whole, d: floating point): a call with
 #: twenty arguments costs ctypes 2.5 us, the same packed 0.9
 _VERIFY_ARGS = struct.Struct("15q")
-_W4_ARGS = struct.Struct("15q")
+_W4_ARGS = struct.Struct("16q")
 _SHARED_ARGS = struct.Struct("28qd")
 
 
@@ -659,7 +659,13 @@ def gemm_f32_out(a: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
 # row-wise kernels
 # ---------------------------------------------------------------------------------------
 
-W4_TENSOR = os.environ.get("W4T", "1") != "0"
+#: gemm_w4: most staged rows (a row of float32 is three) of the mma.sync kernel, and the bytes of x up to which it holds it in one piece; beyond
+#: either the tcgen05 kernel takes the product.  us, mma.sync / tcgen05, groups of 128: 1536 x 2304 at 1, 8, 16, 24, 32 rows 2.4 / 5.0, 3.2 / 5.2,
+#: 4.9 / 5.5, 6.1 / 6.1, 11.4 / 6.2; 4096 x 4096 at 8 and 9 rows (x in one piece, in several) 7.9 / 9.1, 26.5 / 9.2; 4096 x 28672 at 8, 9, 32
+#: 26.3 / 36.9, 36.2 / 36.9, 79.5 / 40.9; 8192 x 1024 at 1 row (several pieces) 22.5 / 8.2
+W4_MMA_ROWS, W4_MMA_BYTES = 24, 108 * 1024
+#: for tests and measurements: False or True sends all of them to the one or the other
+W4_TENSOR: Optional[bool] = None
 
 
 def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -667,7 +673,8 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
     free.  Every weight is taken as it is, (code - zero) * scale, and a sum is rounded once, when it is stored.
 
     For few rows: the weights are streamed once for up to 64 rows of bfloat16 and 21 of float32, and again for as many more.  (A prompt's rows
-    are better off with ``weights.w4.unpack_w4`` and ``gemm``.)"""
+    are better off with ``weights.w4.unpack_w4`` and ``gemm``.)  Two kernels, chosen by rows and K (``W4_MMA_ROWS``); float32 rows, and
+    bfloat16 ones that do not start on 16 bytes, are copied for the second."""
     dtype = a.dtype
     if (dtype is not torch.bfloat16 and dtype is not torch.float32) or a.ndim != 2:
         raise KernelError(f"gemm_w4: rows {dtype} {tuple(a.shape)}; bfloat16 or float32 are taken")
@@ -692,9 +699,18 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
     lib = _lib or library()
     calls["gemm_w4"] += 1
     words, scales, zeros = w.pointers
-    tensor = W4_TENSOR and dtype is torch.bfloat16 and n <= 64 and not (k % 8 or lda % 8 or a.data_ptr() % 16) and lda >= k
+    staged = n if dtype is torch.bfloat16 else 3 * n
+    tensor = W4_TENSOR
+    if tensor is None:
+        tensor = staged > W4_MMA_ROWS or -(-staged // 8) * 16 * (k + 64) > W4_MMA_BYTES
+    copy = at = fault = 0
+    if tensor:
+        fault = tc_fault().data_ptr()
+        if dtype is not torch.bfloat16 or k % 8 or lda % 8 or lda < k or a.data_ptr() % 16:
+            copy = torch.empty((staged, -(-k // 8) * 8), dtype=torch.bfloat16, device=a.device)
+            at = copy.data_ptr()
     _check(lib.tis_gemm_w4(_W4_ARGS.pack(1 if dtype is torch.bfloat16 else 0, a.data_ptr(), lda, words, scales, zeros, out.data_ptr(), ldo, n, k,
-                                         cols, w.group, tensor, tc_fault().data_ptr() if tensor else 0, _stream_number(device))), lib)
+                                         cols, w.group, tensor, at, fault, _stream_number(device))), lib)
     return out
 
 
