@@ -513,15 +513,23 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
 }
 
 // ---- float32: dot products on the CUDA cores, everything in 32 bits ---------------------------------------------------------
-// A CTA has up to 16 row heads; a warp takes every fourth key of the part, a lane's share of the head a stride of 32, and keeps sums of its own for
-// four row heads at a time.
-constexpr int F32_ROWS = 4, F32_LANES = (HD + 31) / 32;
+// R row heads of a tile at a time.  A warp takes 32 keys: first a lane a key (its row against the queries in shared memory, which all lanes
+// read at once), then, with the probabilities in shared memory, a lane four columns (HD / 4 lanes or the next power of two a key, the
+// groups of lanes taking turns).  All loads of 32 keys are independent of one another.  The four warps take turns and merge at the end.
+constexpr int F32_LANES = (HD + 31) / 32;
+constexpr int F32_QUADS = HD / 4, F32_GROUP = F32_QUADS > 16 ? 32 : F32_QUADS > 8 ? 16 : F32_QUADS > 4 ? 8 : 4;
+constexpr int F32_TURNS = 32 / F32_GROUP, F32_EACH = (F32_QUADS + F32_GROUP - 1) / F32_GROUP;        // keys at a time, quads of a lane
+template <int R> constexpr int f32_floats() { return R * HD + 4 * 32 * R + 4 * R * HD; }     // queries, probabilities, the warps' shares
 
-template <bool OWN>
+template <bool OWN, int R>
 __global__ void __launch_bounds__(MMA_THREADS)
 shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int part0) {
-    __shared__ float merge_o[4][F32_ROWS][HD];
-    __shared__ float merge_m[4][F32_ROWS], merge_l[4][F32_ROWS];
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    float* q_smem = reinterpret_cast<float*>(smem_raw);     // [R][HD]
+    float* prob = q_smem + R * HD;                          // [warp][key][R]
+    float* merge_o = prob + 4 * 32 * R;                     // [warp][R][HD]
+    __shared__ float merge_m[4][R], merge_l[4][R];
+    __shared__ size_t row_at[4][32];
     __shared__ int row_pos[16];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -530,88 +538,119 @@ shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
     const int G = p.H / p.KVH;
     constexpr int NCH = HD / 4;
     pdl_wait();
-    if (threadIdx.x < 16) {
-        const int i = threadIdx.x;
-        const int pos = i < t.count ? p.positions[(t.rh0 + i) / G] : -1;
-        row_pos[i] = pos >= t.prefix ? pos : -1;
-    }
+    if (threadIdx.x < 16) row_pos[threadIdx.x] = position_of(p, t, threadIdx.x);
     __syncthreads();
     const int shared = shared_keys(p, t);
-    for (int i0 = 0; i0 < t.count; i0 += F32_ROWS) {
-        int last = shared, pos[F32_ROWS];
-        bool any = false;
-        float q[F32_ROWS][F32_LANES], o[F32_ROWS][F32_LANES], m[F32_ROWS], l[F32_ROWS];
+    int last = shared;
+    if (OWN)
+        for (int i = 0; i < t.count; ++i) last = max(last, row_pos[i] + 1);
+    const Range keys = part_range(OWN ? shared : 0, last, OWN ? shared & ~63 : 0, part, parts, 64);
+    const size_t v_step = (size_t)p.KVH * p.page * HD;
+    const int group = lane / F32_GROUP, quad = lane % F32_GROUP;
+    for (int i0 = 0; i0 < t.count; i0 += R) {
+        int pos[R], least = 0x7fffffff, most = -1;
 #pragma unroll
-        for (int r = 0; r < F32_ROWS; ++r) {
+        for (int r = 0; r < R; ++r) {
             pos[r] = i0 + r < t.count ? row_pos[i0 + r] : -1;
-            any |= pos[r] >= 0;
-            if (OWN) last = max(last, pos[r] + 1);
-            m[r] = -INFINITY;
-            l[r] = 0.f;
-            const int rh = t.rh0 + min(i0 + r, t.count - 1);
-            const float* src = static_cast<const float*>(p.q) + (long long)(rh / G) * p.ldq + (kvh * G + rh % G) * HD;
-#pragma unroll
-            for (int e = 0; e < F32_LANES; ++e) {
-                q[r][e] = lane + e * 32 < HD ? src[lane + e * 32] : 0.f;
-                o[r][e] = 0.f;
-            }
+            if (pos[r] >= 0) { least = min(least, pos[r]); most = max(most, pos[r]); }
         }
-        // (rows of a tile may end at different keys: the part is one of the tile's keys, the same for all)
-        int tile_last = shared;
-        if (OWN)
-            for (int i = 0; i < t.count; ++i) tile_last = max(tile_last, row_pos[i] + 1);
-        const Range keys = part_range(OWN ? shared : 0, tile_last, OWN ? shared & ~63 : 0, part, parts, 64);
-        const int hi = any ? min(keys.hi, last) : keys.lo;
-        for (int key = keys.lo + warp; key < hi; key += 4) {
-            const size_t at = (((size_t)page_at(p, t.slot, key / p.page) * 2 * p.KVH + kvh) * p.page + key % p.page) * HD;
-            const float* k = static_cast<const float*>(p.plane) + at;
-            const float* v = k + (size_t)p.KVH * p.page * HD;
-            float kx[F32_LANES], vx[F32_LANES], s[F32_ROWS];
-#pragma unroll
-            for (int e = 0; e < F32_LANES; ++e) {
-                const int d = lane + e * 32;
-                const int from = d < HD ? cache_chunk(d / 4, key, NCH) * 4 + d % 4 : 0;
-                kx[e] = d < HD ? k[from] : 0.f;
-                vx[e] = d < HD ? v[from] : 0.f;
-            }
-#pragma unroll
-            for (int r = 0; r < F32_ROWS; ++r) {
-                s[r] = 0.f;
-#pragma unroll
-                for (int e = 0; e < F32_LANES; ++e) s[r] = fmaf(q[r][e], kx[e], s[r]);
-            }
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1)
-#pragma unroll
-                for (int r = 0; r < F32_ROWS; ++r) s[r] += __shfl_xor_sync(ALL, s[r], w);
-#pragma unroll
-            for (int r = 0; r < F32_ROWS; ++r) {
-                if (OWN ? key > pos[r] : pos[r] < 0) continue;          // (uniform in the warp)
-                const float x = s[r] * p.scale_log2;
-                if (x > m[r]) {
-                    const float f = exp2f(m[r] - x);                    // (of minus infinity: 0)
-                    l[r] *= f;
-#pragma unroll
-                    for (int e = 0; e < F32_LANES; ++e) o[r][e] *= f;
-                    m[r] = x;
-                }
-                const float w = exp2f(x - (m[r] == -INFINITY ? 0.f : m[r]));
-                l[r] += w;
-#pragma unroll
-                for (int e = 0; e < F32_LANES; ++e) o[r][e] = fmaf(w, vx[e], o[r][e]);
-            }
-        }
-        __syncthreads();                                    // (the merge of the rows before has been read)
-#pragma unroll
-        for (int r = 0; r < F32_ROWS; ++r) {
-            if (lane == 0) { merge_m[warp][r] = m[r]; merge_l[warp][r] = l[r]; }
-#pragma unroll
-            for (int e = 0; e < F32_LANES; ++e)
-                if (lane + e * 32 < HD) merge_o[warp][r][lane + e * 32] = o[r][e];
+        __syncthreads();                                    // (the rows before have been merged and stored)
+        for (int i = threadIdx.x; i < R * HD; i += MMA_THREADS) {
+            const int rh = t.rh0 + min(i0 + i / HD, t.count - 1);
+            q_smem[i] = static_cast<const float*>(p.q)[(long long)(rh / G) * p.ldq + (kvh * G + rh % G) * HD + i % HD];
         }
         __syncthreads();
-        const int r = warp;                                 // a warp a row head
-        if (i0 + r < t.count) {
+        float m[R], l[R], o[R][F32_EACH][4];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+#pragma unroll
+            for (int e = 0; e < F32_EACH * 4; ++e) o[r][e / 4][e % 4] = 0.f;
+        }
+        const int hi = most < 0 ? keys.lo : (OWN ? min(keys.hi, most + 1) : keys.hi);
+        for (int k0 = keys.lo + warp * 32; k0 < hi; k0 += 128) {
+            // ---- scores: a lane a key (behind the last one: the last once more, seen by no row) ----
+            const int key = min(k0 + lane, hi - 1), n = min(32, hi - k0);
+            const size_t at = (((size_t)page_at(p, t.slot, key / p.page) * 2 * p.KVH + kvh) * p.page + key % p.page) * HD;
+            const float* k = static_cast<const float*>(p.plane) + at;
+            row_at[warp][lane] = at + v_step;
+            float s[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) s[r] = 0.f;
+            const int turn = NCH % 8 == 0 ? key & 7 : key % NCH;
+#pragma unroll 8
+            for (int c = 0; c < NCH; ++c) {
+                const int stored = NCH % 8 == 0 ? c ^ turn : c + turn - (c + turn >= NCH ? NCH : 0);
+                const float4 x = *reinterpret_cast<const float4*>(k + stored * 4);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float4 y = *reinterpret_cast<const float4*>(q_smem + r * HD + c * 4);
+                    s[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[r]))));
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const bool sees = lane < n && pos[r] >= 0 && (!OWN || key <= pos[r]);
+                s[r] = sees ? s[r] * p.scale_log2 : -INFINITY;
+                float top = s[r];
+#pragma unroll
+                for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(ALL, top, w));
+                if (top > m[r]) {                           // (uniform in the warp)
+                    const float f = m[r] == -INFINITY ? 1.f : exp2f(m[r] - top);       // (no sums yet, but what is not finite: that stays)
+                    l[r] *= f;
+#pragma unroll
+                    for (int e = 0; e < F32_EACH * 4; ++e) o[r][e / 4][e % 4] *= f;
+                    m[r] = top;
+                }
+                s[r] = sees ? exp2f(s[r] - (m[r] == -INFINITY ? 0.f : m[r])) : 0.f;
+                l[r] += s[r];                               // (a lane's share: added up over the lanes at the end)
+                prob[(warp * 32 + lane) * R + r] = s[r];
+            }
+            __syncwarp();
+            // ---- values: a lane four columns of one of the keys whose turn it is ----
+#pragma unroll 4
+            for (int j = group; j < n; j += F32_TURNS) {
+                const int key_j = k0 + j;
+                const float* v = static_cast<const float*>(p.plane) + row_at[warp][j];
+                const int turn_j = NCH % 8 == 0 ? key_j & 7 : key_j % NCH;
+#pragma unroll
+                for (int e = 0; e < F32_EACH; ++e) {
+                    const int c = quad + e * F32_GROUP;
+                    if (c >= F32_QUADS) continue;
+                    const int stored = NCH % 8 == 0 ? c ^ turn_j : c + turn_j - (c + turn_j >= NCH ? NCH : 0);
+                    const float4 x = *reinterpret_cast<const float4*>(v + stored * 4);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        if (key_j > least && (pos[r] < 0 || (OWN && key_j > pos[r]))) continue;     // (a probability of 0 does not take away what is not finite)
+                        const float w = prob[(warp * 32 + j) * R + r];
+                        o[r][e][0] = fmaf(w, x.x, o[r][e][0]);
+                        o[r][e][1] = fmaf(w, x.y, o[r][e][1]);
+                        o[r][e][2] = fmaf(w, x.z, o[r][e][2]);
+                        o[r][e][3] = fmaf(w, x.w, o[r][e][3]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) l[r] += __shfl_xor_sync(ALL, l[r], w);
+#pragma unroll
+            for (int e = 0; e < F32_EACH * 4; ++e)
+#pragma unroll
+                for (int w = F32_GROUP; w < 32; w <<= 1) o[r][e / 4][e % 4] += __shfl_xor_sync(ALL, o[r][e / 4][e % 4], w);
+            if (lane == 0) { merge_m[warp][r] = m[r]; merge_l[warp][r] = l[r]; }
+#pragma unroll
+            for (int e = 0; e < F32_EACH; ++e) {
+                const int c = quad + e * F32_GROUP;
+                if (group == 0 && c < F32_QUADS)
+                    *reinterpret_cast<float4*>(merge_o + (warp * R + r) * HD + c * 4) = make_float4(o[r][e][0], o[r][e][1], o[r][e][2], o[r][e][3]);
+            }
+        }
+        __syncthreads();
+        for (int r = warp; r < R && i0 + r < t.count; r += 4) {
             const float M = fmaxf(fmaxf(merge_m[0][r], merge_m[1][r]), fmaxf(merge_m[2][r], merge_m[3][r]));
             float f[4], sum = 0.f;
 #pragma unroll
@@ -620,13 +659,13 @@ shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
                 sum += merge_l[w][r] * f[w];
             }
             const int rh = t.rh0 + i0 + r;
-            const size_t at = ((size_t)(part0 + part) * p.rows + rh / G) * p.H + kvh * G + rh % G;
-            if (lane == 0) p.part_ml[at] = make_float2(M, sum);
+            const size_t to = ((size_t)(part0 + part) * p.rows + rh / G) * p.H + kvh * G + rh % G;
+            if (lane == 0) p.part_ml[to] = make_float2(M, sum);
             for (int d = lane; d < HD; d += 32) {
                 float x = 0.f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) x += merge_o[w][r][d] * f[w];
-                p.part_o[at * HD + d] = x;
+                for (int w = 0; w < 4; ++w) x += merge_o[(w * R + r) * HD + d] * f[w];
+                p.part_o[to * HD + d] = x;
             }
         }
     }
@@ -701,6 +740,19 @@ template <typename T> int launch_join(const SharedParams& p, void* out, long lon
     return tis_check_launch("shared_prefix_attention (join)");
 }
 
+template <bool OWN, int R> int launch_f32(const SharedParams& p, const SharedTile* tiles, int count, int parts, int part0, cudaStream_t stream) {
+    const int smem = f32_floats<R>() * 4;
+    static DeviceOnce configured;
+    if (configured.first() && cudaFuncSetAttribute(shared_f32_kernel<OWN, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return tis_check_launch("shared_prefix_attention (shared memory)");
+    tis_launch(shared_f32_kernel<OWN, R>, dim3((unsigned)(count * parts * p.KVH)), dim3(MMA_THREADS), (size_t)smem, stream, p, tiles, parts, part0);
+    return tis_check_launch("shared_prefix_attention");
+}
+// row heads at a time: eight, or four where no tile has more (a tile's keys are read once for them)
+template <bool OWN> int launch_f32_rows(const SharedParams& p, const SharedTile* tiles, int count, int heads, int parts, int part0, cudaStream_t stream) {
+    return heads <= 4 ? launch_f32<OWN, 4>(p, tiles, count, parts, part0, stream) : launch_f32<OWN, 8>(p, tiles, count, parts, part0, stream);
+}
+
 template <bool OWN, int WR, int MT> int launch_mma(const SharedParams& p, const SharedTile* tiles, int count, int parts, int part0, int beside, cudaStream_t stream) {
     constexpr int ROWS = 16 * WR * MT;
     const size_t smem = (size_t)STAGES * 2 * TILE_ELEMENTS * 2 + (size_t)(WR == 1 ? 2 : 1) * ROWS * HD * 2 + (WR == 1 ? 2 * 16 * HD * 4 : 0);
@@ -723,13 +775,14 @@ TIS_API int tis_shared_attn_head_dim() { return HD; }
 TIS_API int tis_shared_attn_widest() { return HD <= 128 ? 128 : 64; }
 
 // `own`, `wide`: tiles on the device, own ones of up to 16 row heads, shared ones of up to `wide_rows`: 16, and in bfloat16
-// 64 or 128 (tis_shared_attn_widest); `tensor`: shared tiles by the tcgen05 kernel, which takes up to 128.
+// 64 or 128 (tis_shared_attn_widest); `tensor`: shared tiles by the tcgen05 kernel, which takes up to
+// 128.  most_heads, own_heads: row heads of the largest group and of the largest request.
 // The first `shared_parts` parts of the scratch are the shared tiles', the `own_parts` behind them the own ones'; rows of groups
 // without shared keys have empty ones.  `rows`: the rows of the plan, all of which are written.
 TIS_API int tis_shared_attn_tensor(int page) { return shared_tc_takes(page); }
 struct SharedArgs {
     long long dtype, q, ldq, out, ldo, plane, table, table_stride, table_width, num_pages, positions, own, own_count, wide, wide_count, wide_rows,
-        tensor, own_parts, shared_parts, rows, H, KVH, page, part_o, part_ml, fault, stream, unused;
+        tensor, own_parts, shared_parts, rows, H, KVH, page, part_o, part_ml, fault, stream, most_heads, own_heads;
     double scale;
 };
 TIS_API int tis_shared_attention(const SharedArgs* a) {
@@ -768,14 +821,8 @@ TIS_API int tis_shared_attention(const SharedArgs* a) {
     const int parts = own_parts + shared_parts, row_heads = rows * H;
     int status = TIS_OK;
     if (dtype == TIS_F32) {
-        if (shared_parts > 0) {
-            tis_launch(shared_f32_kernel<false>, dim3((unsigned)(wide_count * shared_parts * KVH)), dim3(MMA_THREADS), 0, stream, p, w, shared_parts, 0);
-            status = tis_check_launch("shared_prefix_attention");
-        }
-        if (status == TIS_OK) {
-            tis_launch(shared_f32_kernel<true>, dim3((unsigned)(own_count * own_parts * KVH)), dim3(MMA_THREADS), 0, stream, p, o, own_parts, shared_parts);
-            status = tis_check_launch("shared_prefix_attention");
-        }
+        if (shared_parts > 0) status = launch_f32_rows<false>(p, w, wide_count, (int)a->most_heads, shared_parts, 0, stream);
+        if (status == TIS_OK) status = launch_f32_rows<true>(p, o, own_count, (int)a->own_heads, own_parts, shared_parts, stream);
     } else if (dtype == TIS_BF16) {
         if (shared_parts > 0) {
             if (tensor) status = shared_tc_launch(p, w, wide_count, shared_parts, stream);

@@ -114,7 +114,7 @@ class SharedPrefixPlan:
         self.num_heads, self.kv_heads, self.group_size = num_heads, kv_heads, num_heads // kv_heads
         g = self.group_size
         own, shared_tiles = [], {size: [] for size in self.SHARED_TILES}
-        self.most_heads = 0                                   # row heads of the largest group
+        self.most_heads = self.own_heads = 0                  # row heads of the largest group, of the largest request
         rows, self.max_slot, self.max_shared, self.min_shared, slots = 0, -1, 0, None, set()
         for shared, requests in groups:
             if shared < 0 or not requests:
@@ -124,6 +124,7 @@ class SharedPrefixPlan:
                 if slot < 0 or n <= 0 or slot in slots:
                     raise ValueError(f"slot {slot} with {n} rows: every request stands once in a plan, with at least one row")
                 slots.add(slot)
+                self.own_heads = max(self.own_heads, n * g)
                 own += [(rows * g + a, min(self.OWN_TILE, n * g - a), slot, shared) for a in range(0, n * g, self.OWN_TILE)]
                 rows += n
             heads = (rows - first) * g

@@ -36,7 +36,7 @@ class KernelError(RuntimeError):
 #: twenty arguments costs ctypes 2.5 us, the same packed 0.9
 _VERIFY_ARGS = struct.Struct("15q")
 _W4_ARGS = struct.Struct("16q")
-_SHARED_ARGS = struct.Struct("28qd")
+_SHARED_ARGS = struct.Struct("29qd")
 
 
 def library():
@@ -1123,7 +1123,7 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     at = scratch.data_ptr()
     _check(lib.tis_shared_attention(_SHARED_ARGS.pack(code, q_at, ldq, out.data_ptr(), ldo, plane_at, block_table.data_ptr(), table_stride, width,
                                                       pages, positions.data_ptr(), *split[1:], rows, h, kvh, page, at, at + 4 * part_rows * hd,
-                                                      fault.data_ptr(), _stream_number(device), 0, scale)), lib)
+                                                      fault.data_ptr(), _stream_number(device), plan.most_heads, plan.own_heads, scale)), lib)
     return out
 
 
