@@ -513,31 +513,38 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
 }
 
 // ---- float32: dot products on the CUDA cores, everything in 32 bits ---------------------------------------------------------
-// R row heads of a tile at a time.  A warp takes 32 keys: first a lane a key (its row against the queries in shared memory, which all lanes
+// A CTA has R row heads of a tile, four: with eight or sixteen the keys are read fewer times, but a CTA that goes once through code unrolled for
+// that many spends its time fetching it (4 requests behind 1000 keys, 12 heads of 64: 20.7 us with 4, 32.4 with 8; 8 requests of 3 rows behind
+// 2048, 32 heads of 128: 128 and 167).  A warp takes 32 keys: first a lane a key (its row against the queries in shared memory, which all lanes
 // read at once), then, with the probabilities in shared memory, a lane four columns (HD / 4 lanes or the next power of two a key, the
 // groups of lanes taking turns).  All loads of 32 keys are independent of one another.  The four warps take turns and merge at the end.
 constexpr int F32_LANES = (HD + 31) / 32;
 constexpr int F32_QUADS = HD / 4, F32_GROUP = F32_QUADS > 16 ? 32 : F32_QUADS > 8 ? 16 : F32_QUADS > 4 ? 8 : 4;
 constexpr int F32_TURNS = 32 / F32_GROUP, F32_EACH = (F32_QUADS + F32_GROUP - 1) / F32_GROUP;        // keys at a time, quads of a lane
+constexpr int F32_AHEAD = 8;                // loads of a lane on their way
 template <int R> constexpr int f32_floats() { return R * HD + 4 * 32 * R + 4 * R * HD; }     // queries, probabilities, the warps' shares
 
 template <bool OWN, int R>
 __global__ void __launch_bounds__(MMA_THREADS)
-shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int part0) {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
+shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int part0, int beside) {
+    extern __shared__ __align__(128) unsigned char smem_raw[];
     float* q_smem = reinterpret_cast<float*>(smem_raw);     // [R][HD]
     float* prob = q_smem + R * HD;                          // [warp][key][R]
     float* merge_o = prob + 4 * 32 * R;                     // [warp][R][HD]
     __shared__ float merge_m[4][R], merge_l[4][R];
     __shared__ size_t row_at[4][32];
     __shared__ int row_pos[16];
-    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kvh = blockIdx.x % p.KVH, part = blockIdx.x / p.KVH % parts;
+    const int kvh = blockIdx.x % p.KVH, part = blockIdx.x / p.KVH % parts, i0 = (int)blockIdx.y * R;
     const SharedTile t = tiles[blockIdx.x / p.KVH / parts];
+    if (i0 >= t.count) {                                    // (a tile of fewer row heads than the largest)
+        pdl_wait();
+        return;
+    }
     const int G = p.H / p.KVH;
     constexpr int NCH = HD / 4;
-    pdl_wait();
+    if (!beside) pdl_wait();                                // (as above)
+    pdl_launch_dependents();
     if (threadIdx.x < 16) row_pos[threadIdx.x] = position_of(p, t, threadIdx.x);
     __syncthreads();
     const int shared = shared_keys(p, t);
@@ -547,14 +554,13 @@ shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
     const Range keys = part_range(OWN ? shared : 0, last, OWN ? shared & ~63 : 0, part, parts, 64);
     const size_t v_step = (size_t)p.KVH * p.page * HD;
     const int group = lane / F32_GROUP, quad = lane % F32_GROUP;
-    for (int i0 = 0; i0 < t.count; i0 += R) {
+    {
         int pos[R], least = 0x7fffffff, most = -1;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             pos[r] = i0 + r < t.count ? row_pos[i0 + r] : -1;
             if (pos[r] >= 0) { least = min(least, pos[r]); most = max(most, pos[r]); }
         }
-        __syncthreads();                                    // (the rows before have been merged and stored)
         for (int i = threadIdx.x; i < R * HD; i += MMA_THREADS) {
             const int rh = t.rh0 + min(i0 + i / HD, t.count - 1);
             q_smem[i] = static_cast<const float*>(p.q)[(long long)(rh / G) * p.ldq + (kvh * G + rh % G) * HD + i % HD];
@@ -579,14 +585,21 @@ shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
 #pragma unroll
             for (int r = 0; r < R; ++r) s[r] = 0.f;
             const int turn = NCH % 8 == 0 ? key & 7 : key % NCH;
-#pragma unroll 8
-            for (int c = 0; c < NCH; ++c) {
-                const int stored = NCH % 8 == 0 ? c ^ turn : c + turn - (c + turn >= NCH ? NCH : 0);
-                const float4 x = *reinterpret_cast<const float4*>(k + stored * 4);
+            for (int c0 = 0; c0 < NCH; c0 += F32_AHEAD) {
+                float4 x[F32_AHEAD];
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float4 y = *reinterpret_cast<const float4*>(q_smem + r * HD + c * 4);
-                    s[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[r]))));
+                for (int a = 0; a < F32_AHEAD; ++a) {
+                    const int c = min(c0 + a, NCH - 1);
+                    x[a] = *reinterpret_cast<const float4*>(k + (NCH % 8 == 0 ? c ^ turn : c + turn - (c + turn >= NCH ? NCH : 0)) * 4);
+                }
+#pragma unroll
+                for (int a = 0; a < F32_AHEAD; ++a) {
+                    if (NCH % F32_AHEAD != 0 && c0 + a >= NCH) continue;
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const float4 y = *reinterpret_cast<const float4*>(q_smem + r * HD + (c0 + a) * 4);
+                        s[r] = fmaf(x[a].x, y.x, fmaf(x[a].y, y.y, fmaf(x[a].z, y.z, fmaf(x[a].w, y.w, s[r]))));
+                    }
                 }
             }
 #pragma unroll
@@ -609,25 +622,31 @@ shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
             }
             __syncwarp();
             // ---- values: a lane four columns of one of the keys whose turn it is ----
-#pragma unroll 4
-            for (int j = group; j < n; j += F32_TURNS) {
-                const int key_j = k0 + j;
-                const float* v = static_cast<const float*>(p.plane) + row_at[warp][j];
-                const int turn_j = NCH % 8 == 0 ? key_j & 7 : key_j % NCH;
+            for (int j0 = group; j0 < n; j0 += F32_TURNS * F32_AHEAD) {
 #pragma unroll
                 for (int e = 0; e < F32_EACH; ++e) {
-                    const int c = quad + e * F32_GROUP;
-                    if (c >= F32_QUADS) continue;
-                    const int stored = NCH % 8 == 0 ? c ^ turn_j : c + turn_j - (c + turn_j >= NCH ? NCH : 0);
-                    const float4 x = *reinterpret_cast<const float4*>(v + stored * 4);
+                    const int c = min(quad + e * F32_GROUP, F32_QUADS - 1);         // (a lane too many reads what its neighbour reads)
+                    float4 x[F32_AHEAD];
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        if (key_j > least && (pos[r] < 0 || (OWN && key_j > pos[r]))) continue;     // (a probability of 0 does not take away what is not finite)
-                        const float w = prob[(warp * 32 + j) * R + r];
-                        o[r][e][0] = fmaf(w, x.x, o[r][e][0]);
-                        o[r][e][1] = fmaf(w, x.y, o[r][e][1]);
-                        o[r][e][2] = fmaf(w, x.z, o[r][e][2]);
-                        o[r][e][3] = fmaf(w, x.w, o[r][e][3]);
+                    for (int a = 0; a < F32_AHEAD; ++a) {
+                        const int j = min(j0 + a * F32_TURNS, n - 1), turn_j = NCH % 8 == 0 ? (k0 + j) & 7 : (k0 + j) % NCH;
+                        x[a] = *reinterpret_cast<const float4*>(static_cast<const float*>(p.plane) + row_at[warp][j] +
+                                                                (NCH % 8 == 0 ? c ^ turn_j : c + turn_j - (c + turn_j >= NCH ? NCH : 0)) * 4);
+                    }
+#pragma unroll
+                    for (int a = 0; a < F32_AHEAD; ++a) {
+                        const int j = j0 + a * F32_TURNS;
+                        if (j >= n) continue;
+                        const bool some = k0 + j > least;   // do not see it: a probability of 0 does not take away what is not finite
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            if (some && (pos[r] < 0 || (OWN && k0 + j > pos[r]))) continue;
+                            const float w = prob[(warp * 32 + j) * R + r];
+                            o[r][e][0] = fmaf(w, x[a].x, o[r][e][0]);
+                            o[r][e][1] = fmaf(w, x[a].y, o[r][e][1]);
+                            o[r][e][2] = fmaf(w, x[a].z, o[r][e][2]);
+                            o[r][e][3] = fmaf(w, x[a].w, o[r][e][3]);
+                        }
                     }
                 }
             }
@@ -669,6 +688,7 @@ shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
             }
         }
     }
+    if (beside) pdl_wait();
 }
 
 // ---- the parts of a row head joined ------------------------------------------------------------------------------------------
@@ -740,17 +760,15 @@ template <typename T> int launch_join(const SharedParams& p, void* out, long lon
     return tis_check_launch("shared_prefix_attention (join)");
 }
 
-template <bool OWN, int R> int launch_f32(const SharedParams& p, const SharedTile* tiles, int count, int parts, int part0, cudaStream_t stream) {
-    const int smem = f32_floats<R>() * 4;
+template <bool OWN> int launch_f32(const SharedParams& p, const SharedTile* tiles, int count, int heads, int parts, int part0, int beside, cudaStream_t stream) {
+    constexpr int R = 4, smem = f32_floats<R>() * 4;
+    heads = heads < 16 ? heads : 16;                        // (of a tile)
     static DeviceOnce configured;
     if (configured.first() && cudaFuncSetAttribute(shared_f32_kernel<OWN, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return tis_check_launch("shared_prefix_attention (shared memory)");
-    tis_launch(shared_f32_kernel<OWN, R>, dim3((unsigned)(count * parts * p.KVH)), dim3(MMA_THREADS), (size_t)smem, stream, p, tiles, parts, part0);
+    tis_launch(shared_f32_kernel<OWN, R>, dim3((unsigned)(count * parts * p.KVH), (unsigned)((heads + R - 1) / R)), dim3(MMA_THREADS), (size_t)smem, stream,
+               p, tiles, parts, part0, beside);
     return tis_check_launch("shared_prefix_attention");
-}
-// row heads at a time: eight, or four where no tile has more (a tile's keys are read once for them)
-template <bool OWN> int launch_f32_rows(const SharedParams& p, const SharedTile* tiles, int count, int heads, int parts, int part0, cudaStream_t stream) {
-    return heads <= 4 ? launch_f32<OWN, 4>(p, tiles, count, parts, part0, stream) : launch_f32<OWN, 8>(p, tiles, count, parts, part0, stream);
 }
 
 template <bool OWN, int WR, int MT> int launch_mma(const SharedParams& p, const SharedTile* tiles, int count, int parts, int part0, int beside, cudaStream_t stream) {
@@ -821,8 +839,8 @@ TIS_API int tis_shared_attention(const SharedArgs* a) {
     const int parts = own_parts + shared_parts, row_heads = rows * H;
     int status = TIS_OK;
     if (dtype == TIS_F32) {
-        if (shared_parts > 0) status = launch_f32_rows<false>(p, w, wide_count, (int)a->most_heads, shared_parts, 0, stream);
-        if (status == TIS_OK) status = launch_f32_rows<true>(p, o, own_count, (int)a->own_heads, own_parts, shared_parts, stream);
+        if (shared_parts > 0) status = launch_f32<false>(p, w, wide_count, (int)a->most_heads, shared_parts, 0, 0, stream);
+        if (status == TIS_OK) status = launch_f32<true>(p, o, own_count, (int)a->own_heads, own_parts, shared_parts, shared_parts > 0, stream);
     } else if (dtype == TIS_BF16) {
         if (shared_parts > 0) {
             if (tensor) status = shared_tc_launch(p, w, wide_count, shared_parts, stream);
