@@ -190,18 +190,9 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
         // ---- codes to bfloat16: a warp has two strips, 32 lanes of tensor memory, of every other chunk: the two of a stage are two warps' ----
         static_assert(STAGE_CHUNKS == 2, "a chunk of a stage each");
         const int quarter = warp & 3, u = warp >> 2;
-        int stage = 0, stored = -1;                         // stages so far, the operand whose store is under way
+        int stage = 0;
         bool ok = true;
         const int g = lane >> 2;
-        auto finish = [&]() {                               // the store is done: over to the products
-            if (stored >= 0) {
-                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[stored]);
-                stored = -1;
-            }
-        };
         for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
             const unsigned short* zeros[2];
             int seen = -1;                                  // the group whose zero points are here
@@ -223,9 +214,12 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
                     }
                     seen = group;
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (stage / STAGES) & 1, abort, p.fault, 6));
-                if (!ok) break;
                 const int as = stage % A_STAGES;
+                ok = __all_sync(0xffffffffu, mbar_wait_both(&full[s], (stage / STAGES) & 1, &a_empty[as], ((stage / A_STAGES) & 1) ^ 1, abort, p.fault, 6));
+                if (!ok) break;
+                // the products of the stage before the one before are done: its place in the ring is free, codes and rows of x
+                if (stage >= A_STAGES && lane == 0) mbar_arrive(&empty[(stage - A_STAGES) % STAGES]);
+                fence_after();
                 unsigned r[2][16];
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {               // (of a chunk beyond the last: what lies there, for an operand that no product takes)
@@ -248,21 +242,15 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
                         r[q][4 * k + 3] = w4_pair(v >> 12, hi);
                     }
                 }
-                finish();                                   // (the store before had the time of the unpacking)
-                ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[as], ((stage / A_STAGES) & 1) ^ 1, abort, p.fault, 6));
-                if (!ok) break;
-                // the products of the stage before the one before are done: its place in the ring is free, codes and rows of x
-                if (stage >= A_STAGES && lane == 0) mbar_arrive(&empty[(stage - A_STAGES) % STAGES]);
-                fence_after();
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
                     tmem_st_16x256b_x4(tmem + ((unsigned)(quarter * 32 + q * 16) << 16) + COL_A + (as * STAGE_CHUNKS + u) * A_COLS, r[q]);
-                stored = as;
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&a_full[as]);
             }
-            // (the tile's last operands are handed over before its sums are waited for elsewhere: nothing behind waits for this warp's next)
-            finish();
         }
-        finish();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 96;\n" ::);
         // ---- a thread a column: the groups' sums, times their scales, added up ----

@@ -161,6 +161,18 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
             const int kvh = item % p.KVH, part = item / p.KVH % parts, slot = n % SLOTS;
             const SharedTile t = tiles[item / p.KVH / parts];
             const int shared = shared_keys(p, t);
+            // ---- queries, a copy a row's heads.  (Copies, pages and positions all go out as soon as the tile is known: one round of loads, not three.) ----
+            ok = __all_sync(ALL, tc::mbar_wait(&q_empty[slot], ((n / SLOTS) & 1) ^ 1, abort, p.fault, 6));
+            if (!ok) break;
+            for (int row = t.rh0 / G + lane; row * G < t.rh0 + t.count; row += 32) {
+                const int a = max(t.rh0, row * G), b = min(t.rh0 + t.count, (row + 1) * G);
+                bulk_copy(q_smem + (slot * ROWS + a - t.rh0) * HD, static_cast<const bf16*>(p.q) + (long long)row * p.ldq + (kvh * G + a - row * G) * HD,
+                          (b - a) * HD * 2, &q_full[slot]);
+            }
+            // the first tile's pages, if it is the part that begins with the first key (else, and if they are not there, they are looked up below)
+            int early = -1;
+            const int first_index = (OWN ? shared / p.page : 0) + lane;
+            if (part == 0 && first_index < p.table_width) early = p.table[(size_t)t.slot * p.table_stride + first_index];
             int last = shared, least = 0x7fffffff;          // keys [.., last) are seen by some row; the smallest position of one that sees any
             int pos[ROWS / 32 + 1];
 #pragma unroll
@@ -183,22 +195,14 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
                 const int index = j < count ? first_page(j) + lane : 0;
                 return j < count && index * p.page < min(kt0 + (j + 1) * KT, keys.hi) ? page_at(p, t.slot, index) : 0;
             };
-            int page = page_of(0);
-            // ---- positions, queries (a copy a row's heads) and what the item is ----
-            ok = __all_sync(ALL, tc::mbar_wait(&q_empty[slot], ((n / SLOTS) & 1) ^ 1, abort, p.fault, 6));
-            if (!ok) break;
+            int page = early >= 0 && early < p.num_pages ? early : page_of(0);
+            // ---- positions, and what the item is ----
 #pragma unroll
             for (int i = 0; i < (ROWS + 31) / 32; ++i)
                 if (lane + i * 32 < ROWS) row_pos[slot][lane + i * 32] = pos[i];
             if (lane == 0) item_of[slot] = Item{t.rh0, t.count, kvh, part, keys.lo, keys.hi, least, all};
             __syncwarp();
             if (lane == 0) tc::mbar_arrive_expect_tx(&q_full[slot], t.count * HD * 2);
-            __syncwarp();
-            for (int row = t.rh0 / G + lane; row * G < t.rh0 + t.count; row += 32) {
-                const int a = max(t.rh0, row * G), b = min(t.rh0 + t.count, (row + 1) * G);
-                bulk_copy(q_smem + (slot * ROWS + a - t.rh0) * HD, static_cast<const bf16*>(p.q) + (long long)row * p.ldq + (kvh * G + a - row * G) * HD,
-                          (b - a) * HD * 2, &q_full[slot]);
-            }
             // ---- keys and values of tile j: its rows in [lo, hi) ----
             for (int j = 0; j < count; ++j, ++stage) {
                 const int next = page_of(j + 1), s = stage % STAGES;
@@ -362,20 +366,20 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
                         }
                 }
                 float top[2];
-                bool raise = false;
+                bool raise[2];                              // (each row for itself: its bits do not depend on the rows beside it)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     top[y] = fmaxf(fmaxf(s[x][0][2 * y], s[x][0][2 * y + 1]), fmaxf(s[x][1][2 * y], s[x][1][2 * y + 1]));
                     top[y] = fmaxf(top[y], __shfl_xor_sync(ALL, top[y], 1));
                     top[y] = fmaxf(top[y], __shfl_xor_sync(ALL, top[y], 2)) * p.scale_log2;     // (the scale is positive)
-                    raise |= top[y] > m[x][y] + RAISE_STEP || (m[x][y] == -INFINITY && top[y] > -INFINITY);
+                    raise[y] = top[y] > m[x][y] + RAISE_STEP || (m[x][y] == -INFINITY && top[y] > -INFINITY);
                 }
-                if (__any_sync(ALL, raise)) {
+                if (__any_sync(ALL, raise[0] || raise[1])) {
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        const float up = fmaxf(m[x][y], top[y]);
+                        const float up = raise[y] ? top[y] : m[x][y];
                         // (a row without a maximum has no sums yet but what is not finite: that stays)
-                        const float f = m[x][y] == -INFINITY ? 1.f : exp2_fast(m[x][y] - up);
+                        const float f = m[x][y] == -INFINITY || !raise[y] ? 1.f : exp2_fast(m[x][y] - up);
                         l[x][y] *= f;
 #pragma unroll
                         for (int n = 0; n < HD / 8; ++n) { o[x][n][2 * y] *= f; o[x][n][2 * y + 1] *= f; }

@@ -1030,6 +1030,13 @@ def shared_attention_library(head_dim: int):
     return lib
 
 
+#: row heads of a group from which its shared keys go to the tcgen05 kernel whatever their number, and the number from which they do with more than 16
+#: row heads.  us a call, mma.sync / tcgen05, 32 heads on 8 of 128, requests of one row with 64 keys of their own, behind 512, 2048, 8192 shared
+#: ones: 2 requests (8 row heads) 9.6 / 13.2, 11.7 / 17.3, 20.0 / 21.8; 16 (64) 11.0 / 14.0, 17.8 / 21.6, 32.5 / 26.6; 64 (256) 27.6 / 24.7,
+#: 52.2 / 28.6, 105.6 / 36.0; 12 heads on 3, 16 requests behind 2048 and 4096 14.9 / 16.0, 18.9 / 16.7
+SHARED_TC_HEADS, SHARED_TC_KEYS = 64, 2500
+
+
 def _split_parts(items: int, tiles: int, resident: int, start: float, join: float = 0.0, most: int = 64) -> int:
     """Parts that ``tiles`` of keys are split into, for ``items`` (row heads, kv head) of which ``resident`` are worked on at a time: the
     fewest rounds of the longest part, an item costing ``start`` tiles beside its own, a part a tenth of one to join, and more than one part
@@ -1097,7 +1104,8 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     lib = _shared_attn_libs.get(hd) or shared_attention_library(hd)
     own_tiles = max(1, -(-((width * page if max_position is None else max_position + 1) - plan.min_shared // page * page) // 64))
     # how the keys are split: found once for a plan and as long as the own keys stay within the same 64
-    tensor = code == 1 and TC_ATTENTION and 2 * pages * kvh * page < 1 << 31
+    tensor = (code == 1 and TC_ATTENTION and 2 * pages * kvh * page < 1 << 31
+              and (plan.most_heads > SHARED_TC_HEADS or (plan.most_heads > 16 and plan.max_shared > SHARED_TC_KEYS)))
     key = (hd, page, code, tensor, own_tiles)
     split = plan.splits.get(key)
     if split is None:
