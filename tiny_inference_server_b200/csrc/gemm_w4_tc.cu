@@ -138,7 +138,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
             // have landed the unpacking warps have seen.  (The warp walks together and one lane issues what a stage has in one go, so that
             // operands come from uniform registers: alone in its branch a thread takes 100 cycles a product, this way 25.) ----
             constexpr unsigned IDESC = instr_desc(TILE, NB, false);
-            constexpr int SUMS = SPAN == 128 ? 1 : 128 / SPAN / (HALVES ? 2 : 1);       // groups that a round begins: of a stage, or of a chunk
+            // (groups of 32 and 64: a chunk a round, with its two groups or its one, so that a round waits for places of its own sums only)
+            constexpr int ROUNDS = SPAN == 128 ? 1 : STAGE_CHUNKS, SUMS = HALVES ? 2 : 1;
             const unsigned long long x_desc0 = smem_desc(smem_u32(ring + STAGE_WORDS), 16, 1024);
             int stage = 0, d = 0;                           // stages and sums so far
             bool ok = true;
@@ -150,11 +151,11 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
                     if (!ok) break;
                     const bool ends = SPAN != 128 || c + n == c1 || ((2 * c) >> p.group_shift) != ((2 * (c + n)) >> p.group_shift);
 #pragma unroll
-                    for (int round = 0; round < (HALVES ? 2 : 1); ++round) {
-                        if (HALVES && round == 1 && n == 1) break;
-                        const int sums = SPAN == 64 ? n : SUMS;
+                    for (int round = 0; round < ROUNDS; ++round) {
+                        if (round == 1 && n == 1) break;
                         if (!open) {
-                            for (int q = 0; q < sums; ++q)
+#pragma unroll
+                            for (int q = 0; q < SUMS; ++q)
                                 ok = ok && __all_sync(0xffffffffu, mbar_wait(&d_empty[(d + q) & 1], (((d + q) >> 1) & 1) ^ 1, abort, p.fault, 6));
                             if (!ok) break;
                         }
@@ -163,25 +164,23 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
                             const unsigned a0 = tmem + COL_A + as * (STAGE_CHUNKS * A_COLS);
                             const unsigned long long x0 = x_desc0 + (unsigned long long)((s * BYTES) >> 4);
 #pragma unroll
-                            for (int u = HALVES ? round : 0; u < (HALVES ? round + 1 : STAGE_CHUNKS); ++u) {
+                            for (int u = SPAN == 128 ? 0 : round; u < (SPAN == 128 ? STAGE_CHUNKS : round + 1); ++u) {
                                 if (u == 1 && n == 1) break;
-                                // the place of this chunk's sum (SPAN 32: of its halves')
-                                const int at = SPAN == 64 ? d + u : d;
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) {
-                                    const unsigned dst = tmem + COL_D + ((at + (HALVES ? k / 2 : 0)) & 1) * 64;
+                                    const unsigned dst = tmem + COL_D + ((d + (HALVES ? k / 2 : 0)) & 1) * 64;
                                     const unsigned going = SPAN == 128 ? (open || u > 0 || k > 0) : (SPAN == 64 ? k > 0 : (k & 1));
                                     umma_ts(dst, a0 + u * A_COLS + k * 8, x0 + (unsigned long long)((u * NB * 128 + k * 32) >> 4), IDESC, going);
-                                    if (HALVES && (k & 1)) umma_commit(&d_full[(at + k / 2) & 1]);
+                                    if (HALVES && (k & 1)) umma_commit(&d_full[(d + k / 2) & 1]);
                                 }
-                                if (SPAN == 64) umma_commit(&d_full[at & 1]);
+                                if (SPAN == 64) umma_commit(&d_full[d & 1]);
                             }
                             if (SPAN == 128 && ends) umma_commit(&d_full[d & 1]);
-                            if (!HALVES || round == 1 || n == 1) umma_commit(&a_empty[as]);
+                            if (round == ROUNDS - 1 || n == 1) umma_commit(&a_empty[as]);
                         }
                         __syncwarp();
                         if (SPAN == 128) { open = !ends; d += ends; }
-                        else d += sums;
+                        else d += SUMS;
                     }
                 }
             }
@@ -272,21 +271,23 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d & 1], (d >> 1) & 1, abort, p.fault, 6));
                 if (!ok) break;
                 fence_after();
-                constexpr int STEP = NB % 32 == 0 ? 32 : 16;
 #pragma unroll
-                for (int b = 0; b < NB; b += STEP) {
+                for (int b = 0; b < NB; b += 32) {
+                    constexpr int STEP = 32;
                     float v[STEP];
 #pragma unroll
-                    for (int e = 0; e < STEP; e += 16) tmem_ld16(from + (d & 1) * 64 + b + e, v + e);
+                    for (int e = 0; e < STEP; e += 16)
+                        if (b + e < NB) tmem_ld16(from + (d & 1) * 64 + b + e, v + e);
                     tmem_ld_wait();
                     tmem_ld_arrived(v);
-                    if (b + STEP == NB) {
+                    if (b + STEP >= NB) {
                         fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&d_empty[d & 1]);
                     }
 #pragma unroll
-                    for (int e = 0; e < STEP; ++e) total[b + e] = fmaf(v[e], f, total[b + e]);
+                    for (int e = 0; e < STEP; ++e)
+                        if (b + e < NB) total[b + e] = fmaf(v[e], f, total[b + e]);
                 }
             }
             if (!ok) break;
