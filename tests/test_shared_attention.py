@@ -295,5 +295,7 @@ def test_refusals():
                 dict(q=torch.zeros(2, 128).half(), out=torch.zeros(2, 128).half(), plane=torch.zeros(3, 2, 2, 16, 32).half())):
         with pytest.raises(ops.KernelError):
             ops.shared_prefix_attention(**{**good, **bad})
+    with pytest.raises(ops.KernelError, match="own"):
+        ops.shared_prefix_attention(**{**good, "out": good["q"]})
     with pytest.raises(ops.KernelError, match="CUDA tensors"):
         ops.shared_prefix_attention(**good)

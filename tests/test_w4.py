@@ -5,6 +5,8 @@ What is rounded is the sums: a chunk of 64 products in 32 bits by the tensor cor
 of an addition instead of rounding it (2^-23 relative, 17 terms at a time, 4 times, and a scale): each partial result is off by at most some
 (17 + 4 + 2) 2^-23 of the sum of the absolute terms, and the sum over the chunks adds one 2^-24 of the running sum each.  So |error| <=
 (24 * 2^-23 + chunks * 2^-24) * sum |x| |w| bounds every entry, and a bfloat16 result adds half a step, 2^-8 of itself."""
+import dataclasses
+
 import pytest
 import torch
 
@@ -95,8 +97,16 @@ def test_refusals():
                    (x, torch.zeros(2, 31, dtype=torch.bfloat16)), (x, torch.zeros(32, 2, dtype=torch.bfloat16).t())):
         with pytest.raises(ops.KernelError):
             ops.gemm_w4(a, w, out)
+    square = pack_w4(*make(32, 32, 32, False), 32)
+    y = torch.zeros(2, 32, dtype=torch.bfloat16)
+    with pytest.raises(ops.KernelError, match="where the rows are"):
+        ops.gemm_w4(y, square, y)
     with pytest.raises(ops.KernelError, match="CUDA tensors"):
         ops.gemm_w4(x, w)
+    for change in (dict(words=w.words[:, :1]), dict(scales=w.scales.float()), dict(zeros=w.zeros.transpose(0, 1)), dict(n=200), dict(k=129), dict(group=32),
+                   dict(words=w.words.transpose(3, 4).contiguous().transpose(3, 4))):
+        with pytest.raises(ValueError):
+            dataclasses.replace(w, **change)
 
 
 SIZES = [(1, 1, 1, 32), (1, 64, 16, 32), (1, 1536, 2304, 128), (8, 1536, 520, 64), (5, 2005, 1001, 32), (3, 96, 33, 64), (9, 512, 160, 128),

@@ -689,8 +689,8 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
         if out.dtype is not dtype or out.shape != (n, cols):
             raise KernelError(f"gemm_w4: result {out.dtype} {tuple(out.shape)} for {n} rows of {dtype} and weights {w.k} x {cols}")
         ldo, unit = out.stride()
-        if unit != 1 and cols > 1:
-            raise KernelError("gemm_w4: a row of the result is contiguous")
+        if (unit != 1 and cols > 1) or (out.data_ptr() == a.data_ptr() and n > 0):
+            raise KernelError("gemm_w4: a row of the result is contiguous, and the result is not where the rows are")
     device = a.get_device()
     if device < 0 or out.get_device() != device or w.place != device or _current_device() != device:
         _elsewhere("gemm_w4", a, out, w.words)
@@ -1080,10 +1080,10 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     ldq, unit = q.stride()
     n_out, width_out = out.shape
     ldo, unit_out = out.stride()
-    if n < rows or n_out < rows or width < h * hd or width_out < h * hd or unit != 1 or unit_out != 1:
-        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)}, results {tuple(out.shape)} (rows contiguous) for {rows} rows of {h} "
-                          f"heads of {hd}")
-    q_at, plane_at = q.data_ptr(), plane.data_ptr()
+    q_at, plane_at, out_at = q.data_ptr(), plane.data_ptr(), out.data_ptr()
+    if n < rows or n_out < rows or width < h * hd or width_out < h * hd or unit != 1 or unit_out != 1 or q_at == out_at:
+        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)}, results {tuple(out.shape)} (rows contiguous, and not the queries' own) for "
+                          f"{rows} rows of {h} heads of {hd}")
     code = 1 if dtype is torch.bfloat16 else 0
     if (plane_at | (q_at | 2 * ldq if code else 0)) % 16 or (not code and dtype is not torch.float32):
         raise KernelError(f"shared_prefix_attention: bfloat16 or float32, not {dtype}; the cache and in bfloat16 the rows of queries start on 16 bytes")
@@ -1129,7 +1129,7 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     scratch = torch.empty(part_rows * (hd + 2), dtype=torch.float32, device=q.device)
     calls["shared_prefix_attention"] += 1
     at = scratch.data_ptr()
-    _check(lib.tis_shared_attention(_SHARED_ARGS.pack(code, q_at, ldq, out.data_ptr(), ldo, plane_at, block_table.data_ptr(), table_stride, width,
+    _check(lib.tis_shared_attention(_SHARED_ARGS.pack(code, q_at, ldq, out_at, ldo, plane_at, block_table.data_ptr(), table_stride, width,
                                                       pages, positions.data_ptr(), *split[1:], rows, h, kvh, page, at, at + 4 * part_rows * hd,
                                                       fault.data_ptr(), _stream_number(device), plan.most_heads, plan.own_heads, scale)), lib)
     return out

@@ -34,6 +34,15 @@ class W4Weights:
     group: int
 
     def __post_init__(self):
+        strips, groups = -(-self.n // STRIP), _groups(self.k, self.group)
+        want = {"words": (torch.int32, (-(-strips // TILE_STRIPS), -(-self.k // CHUNK), TILE_STRIPS, 32, 4)),
+                "scales": (torch.bfloat16, (strips, groups, 8, 2)), "zeros": (torch.uint8, (strips, groups, 8, 2))}
+        for name, (dtype, shape) in want.items():
+            x = getattr(self, name)
+            if x is None and name == "zeros":
+                continue
+            if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous() or x.device != self.words.device:
+                raise ValueError(f"{name}: {x.dtype} {tuple(x.shape)} on {x.device}; contiguous {dtype} {shape} is wanted")
         # what a launch takes, found once: the weights stay where they are
         object.__setattr__(self, "place", self.words.get_device())
         object.__setattr__(self, "pointers", (self.words.data_ptr(), self.scales.data_ptr(), 0 if self.zeros is None else self.zeros.data_ptr()))
