@@ -5,7 +5,9 @@ What is rounded is the sums: a chunk of 64 products in 32 bits by the tensor cor
 of an addition instead of rounding it (2^-23 relative, 17 terms at a time, 4 times, and a scale): each partial result is off by at most some
 (17 + 4 + 2) 2^-23 of the sum of the absolute terms, and the sum over the chunks adds one 2^-24 of the running sum each.  So |error| <=
 (24 * 2^-23 + chunks * 2^-24) * sum |x| |w| bounds every entry, and a bfloat16 result adds half a step, 2^-8 of itself."""
+import copy
 import dataclasses
+import pickle
 
 import pytest
 import torch
@@ -230,3 +232,22 @@ def test_quantized_matrix_like_the_unpacked_one():
     # (unpacked weights are rounded to float32, 2^-24 each)
     room = (24 * 2.0 ** -23 + 12 * 2.0 ** -24 + 2.0 ** -24) * (x.double().abs() @ d.abs())
     assert ((got - x.double() @ d).abs() <= room).all()
+
+
+def test_packed_weights_hold_tensors_and_sizes_only():
+    """Nothing of a place in memory: copies, and weights read from a file, have places of their own."""
+    w = pack_w4(*make(100, 40, 32, True), 32)
+    for other in (copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert set(vars(other)) == {f.name for f in dataclasses.fields(w)} == {"words", "scales", "zeros", "k", "n", "group"}
+        assert torch.equal(other.words, w.words) and other.words.data_ptr() != w.words.data_ptr()
+
+
+@pytest.mark.gpu
+def test_a_copy_of_packed_weights(kernel):
+    w = pack_w4(*make(512, 96, 64, True, device="cuda"), 64)
+    x = torch.randn(3, 512, device="cuda").bfloat16()
+    want = ops.gemm_w4(x, w)
+    other = copy.deepcopy(w)
+    for part in (w.words, w.scales, w.zeros):
+        part.zero_()
+    assert torch.equal(ops.gemm_w4(x, other), want)

@@ -692,13 +692,12 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
         if (unit != 1 and cols > 1) or (out.data_ptr() == a.data_ptr() and n > 0):
             raise KernelError("gemm_w4: a row of the result is contiguous, and the result is not where the rows are")
     device = a.get_device()
-    if device < 0 or out.get_device() != device or w.place != device or _current_device() != device:
+    if device < 0 or out.get_device() != device or w.words.get_device() != device or _current_device() != device:
         _elsewhere("gemm_w4", a, out, w.words)
     if n == 0:
         return out
     lib = _lib or library()
     calls["gemm_w4"] += 1
-    words, scales, zeros = w.pointers
     staged = n if dtype is torch.bfloat16 else 3 * n
     tensor = W4_TENSOR
     if tensor is None:
@@ -709,8 +708,9 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
         if dtype is not torch.bfloat16 or k % 8 or lda % 8 or lda < k or a.data_ptr() % 16:
             copy = torch.empty((staged, -(-k // 8) * 8), dtype=torch.bfloat16, device=a.device)
             at = copy.data_ptr()
-    _check(lib.tis_gemm_w4(_W4_ARGS.pack(1 if dtype is torch.bfloat16 else 0, a.data_ptr(), lda, words, scales, zeros, out.data_ptr(), ldo, n, k,
-                                         cols, w.group, tensor, at, fault, _stream_number(device))), lib)
+    _check(lib.tis_gemm_w4(_W4_ARGS.pack(1 if dtype is torch.bfloat16 else 0, a.data_ptr(), lda, w.words.data_ptr(), w.scales.data_ptr(),
+                                         0 if w.zeros is None else w.zeros.data_ptr(), out.data_ptr(), ldo, n, k, cols, w.group,
+                                         tensor, at, fault, _stream_number(device))), lib)
     return out
 
 

@@ -43,9 +43,6 @@ class W4Weights:
                 continue
             if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous() or x.device != self.words.device:
                 raise ValueError(f"{name}: {x.dtype} {tuple(x.shape)} on {x.device}; contiguous {dtype} {shape} is wanted")
-        # what a launch takes, found once: the weights stay where they are
-        object.__setattr__(self, "place", self.words.get_device())
-        object.__setattr__(self, "pointers", (self.words.data_ptr(), self.scales.data_ptr(), 0 if self.zeros is None else self.zeros.data_ptr()))
 
     @property
     def shape(self) -> Tuple[int, int]:
