@@ -6,6 +6,8 @@ worst in the sums, of the scores' absolute sums in the exponents; at random and 
 result are rounded, half a step of 2^-9 .. 2^-8 each: an entry is off by at most 2^-8 of the largest value that it averages (the
 probabilities' roundings, weighed by the probabilities) and 2^-8 of itself, and the sums as above (scores of bfloat16 inputs are exact
 products, so the same 32-bit bound)."""
+import copy
+
 import pytest
 import torch
 
@@ -299,3 +301,16 @@ def test_refusals():
         ops.shared_prefix_attention(**{**good, "out": good["q"]})
     with pytest.raises(ops.KernelError, match="CUDA tensors"):
         ops.shared_prefix_attention(**good)
+
+
+@pytest.mark.gpu
+def test_a_copy_of_a_plan():
+    """A plan copied after a call reads its own tiles, not those it was copied from."""
+    b = Batch([(32, [(40, 1), (50, 2)])], 4, 2, 64, 16)
+    b.check()
+    first, b.plan = b.plan, copy.deepcopy(b.plan)
+    assert all(isinstance(x, (int, tuple)) for split in first.splits.values() for x in split) and len(first.splits) == 1
+    first.own.zero_()
+    for tiles in first.shared.values():
+        tiles.zero_()
+    b.check()

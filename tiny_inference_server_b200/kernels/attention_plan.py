@@ -142,7 +142,7 @@ class SharedPrefixPlan:
         words = torch.tensor(sum(parts, []), dtype=torch.int32).to(device)
         self.own, *shared_words = words.split([len(p) for p in parts])
         self.shared = dict(zip(self.SHARED_TILES, shared_words))
-        self.device, self.place = words.device, words.get_device()
+        self.device = words.device
         self.splits: Dict[tuple, tuple] = {}                  # how the kernels split the keys (kernels.ops)
 
 

@@ -1099,7 +1099,7 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
         raise KernelError(f"shared_prefix_attention: the scores are multiplied by a positive number, not {scale}")
     device = q.get_device()
     if (device < 0 or out.get_device() != device or plane.get_device() != device or block_table.get_device() != device
-            or positions.get_device() != device or plan.place != device or fault.get_device() != device or _current_device() != device):
+            or positions.get_device() != device or plan.own.get_device() != device or fault.get_device() != device or _current_device() != device):
         _elsewhere("shared_prefix_attention", q, out, plane, block_table, positions, plan.own, fault)
     lib = _shared_attn_libs.get(hd) or shared_attention_library(hd)
     own_tiles = max(1, -(-((width * page if max_position is None else max_position + 1) - plan.min_shared // page * page) // 64))
@@ -1123,15 +1123,15 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
         own_parts = _split_parts(n_own * kvh, own_tiles, (2 if hd <= 128 else 1) * 148, 1, 8 if code else 0)
         if len(plan.splits) > 256:
             plan.splits.clear()
-        split = plan.splits[key] = ((shared_parts + own_parts) * rows * h, plan.own.data_ptr(), n_own, plan.shared[wide_rows].data_ptr(), n_wide,
-                                    wide_rows, tensor, own_parts, shared_parts)
-    part_rows = split[0]
+        split = plan.splits[key] = ((shared_parts + own_parts) * rows * h, n_own, wide_rows, (n_wide, wide_rows, tensor, own_parts, shared_parts))
+    part_rows, n_own, wide_rows, rest = split
     scratch = torch.empty(part_rows * (hd + 2), dtype=torch.float32, device=q.device)
     calls["shared_prefix_attention"] += 1
     at = scratch.data_ptr()
     _check(lib.tis_shared_attention(_SHARED_ARGS.pack(code, q_at, ldq, out_at, ldo, plane_at, block_table.data_ptr(), table_stride, width,
-                                                      pages, positions.data_ptr(), *split[1:], rows, h, kvh, page, at, at + 4 * part_rows * hd,
-                                                      fault.data_ptr(), _stream_number(device), plan.most_heads, plan.own_heads, scale)), lib)
+                                                      pages, positions.data_ptr(), plan.own.data_ptr(), n_own, plan.shared[wide_rows].data_ptr(),
+                                                      *rest, rows, h, kvh, page, at, at + 4 * part_rows * hd, fault.data_ptr(),
+                                                      _stream_number(device), plan.most_heads, plan.own_heads, scale)), lib)
     return out
 
 
