@@ -314,3 +314,31 @@ def test_a_copy_of_a_plan():
     for tiles in first.shared.values():
         tiles.zero_()
     b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("position", [1 << 20, 1 << 29, (1 << 31) - 1])
+def test_a_position_far_behind_the_table(position, dtype):
+    """Marked, and not walked to: the keys end where the tables do.  The other request's row is what it was."""
+    b = Batch([(32, [(40, 1), (50, 1)])], 4, 2, 64, 16, dtype, junk=0.0)
+    want = b.check()
+    b.positions[1] = position
+    for split in (dict(), dict(max_position=700)):                  # one own part, several
+        b.fault.zero_()
+        got = b.run(**split)
+        assert int(b.fault[0]) == 3
+        # (two results of other splits: each off by 2^-8 of itself and of the values' mean size, less than 2 here)
+        room = 1e-5 * (want[0].abs() + 1) + (0 if dtype == torch.float32 else want[0].abs() * 2.0 ** -6 + 2.0 ** -6)
+        assert bool(((got[0] - want[0]).abs() <= room).all())
+
+
+def test_tables_shorter_than_the_shared_keys():
+    plan = SharedPrefixPlan([(64, [(0, 1), (1, 1)])], 4, 2, "cpu")
+    t = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    call = dict(q=bf(2, 128), out=bf(2, 128), plane=bf(3, 2, 2, 16, 32), positions=t(2), plan=plan, fault=t(4))
+    with pytest.raises(ops.KernelError, match="64 shared keys"):
+        ops.shared_prefix_attention(block_table=t(2, 3), **call)
+    with pytest.raises(ops.KernelError, match="CUDA tensors"):
+        ops.shared_prefix_attention(block_table=t(2, 4), **call)

@@ -58,6 +58,13 @@ __device__ __forceinline__ int position_of(const SharedParams& p, const SharedTi
     return pos >= t.prefix ? pos : -1;
 }
 
+// The end of a request's keys, for the largest position of its rows + 1: no further than its table goes (what lies behind is marked, not walked).
+__device__ __forceinline__ int end_of_keys(const SharedParams& p, int last, bool mark) {
+    const long long there = min((long long)p.table_width * p.page, 1ll << 30);
+    if (last > there && mark) atomicExch(p.fault, 3);
+    return (int)min((long long)last, there);
+}
+
 // Chunk c of the cache row of a position (common.cuh: cache_chunk), the position's part worked out once.
 struct RowChunks {
     int base;
@@ -178,10 +185,10 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
 #pragma unroll
             for (int i = 0; i < (ROWS + 31) / 32; ++i) {
                 pos[i] = lane + i * 32 < ROWS ? position_of(p, t, lane + i * 32) : -1;
-                if (pos[i] >= 0) { least = min(least, pos[i]); if (OWN) last = max(last, pos[i] + 1); }
+                if (pos[i] >= 0) { least = min(least, pos[i]); if (OWN) last = max(last, min(pos[i], 1 << 30) + 1); }
             }
             least = __reduce_min_sync(ALL, least);
-            last = __reduce_max_sync(ALL, last);
+            last = end_of_keys(p, __reduce_max_sync(ALL, last), lane == 0);
             bool all = true;
 #pragma unroll
             for (int i = 0; i < (ROWS + 31) / 32; ++i) all = all && (pos[i] >= 0 || lane + i * 32 >= t.count);
@@ -554,7 +561,8 @@ shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
     const int shared = shared_keys(p, t);
     int last = shared;
     if (OWN)
-        for (int i = 0; i < t.count; ++i) last = max(last, row_pos[i] + 1);
+        for (int i = 0; i < t.count; ++i) last = max(last, min(row_pos[i], 1 << 30) + 1);
+    last = end_of_keys(p, last, threadIdx.x == 0);
     const Range keys = part_range(OWN ? shared : 0, last, OWN ? shared & ~63 : 0, part, parts, 64);
     const size_t v_step = (size_t)p.KVH * p.page * HD;
     const int group = lane / F32_GROUP, quad = lane % F32_GROUP;
@@ -563,7 +571,7 @@ shared_f32_kernel(const SharedParams p, const SharedTile* tiles, int parts, int 
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             pos[r] = i0 + r < t.count ? row_pos[i0 + r] : -1;
-            if (pos[r] >= 0) { least = min(least, pos[r]); most = max(most, pos[r]); }
+            if (pos[r] >= 0) { least = min(least, pos[r]); most = max(most, min(pos[r], 1 << 30)); }
         }
         for (int i = threadIdx.x; i < R * HD; i += MMA_THREADS) {
             const int rh = t.rh0 + min(i0 + i / HD, t.count - 1);

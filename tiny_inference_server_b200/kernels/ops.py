@@ -1091,9 +1091,10 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     table_stride, unit = block_table.stride()
     i32 = torch.int32
     if (positions.dtype is not i32 or block_table.dtype is not i32 or fault.dtype is not i32 or positions.numel() < rows or fault.numel() < 1
-            or unit != 1 or slots <= plan.max_slot or width < 1 or not positions.is_contiguous()):
+            or unit != 1 or slots <= plan.max_slot or width < max(1, plan.max_shared // page) or not positions.is_contiguous()):
         raise KernelError(f"shared_prefix_attention: positions {positions.dtype} {tuple(positions.shape)} for {rows} rows, tables "
-                          f"{block_table.dtype} {tuple(block_table.shape)} for slots up to {plan.max_slot}, fault {fault.dtype}: int32, contiguous")
+                          f"{block_table.dtype} {tuple(block_table.shape)} for slots up to {plan.max_slot} and {plan.max_shared} shared keys, "
+                          f"fault {fault.dtype}: int32, contiguous")
     scale = hd ** -0.5 if scale is None else float(scale)
     if not 0 < scale < math.inf:
         raise KernelError(f"shared_prefix_attention: the scores are multiplied by a positive number, not {scale}")
