@@ -342,3 +342,12 @@ def test_tables_shorter_than_the_shared_keys():
         ops.shared_prefix_attention(block_table=t(2, 3), **call)
     with pytest.raises(ops.KernelError, match="CUDA tensors"):
         ops.shared_prefix_attention(block_table=t(2, 4), **call)
+
+
+def test_rows_of_the_result_on_one_another():
+    plan = SharedPrefixPlan([(16, [(0, 1), (1, 1)])], 4, 2, "cpu")
+    t = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    with pytest.raises(ops.KernelError, match="on one another"):
+        ops.shared_prefix_attention(q=bf(2, 128), out=bf(1, 128).expand(2, 128), plane=bf(3, 2, 2, 16, 32), block_table=t(2, 2), positions=t(2), plan=plan,
+                                    fault=t(4))

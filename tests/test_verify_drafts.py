@@ -225,3 +225,24 @@ def test_refusals():
             ops.verify_drafts(**{**good, **bad})
     with pytest.raises(ops.KernelError, match="CUDA tensors"):
         ops.verify_drafts(**good)
+
+
+def test_tokens_in_the_place_of_an_argument():
+    p, q, drafts, u = make(3, 2, 10, 0)
+    room = torch.zeros(20, dtype=torch.int32)
+    room[:6] = drafts.reshape(-1)
+    for bad in (dict(drafts=room[:6].view(3, 2), tokens=room[:9].view(3, 3)), dict(tokens=u.view(torch.int32)),
+                dict(tokens=room[:9].view(3, 3), accepted=room[:3])):
+        with pytest.raises(ops.KernelError, match="do not lie where"):
+            ops.verify_drafts(**{**dict(target_probs=p, draft_probs=q, drafts=drafts, uniforms=u), **bad})
+
+
+@pytest.mark.gpu
+def test_kept_drafts_in_the_place_of_their_lengths():
+    """A request's length is read before its result is written."""
+    p, q, drafts, u = (t.cuda() for t in make(40, 3, 5000, 3))
+    lens = (torch.arange(40, dtype=torch.int32) % 4).cuda()
+    tokens, kept = ops.verify_drafts(p, q, drafts, u, lens)
+    there = lens.clone()
+    again, place = ops.verify_drafts(p, q, drafts, u, there, accepted=there)
+    assert place.data_ptr() == there.data_ptr() and torch.equal(again, tokens) and torch.equal(there, kept)

@@ -251,3 +251,11 @@ def test_a_copy_of_packed_weights(kernel):
     for part in (w.words, w.scales, w.zeros):
         part.zero_()
     assert torch.equal(ops.gemm_w4(x, other), want)
+
+
+def test_rows_of_the_result_on_one_another():
+    w = pack_w4(*make(64, 32, 32, False), 32)
+    x = torch.zeros(3, 64, dtype=torch.bfloat16)
+    for out in (torch.zeros(1, 32, dtype=torch.bfloat16).expand(3, 32), torch.zeros(200, dtype=torch.bfloat16).as_strided((3, 32), (16, 1))):
+        with pytest.raises(ops.KernelError, match="on one another"):
+            ops.gemm_w4(x, w, out)

@@ -689,8 +689,8 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
         if out.dtype is not dtype or out.shape != (n, cols):
             raise KernelError(f"gemm_w4: result {out.dtype} {tuple(out.shape)} for {n} rows of {dtype} and weights {w.k} x {cols}")
         ldo, unit = out.stride()
-        if (unit != 1 and cols > 1) or (out.data_ptr() == a.data_ptr() and n > 0):
-            raise KernelError("gemm_w4: a row of the result is contiguous, and the result is not where the rows are")
+        if (unit != 1 and cols > 1) or (ldo < cols and n > 1) or (out.data_ptr() == a.data_ptr() and n > 0):
+            raise KernelError("gemm_w4: a row of the result is contiguous, its rows do not lie on one another, and the result is not where the rows are")
     device = a.get_device()
     if device < 0 or out.get_device() != device or w.words.get_device() != device or _current_device() != device:
         _elsewhere("gemm_w4", a, out, w.words)
@@ -1081,8 +1081,8 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     n_out, width_out = out.shape
     ldo, unit_out = out.stride()
     q_at, plane_at, out_at = q.data_ptr(), plane.data_ptr(), out.data_ptr()
-    if n < rows or n_out < rows or width < h * hd or width_out < h * hd or unit != 1 or unit_out != 1 or q_at == out_at:
-        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)}, results {tuple(out.shape)} (rows contiguous, and not the queries' own) for "
+    if n < rows or n_out < rows or width < h * hd or width_out < h * hd or unit != 1 or unit_out != 1 or q_at == out_at or (ldo < h * hd and rows > 1):
+        raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)}, results {tuple(out.shape)} (rows contiguous, not on one another, and not the queries' own) for "
                           f"{rows} rows of {h} heads of {hd}")
     code = 1 if dtype is torch.bfloat16 else 0
     if (plane_at | (q_at | 2 * ldq if code else 0)) % 16 or (not code and dtype is not torch.float32):
@@ -2101,6 +2101,9 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
         raise KernelError(f"verify_drafts: results {tuple(tokens.shape)} {tokens.dtype}, {tuple(accepted.shape)} {accepted.dtype}")
     if not (drafts.is_contiguous() and uniforms.is_contiguous() and tokens.is_contiguous() and accepted.is_contiguous()):
         raise KernelError("verify_drafts: drafts, numbers and results are contiguous")
+    drafts_at, uniforms_at, tokens_at = drafts.data_ptr(), uniforms.data_ptr(), tokens.data_ptr()
+    if n > 0 and (tokens_at == uniforms_at or tokens_at == drafts_at or tokens_at == accepted.data_ptr()):
+        raise KernelError("verify_drafts: the tokens do not lie where drafts, numbers or the numbers of kept drafts do")
     lens = 0
     if draft_lens is not None:
         if draft_lens.dtype is not i32 or draft_lens.shape != (n,) or not draft_lens.is_contiguous():
@@ -2114,8 +2117,8 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
         return tokens, accepted
     lib = _lib or library()
     calls["verify_drafts"] += 1
-    _check(lib.tis_verify_drafts(_VERIFY_ARGS.pack(target_probs.data_ptr(), p_request, p_row, q, q_request, q_row, drafts.data_ptr(),
-                                                   uniforms.data_ptr(), lens, tokens.data_ptr(), accepted.data_ptr(), n, k, v,
+    _check(lib.tis_verify_drafts(_VERIFY_ARGS.pack(target_probs.data_ptr(), p_request, p_row, q, q_request, q_row, drafts_at,
+                                                   uniforms_at, lens, tokens_at, accepted.data_ptr(), n, k, v,
                                                    _stream_number(device))), lib)
     return tokens, accepted
 
