@@ -7,6 +7,9 @@
 // conflicts for ldmatrix).  Four warps: with at most 16 row heads each takes a quarter of every tile's keys and they merge at the end; shared
 // tiles of up to 64 or 128 row heads give each warp 16 or 32 of them and all keys, so that an operand of keys or values read from shared
 // memory serves 32.
+// Measured, both kernels and where there is one the join: 2 requests behind 128 keys, 12 heads on 3 of 128, 8.4 us (the chain); 16 behind 4096 with up to
+// 512 own keys 16.7 us; in float32 4 behind 1000, heads of 64, 12.6 us.  Own keys of 64 requests, up to 1024 each, 8 kv heads of 128 (201 MB):
+// 40 us, 5 TB/s.
 #include "tc_common.cuh"
 #include "shared_attention.cuh"
 

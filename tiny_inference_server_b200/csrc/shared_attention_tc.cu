@@ -10,6 +10,8 @@
 // sums in 32 bits for the join instead of a result.
 // Bound, with 128 row heads a tile, by the exponentials and hand-overs of a tile (about 1800 cycles for 128 x 128 scores, the products 1050);
 // with few row heads by the bytes.
+// Measured: 64 rows of 32 heads on 8 of 128 behind 32768 keys (34 GFLOP) some 42 us, 0.8 PFLOP/s, and with the requests' own keys beside it 96 us;
+// the same on mma.sync 326 us.
 // All hand-offs are mbarriers with bounded waits; a wait that runs out sets the fault word and every role leaves; tensor memory is
 // freed on every path.
 #include "tc_common.cuh"

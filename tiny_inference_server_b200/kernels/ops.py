@@ -674,7 +674,7 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
 
     For few rows: the weights are streamed once for up to 64 rows of bfloat16 and 21 of float32, and again for as many more.  (A prompt's rows
     are better off with ``weights.w4.unpack_w4`` and ``gemm``.)  Two kernels, chosen by rows and K (``W4_MMA_ROWS``); float32 rows, and
-    bfloat16 ones that do not start on 16 bytes, are copied for the second."""
+    bfloat16 ones that do not start on 16 bytes, are copied for the second.  A wait that runs out inside the second sets ``tc_fault``."""
     dtype = a.dtype
     if (dtype is not torch.bfloat16 and dtype is not torch.float32) or a.ndim != 2:
         raise KernelError(f"gemm_w4: rows {dtype} {tuple(a.shape)}; bfloat16 or float32 are taken")
