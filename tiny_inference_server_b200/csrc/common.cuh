@@ -225,14 +225,18 @@ inline cudaError_t tis_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 
-// Whether a launcher sees the current device for the first time (a kernel's attributes are set on each device).
+// What a launcher sets once on each device (a kernel's attributes).  A device counts as done behind the call that succeeded there, not before: a second
+// thread that comes meanwhile sets it too, and one that failed is tried again.
 struct DeviceOnce {
-    std::atomic<unsigned long long> seen{0};
-    bool first() {
+    std::atomic<unsigned long long> done{0};
+    template <typename Set> cudaError_t operator()(Set set) {
         int device = 0;
         cudaGetDevice(&device);
         const unsigned long long bit = 1ull << (device & 63);
-        return !(seen.load(std::memory_order_relaxed) & bit) && (seen.fetch_or(bit), true);
+        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        const cudaError_t status = set();
+        if (status == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return status;
     }
 };
 

@@ -277,7 +277,7 @@ template <int NT, int SP, int AHEAD, int CTAS, bool HALVES, bool ZEROS> int w4_l
     }
     const size_t smem = bytes(p.stage_chunks, p.stages > 1 ? 2 : 1);
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(w4_kernel<NT, SP, AHEAD, CTAS, HALVES, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
+    if (configured([&] { return cudaFuncSetAttribute(w4_kernel<NT, SP, AHEAD, CTAS, HALVES, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); }) != cudaSuccess)
         return tis_check_launch("gemm_w4 (shared memory)");
     if (smem > 227 * 1024) {
         tis_set_error("gemm_w4: %zu bytes of shared memory", smem);

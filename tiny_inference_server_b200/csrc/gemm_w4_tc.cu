@@ -370,7 +370,7 @@ template <int NB, int SPAN, bool F32> int launch(const CUtensorMap& map, const W
     static_assert(Ring<NB>::STAGES > A_STAGES, "the ring is ahead of the operands");
     static_assert(Ring<NB>::STAGES * Ring<NB>::BYTES >= NB * TILE * 4, "a CTA's sums fit the ring");
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(w4_tc_kernel<NB, SPAN, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    if (configured([&] { return cudaFuncSetAttribute(w4_tc_kernel<NB, SPAN, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }) != cudaSuccess)
         return tis_check_launch("gemm_w4 (shared memory)");
     const int most = 2 * sm_count();
     cudaLaunchConfig_t cfg = {};

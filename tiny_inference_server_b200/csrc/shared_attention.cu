@@ -779,7 +779,7 @@ template <bool OWN> int launch_f32(const SharedParams& p, const SharedTile* tile
     constexpr int R = 4, smem = f32_floats<R>() * 4;
     heads = heads < 16 ? heads : 16;                        // (of a tile)
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(shared_f32_kernel<OWN, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    if (configured([&] { return cudaFuncSetAttribute(shared_f32_kernel<OWN, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }) != cudaSuccess)
         return tis_check_launch("shared_prefix_attention (shared memory)");
     tis_launch(shared_f32_kernel<OWN, R>, dim3((unsigned)(count * parts * p.KVH), (unsigned)((heads + R - 1) / R)), dim3(MMA_THREADS), (size_t)smem, stream,
                p, tiles, parts, part0, beside);
@@ -791,7 +791,7 @@ template <bool OWN, int WR, int MT> int launch_mma(const SharedParams& p, const 
     const size_t smem = (size_t)STAGES * 2 * TILE_ELEMENTS * 2 + (size_t)(WR == 1 ? 2 : 1) * ROWS * HD * 2 + (WR == 1 ? 2 * 16 * HD * 4 : 0);
     const int items = count * parts * p.KVH, ctas = WR == 1 ? (HD <= 128 ? 2 : 1) * tc::sm_count() : items;
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(shared_mma_kernel<OWN, WR, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    if (configured([&] { return cudaFuncSetAttribute(shared_mma_kernel<OWN, WR, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }) != cudaSuccess)
         return tis_check_launch("shared_prefix_attention (shared memory)");
     tis_launch(shared_mma_kernel<OWN, WR, MT>, dim3((unsigned)(items < ctas ? items : ctas)), dim3(MMA_THREADS + LOAD_THREADS), smem, stream, p, tiles, items, parts, part0, beside);
     return tis_check_launch("shared_prefix_attention");

@@ -377,7 +377,7 @@ int shared_tc_launch(const SharedParams& p, const SharedTile* tiles, int count, 
     if (!tensor_map(p.plane, HD, (long long)p.num_pages * 2 * p.KVH * p.page, HD, p.page, false, &map)) return TIS_CUDA_ERROR;
     constexpr int smem = Q_BYTES + 2 * P_BYTES + 2 * SLOTS * SLOT_BYTES + 1024;
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(shared_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    if (configured([&] { return cudaFuncSetAttribute(shared_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }) != cudaSuccess)
         return tis_check_launch("shared_prefix_attention (shared memory)");
     tis_launch(shared_tc_kernel, dim3((unsigned)(count * parts * p.KVH)), dim3(NTH), (size_t)smem, stream, map, p, tiles, parts);
     return tis_check_launch("shared_prefix_attention");

@@ -286,7 +286,7 @@ verify_kernel(const VerifyParams v, int steps, int strides) {
 
 template <int N> int verify_launch(const cudaLaunchConfig_t& cfg, const VerifyParams& v, long long run) {
     static DeviceOnce configured;
-    if (configured.first() && cudaFuncSetAttribute(verify_kernel<N>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    if (configured([&] { return cudaFuncSetAttribute(verify_kernel<N>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); }) != cudaSuccess)
         return tis_check_launch("verify_drafts (cluster size)");
     const long long strides = (run + 128 * N * VERIFY_STEPS - 1) / (128 * N * VERIFY_STEPS);
     const long long steps = (run + 128 * N * strides - 1) / (128 * N * strides);
