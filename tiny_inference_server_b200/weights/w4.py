@@ -25,7 +25,8 @@ STRIP, CHUNK, TILE_STRIPS = 16, 64, 8
 @dataclass(frozen=True)
 class W4Weights:
     """Codes in the kernel's layout: ``words`` (tiles, chunks, 8, 32, 4) int32, ``scales`` (strips, groups, 8, 2) bfloat16, ``zeros``
-    the same in uint8 (None: 8 everywhere)."""
+    the same in uint8 (None: 8 everywhere).  They are read 16, 4 and 2 bytes at a time and start on such a place: parts of one buffer are cut at
+    multiples of 16 bytes."""
     words: torch.Tensor
     scales: torch.Tensor
     zeros: Optional[torch.Tensor]
@@ -35,14 +36,16 @@ class W4Weights:
 
     def __post_init__(self):
         strips, groups = -(-self.n // STRIP), _groups(self.k, self.group)
-        want = {"words": (torch.int32, (-(-strips // TILE_STRIPS), -(-self.k // CHUNK), TILE_STRIPS, 32, 4)),
-                "scales": (torch.bfloat16, (strips, groups, 8, 2)), "zeros": (torch.uint8, (strips, groups, 8, 2))}
-        for name, (dtype, shape) in want.items():
+        want = {"words": (torch.int32, (-(-strips // TILE_STRIPS), -(-self.k // CHUNK), TILE_STRIPS, 32, 4), 16),
+                "scales": (torch.bfloat16, (strips, groups, 8, 2), 4), "zeros": (torch.uint8, (strips, groups, 8, 2), 2)}
+        for name, (dtype, shape, start) in want.items():
             x = getattr(self, name)
             if x is None and name == "zeros":
                 continue
             if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous() or x.device != self.words.device:
                 raise ValueError(f"{name}: {x.dtype} {tuple(x.shape)} on {x.device}; contiguous {dtype} {shape} is wanted")
+            if x.device.type != "meta" and x.data_ptr() % start:
+                raise ValueError(f"{name}: starts on a multiple of {start} bytes, not at {x.data_ptr() % start} behind one")
 
     @property
     def shape(self) -> Tuple[int, int]:
