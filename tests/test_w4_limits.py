@@ -35,3 +35,36 @@ def test_packed_weights_in_one_buffer(kernel):  # noqa: F811
     other = dataclasses.replace(w, words=behind(w.words, 16), scales=behind(w.scales, 4), zeros=behind(w.zeros, 2))
     x = torch.randn(5, 300, device="cuda").bfloat16()
     assert torch.equal(ops.gemm_w4(x, other), ops.gemm_w4(x, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("exponent", [-100, -110, -118, -125, -130, -140])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows", [1, 3, 8])
+def test_very_small_float32_rows_keep_their_bits(exponent, zeros, rows, kernel):  # noqa: F811
+    """Entries whose last bits lie far below bfloat16's smallest number, and entries below float32's smallest normal one.  Room: that of test_w4.py, and what
+    is rounded to steps of 2^-149, by half of one each: a group's scaled sum of the high parts (8 groups), the same of the two lower parts (2^-8 of it) and
+    their two joins."""
+    g = torch.Generator().manual_seed(rows)
+    codes, scales, z = make(256, 70, 32, zeros, 7, "cuda")
+    x = (torch.randn(rows, 256, generator=g, dtype=torch.float64) * 2.0 ** exponent).float().cuda()
+    d = dense(codes, scales, z, 32)
+    want, size = x.double() @ d, x.double().abs() @ d.abs()
+    got = ops.gemm_w4(x, pack_w4(codes, scales, z, 32)).double()
+    room = (24 * 2.0 ** -23 + 4 * 2.0 ** -24) * size + (8 + 2 * 8 * 2.0 ** -8 + 2) * 2.0 ** -150
+    assert ((got - want).abs() <= room).all(), ((got - want).abs() / size).max().item()
+
+
+@pytest.mark.gpu
+def test_float32_rows_up_to_the_largest(kernel):  # noqa: F811
+    """Every bit of numbers of any size counts, the largest float32 number's too."""
+    codes, scales, _ = make(64, 16, 64, False, 6, "cuda")
+    codes.fill_(8)
+    codes[:5] = 9
+    scales.fill_(1.0)
+    w = pack_w4(codes, scales, None, 64)
+    x = torch.zeros(5, 64, device="cuda")
+    for i, v in enumerate((torch.finfo(torch.float32).max, 1 + 2.0 ** -23, 2.0 ** -126 * (1 + 2.0 ** -23), 2.0 ** -149, 2.0 ** -127 + 2.0 ** -149)):
+        x[i, i] = v
+    got = ops.gemm_w4(x, w)
+    assert torch.equal(got, x.sum(1, keepdim=True).expand_as(got))

@@ -8,7 +8,9 @@
 // multiplied by its scale once, in 32 bits: weights are never rounded.
 //
 // x in float32 goes through the same products as three bfloat16 numbers each, cut off and not rounded: 8 + 8 + 8 bits hold all 24
-// of a float, so nothing is lost there either.
+// of a float, and the lower ones are scaled (`three`) so that those of the smallest floats are held too: nothing is lost there either.
+// A group's sum of whole numbers is formed before its scale, in 32 bits: 15 times the sum of a group's |x|, in float32 twice that, has to stay below
+// 2^128, or a result comes out as infinite that with the scale would not be.
 //
 // A CTA of eight warps takes a few strips of 16 columns; its warps share them out (`ws` of them side by side) and the chunks of
 // 64 entries of the sum (`wk` of them take turns), and add up in shared memory, in a fixed order.  x waits in shared memory, whole or in
@@ -230,7 +232,7 @@ w4_kernel(const W4Params p) {
                 advance();
             }
         }
-        // ---- the warps' turns added up, float32's three parts too (the small ones first), and stored.  Two tiles' sums lie side by
+        // ---- the warps' turns added up, float32's three parts too, and stored.  Two tiles' sums lie side by
         // side: a warp may be a tile ahead of the slowest, not two ----
         float* here = part + flip * part_floats;
 #pragma unroll
@@ -245,12 +247,13 @@ w4_kernel(const W4Params p) {
         for (int i = threadIdx.x; i < rows * cols; i += W4_THREADS) {
             const int r = i / cols, c = i - r * cols;
             if (first + c >= p.N) continue;
-            float v = 0.f;
-            for (int q = p.f32 ? 2 : 0; q >= 0; --q)
-                for (int w = 0; w < p.wk; ++w) v += here[((size_t)w * NT * 8 + q * rows + r) * pitch + c];
+            float v[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+                for (int w = 0; w < (q == 0 || p.f32 ? p.wk : 0); ++w) v[q] += here[((size_t)w * NT * 8 + q * rows + r) * pitch + c];
             const long long at = (long long)(row0 + r) * p.ldo + first + c;
-            if (p.f32) static_cast<float*>(p.out)[at] = v;
-            else static_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(v);
+            if (p.f32) static_cast<float*>(p.out)[at] = of_three(v[0], v[1], v[2]);
+            else static_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(v[0]);
         }
     }
 }

@@ -299,8 +299,8 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
                 if (n < p.N) {
                     if (F32) {
 #pragma unroll
-                        for (int r = 0; r < NB / 3; ++r)    // the small parts first
-                            if (r < p.rows) static_cast<float*>(p.out)[r * p.ldo + n] = (total[3 * r + 2] + total[3 * r + 1]) + total[3 * r];
+                        for (int r = 0; r < NB / 3; ++r)
+                            if (r < p.rows) static_cast<float*>(p.out)[r * p.ldo + n] = of_three(total[3 * r], total[3 * r + 1], total[3 * r + 2]);
                     } else {
 #pragma unroll
                         for (int r = 0; r < NB; ++r)
@@ -337,7 +337,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
 #pragma unroll
                 for (int e = 0; e < (F32 ? 3 : 1); ++e) v[e] += load_rank(part + ((F32 ? 3 : 1) * r + e) * TILE + (threadIdx.x & 127), q);
             if (n < p.N) {
-                if (F32) static_cast<float*>(p.out)[r * p.ldo + n] = (v[2] + v[1]) + v[0];
+                if (F32) static_cast<float*>(p.out)[r * p.ldo + n] = of_three(v[0], v[1], v[2]);
                 else static_cast<bf16*>(p.out)[r * p.ldo + n] = __float2bfloat16_rn(v[0]);
             }
         }
@@ -346,7 +346,7 @@ w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const W4TcParams p) {
     }
 }
 
-// x's rows as the products take them: bfloat16 in rows that start on 16 bytes; a row of float32 is three, its high, middle and low parts.
+// x's rows as the products take them: bfloat16 in rows that start on 16 bytes; a row of float32 is three (`three`).
 template <typename T>
 __global__ void __launch_bounds__(256) w4_copy_kernel(const T* x, long long ldx, bf16* to, long long ldt, int rows, int K) {
     pdl_launch_dependents();

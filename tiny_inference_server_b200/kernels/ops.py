@@ -670,7 +670,8 @@ W4_TENSOR: Optional[bool] = None
 
 def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a (n, K) @ w (K, N)`` for weights of four bits (``weights.w4.pack_w4``), a and the result in bfloat16 or float32; row strides
-    free.  Every weight is taken as it is, (code - zero) * scale, and a sum is rounded once, when it is stored.
+    free.  Every weight is taken as it is, (code - zero) * scale, and a sum is rounded once, when it is stored.  A group's sums are formed before their
+    scale: 15 times the sum of a group's ``|a|``, in float32 twice that, has to stay below 2^128.
 
     For few rows: the weights are streamed once for up to 64 rows of bfloat16 and 21 of float32, and again for as many more.  (A prompt's rows
     are better off with ``weights.w4.unpack_w4`` and ``gemm``.)  Two kernels, chosen by rows and K (``W4_MMA_ROWS``); float32 rows, and
