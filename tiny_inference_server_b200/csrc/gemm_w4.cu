@@ -258,27 +258,32 @@ w4_kernel(const W4Params p) {
     }
 }
 
+// Shared memory of a CTA: `eights` of staged rows, strips of a warp, warps side by side and in turns, chunks of a stage; and what two CTAs of an SM have.
+constexpr size_t W4_SMEM = 224 * 1024 / 2;
+constexpr size_t w4_bytes(int eights, int sp, int ws, int wk, int stage_chunks, int buffers) {
+    return (size_t)eights * 8 * ((size_t)stage_chunks * W4_CHUNK + W4_PAD) * 2 * buffers + (size_t)2 * wk * eights * 8 * (ws * sp * W4_STRIP + 1) * 4;
+}
+// Strips of a warp: two where that leaves all CTAs some, and the registers take it.
+constexpr int w4_side(int eights, int strips) { return eights == 2 || (eights == 1 && strips > 2 * 148) ? 2 : 1; }
+// Chunks of x in one piece: every warp has as many turns.
+constexpr int w4_whole(int chunks) { return (chunks + W4_WARPS - 1) / W4_WARPS * W4_WARPS; }
+constexpr bool w4_one_piece(int eights, int sp, int chunks) { return w4_bytes(eights, sp, 1, W4_WARPS, w4_whole(chunks), 1) <= W4_SMEM; }
 
 template <int NT, int SP, int AHEAD, int CTAS, bool HALVES, bool ZEROS> int w4_launch(W4Params p, int slabs, cudaStream_t stream) {
-    auto bytes = [&](int stage_chunks, int buffers) {
-        const size_t count = (size_t)stage_chunks * W4_CHUNK;
-        const size_t staged = (size_t)NT * 8 * (count + W4_PAD) * 2 * buffers;
-        return staged + (size_t)2 * p.wk * NT * 8 * (p.ws * SP * W4_STRIP + 1) * 4;
-    };
     // x in one stage where it fits: all warps share out the sum.  Else four of them stand side by side, for fewer passes over x.
     p.ws = 1;
     p.wk = W4_WARPS;
     p.stages = 1;
-    p.stage_chunks = (p.chunks + p.wk - 1) / p.wk * p.wk;
-    if (bytes(p.stage_chunks, 1) > (224 * 1024 / CTAS)) {
+    p.stage_chunks = w4_whole(p.chunks);
+    if (!w4_one_piece(NT, SP, p.chunks)) {
         p.ws = 4;
         p.wk = W4_WARPS / p.ws;
         const int unit = p.wk * AHEAD;
         p.stage_chunks = unit;
-        while (bytes(p.stage_chunks + unit, 2) <= (224 * 1024 / CTAS)) p.stage_chunks += unit;
+        while (w4_bytes(NT, SP, p.ws, p.wk, p.stage_chunks + unit, 2) <= W4_SMEM) p.stage_chunks += unit;
         p.stages = (p.chunks + p.stage_chunks - 1) / p.stage_chunks;
     }
-    const size_t smem = bytes(p.stage_chunks, p.stages > 1 ? 2 : 1);
+    const size_t smem = w4_bytes(NT, SP, p.ws, p.wk, p.stage_chunks, p.stages > 1 ? 2 : 1);
     static DeviceOnce configured;
     if (configured([&] { return cudaFuncSetAttribute(w4_kernel<NT, SP, AHEAD, CTAS, HALVES, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); }) != cudaSuccess)
         return tis_check_launch("gemm_w4 (shared memory)");
@@ -300,6 +305,12 @@ template <int NT, int SP, int AHEAD, int CTAS> int w4_forms(const W4Params& p, i
 }
 
 }  // namespace
+
+// Whether the mma.sync kernel holds `staged` rows of x (a row of float32 is three) in one piece, for the choice between the two.
+TIS_API int tis_gemm_w4_one_piece(int staged, int K, int N) {
+    const int eights = (staged + 7) / 8, strips = (N + W4_STRIP - 1) / W4_STRIP;
+    return w4_one_piece(eights, w4_side(eights, strips), (K + W4_CHUNK - 1) / W4_CHUNK);
+}
 
 // out (rows, N) = x (rows, K) times the packed weights; dtype is that of x and out, rows of both contiguous, row strides free.
 struct W4Args { long long dtype, x, ldx, words, scales, zeros, out, ldo, rows, K, N, group, tensor, copy, fault, stream; };
@@ -347,8 +358,7 @@ TIS_API int tis_gemm_w4(const W4Args* a) {
     p.slab = (rows + slabs - 1) / slabs;
     const int eights = ((p.f32 ? 3 : 1) * p.slab + 7) / 8;
     switch (eights) {
-        case 1:
-            return p.strips <= 2 * 148 ? w4_forms<1, 1, 4, 2>(p, slabs, stream) : w4_forms<1, 2, 4, 2>(p, slabs, stream);
+        case 1: return w4_side(1, p.strips) == 1 ? w4_forms<1, 1, 4, 2>(p, slabs, stream) : w4_forms<1, 2, 4, 2>(p, slabs, stream);
         case 2: return w4_forms<2, 2, 2, 2>(p, slabs, stream);
         case 3: return w4_forms<3, 1, 4, 2>(p, slabs, stream);
         case 4: return w4_forms<4, 1, 4, 2>(p, slabs, stream);

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import collections
 import ctypes
+import functools
 import math
 import os
 import struct
@@ -659,13 +660,30 @@ def gemm_f32_out(a: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
 # row-wise kernels
 # ---------------------------------------------------------------------------------------
 
-#: gemm_w4: most staged rows (a row of float32 is three) of the mma.sync kernel, and the bytes of x up to which it holds it in one piece; beyond
-#: either the tcgen05 kernel takes the product.  us, mma.sync / tcgen05, groups of 128: 1536 x 2304 at 1, 8, 16, 24, 32 rows 2.4 / 5.0, 3.2 / 5.2,
-#: 4.9 / 5.5, 6.1 / 6.1, 11.4 / 6.2; 4096 x 4096 at 8 and 9 rows (x in one piece, in several) 7.9 / 9.1, 26.5 / 9.2; 4096 x 28672 at 8, 9, 32
-#: 26.3 / 36.9, 36.2 / 36.9, 79.5 / 40.9; 8192 x 1024 at 1 row (several pieces) 22.5 / 8.2
-W4_MMA_ROWS, W4_MMA_BYTES = 24, 108 * 1024
-#: for tests and measurements: False or True sends all of them to the one or the other
+#: gemm_w4: most staged rows (a row of float32 is three) of the mma.sync kernel
+W4_MMA_ROWS = 24
+#: for tests and measurements: True sends all products to the tcgen05 kernel, False all that it takes to the mma.sync one
 W4_TENSOR: Optional[bool] = None
+
+
+@functools.lru_cache(maxsize=1 << 14)
+def _w4_tensor(staged: int, k: int, n: int, group: int) -> bool:
+    """Whether a product goes to the tcgen05 kernel: by the staged rows, by whether the mma.sync kernel holds x in one piece (its launcher says so; K up to
+    6144, of many columns 5632, with up to 8 staged rows, 2048 with 16, 1536 with 24), and by the tiles of 128 columns.  The tcgen05 kernel shares a sum out
+    over more CTAs up to 148 tiles and takes two turns behind 296; its time goes up with groups of less than 128.  x in several pieces leaves the mma.sync kernel
+    fewer CTAs than SMs up to 148 tiles.  us, mma.sync / tcgen05, groups of 128 (a further pair: of 32):
+
+    one piece       K 1536 by 2304, 12288, 16384, 49152 columns, 24 rows 6.3 / 5.8, 12.0 / 11.4, 14.8 / 11.6 (15.9 / 15.1), 35.5 / 22.7 (38.7 / 42.6); 16 rows 4.7 / 5.3,
+                    10.1 / 10.4, 10.7 / 10.6, 23.8 / 21.3 (26.4 / 41.3); 8 rows 3.4 / 5.0, 7.7 / 10.4, 7.7 / 10.5, 18.2 / 21.0
+    several pieces  24 rows, K 2048 by 2304, 8192, 28672 11.8 / 7.1, 16.1 / 9.4, 35.6 / 21.1 (36.8 / 32.7); 16 rows, K 2560 by 4096, 16384, 20480, 28672, 49152
+                    19.0 / 6.6, 25.6 / 14.7, 26.7 / 23.6 (29.8 / 36.0; of 64: 26.6 / 26.1), 27.0 / 24.0 (30.0 / 38.9), 51.5 / 33.1 (57.3 / 65.7); 8 rows, K 6144 by
+                    8192, 16384, 20480, 28672, 49152 40.9 / 16.4, 45.1 / 28.9 (53.8 / 46.4), 45.9 / 51.9, 46.2 / 52.2, 89.4 / 73.7 (of 64: 90.6 / 85.1; of 32: 113 / 147)"""
+    if staged > W4_MMA_ROWS:
+        return True
+    tiles = -(-n // 128)
+    if (_lib or library()).tis_gemm_w4_one_piece(staged, k, n):
+        return (staged > 16 and tiles > 96 and group >= 64) or (staged > 8 and tiles > 296 and group >= 128)
+    return staged > 16 or tiles <= 148 or group >= (64 if tiles > 296 else 128 if staged > 8 else math.inf)
 
 
 def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -674,7 +692,7 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
     scale: 15 times the sum of a group's ``|a|``, in float32 twice that, has to stay below 2^128.
 
     For few rows: the weights are streamed once for up to 64 rows of bfloat16 and 21 of float32, and again for as many more.  (A prompt's rows
-    are better off with ``weights.w4.unpack_w4`` and ``gemm``.)  Two kernels, chosen by rows and K (``W4_MMA_ROWS``); float32 rows, and
+    are better off with ``weights.w4.unpack_w4`` and ``gemm``.)  Two kernels, chosen by the sizes (``_w4_tensor``); float32 rows, and
     bfloat16 ones that do not start on 16 bytes, are copied for the second.  A wait that runs out inside the second sets ``tc_fault``."""
     dtype = a.dtype
     if (dtype is not torch.bfloat16 and dtype is not torch.float32) or a.ndim != 2:
@@ -700,9 +718,7 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
     lib = _lib or library()
     calls["gemm_w4"] += 1
     staged = n if dtype is torch.bfloat16 else 3 * n
-    tensor = W4_TENSOR
-    if tensor is None:
-        tensor = staged > W4_MMA_ROWS or -(-staged // 8) * 16 * (k + 64) > W4_MMA_BYTES
+    tensor = _w4_tensor(staged, k, cols, w.group) if W4_TENSOR is None else W4_TENSOR
     copy = at = fault = 0
     if tensor:
         fault = tc_fault().data_ptr()
