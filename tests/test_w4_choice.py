@@ -58,3 +58,11 @@ def test_between_the_sizes_that_fit(staged, k, n, library):
 @pytest.mark.parametrize("staged,k,n", [(1, 1536, 2304), (8, 4096, 28672), (8, 4096, 4096), (9, 2005, 5501), (16, 2048, 2304), (24, 1536, 2304)])
 def test_sizes_that_fit(staged, k, n, library):
     assert not any(ops._w4_tensor(staged, k, n, group) for group in (32, 64, 128))
+
+
+@pytest.mark.parametrize("dtype,rows", [(1, 25), (0, 9), (1, 64)])
+def test_the_mma_launcher_refuses_more_rows_than_it_is_built_for(dtype, rows, library):
+    library.tis_last_error.restype = ctypes.c_char_p
+    library.tis_gemm_w4.argtypes = [ctypes.c_char_p]
+    assert library.tis_gemm_w4(ops._W4_ARGS.pack(dtype, 0, 64, 0, 0, 0, 0, 64, rows, 64, 64, 32, 0, 0, 0, 0)) != 0
+    assert b"rows" in library.tis_last_error()

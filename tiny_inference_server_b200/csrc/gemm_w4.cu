@@ -25,8 +25,7 @@ namespace {
 
 constexpr int W4_THREADS = 256, W4_WARPS = 8;
 constexpr int W4_PAD = 16;                  // elements behind a staged row
-constexpr int W4_ROWS = 64;                 // rows of a slab in bfloat16
-constexpr int W4_ROWS_F32 = 21;             // and in float32, three numbers each
+constexpr int W4_STAGED = 24;                // most staged rows: those of bfloat16, three of each of float32
 
 __device__ __forceinline__ uint4 load_stream(const uint4* p) {
     uint4 v;
@@ -41,15 +40,15 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const unsigned (&a)[4], 
 __device__ __forceinline__ float low_half(unsigned v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high_half(unsigned v) { return __uint_as_float(v & 0xffff0000u); }
 
-// Entries [k0, k0 + count) of the slab's rows of x into shared memory, zero beyond K.  In float32 the rows stand three times, the
+// Entries [k0, k0 + count) of the rows of x into shared memory, zero beyond K.  In float32 the rows stand three times, the
 // high parts, the middle ones, the low ones.
-__device__ __forceinline__ void stage_rows(const W4Params& p, bf16* to, int stride, int row0, int rows, int k0, int count) {
+__device__ __forceinline__ void stage_rows(const W4Params& p, bf16* to, int stride, int rows, int k0, int count) {
     const int pieces = count / 8;
     for (int i = threadIdx.x; i < rows * pieces; i += W4_THREADS) {
         const int r = i / pieces, k = k0 + (i - r * pieces) * 8;
         bf16* dst = to + (size_t)r * stride + (k - k0);
         if (!p.f32) {
-            const bf16* src = static_cast<const bf16*>(p.x) + (long long)(row0 + r) * p.ldx + k;
+            const bf16* src = static_cast<const bf16*>(p.x) + (long long)r * p.ldx + k;
             if (p.vectors) {
                 const int bytes = k < p.K ? 16 : 0;         // (whole pieces: K is a multiple of 8 here)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
@@ -62,7 +61,7 @@ __device__ __forceinline__ void stage_rows(const W4Params& p, bf16* to, int stri
                                                             v[4] | (unsigned)v[5] << 16, v[6] | (unsigned)v[7] << 16);
             }
         } else {
-            const float* src = static_cast<const float*>(p.x) + (long long)(row0 + r) * p.ldx + k;
+            const float* src = static_cast<const float*>(p.x) + (long long)r * p.ldx + k;
             float f[8];
             if (p.vectors && k < p.K) {
                 const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
@@ -91,7 +90,7 @@ w4_kernel(const W4Params p) {
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int side = warp % p.ws, turn = warp / p.ws;
-    const int row0 = (int)blockIdx.y * p.slab, rows = min(p.slab, p.rows - row0);
+    const int rows = p.rows;
     constexpr int GROUPS = HALVES ? 2 : 1;                  // of a chunk
     const int strips_of_tile = p.ws * SP, tiles = (p.strips + strips_of_tile - 1) / strips_of_tile;
     const int mine = turn < p.chunks ? (p.chunks - turn + p.wk - 1) / p.wk : 0;         // this warp's chunks of a tile
@@ -148,7 +147,7 @@ w4_kernel(const W4Params p) {
     float* part = reinterpret_cast<float*>(x_smem + buffers * buffer);          // [two][turn][staged row][column]
     const int part_floats = p.wk * NT * 8 * pitch;
 
-    stage_rows(p, x_smem, stride, row0, rows, 0, count);
+    stage_rows(p, x_smem, stride, rows, 0, count);
     asm volatile("cp.async.commit_group;\n" ::: "memory");
     const int per_stage = p.stage_chunks / p.wk;
     bool staged = false;                                    // (x in one stage: it stays)
@@ -169,7 +168,7 @@ w4_kernel(const W4Params p) {
                 __syncthreads();
                 if (p.stages > 1) {
                     if (stage + 1 < p.stages || tile + (int)gridDim.x < tiles)
-                        stage_rows(p, x_smem + (now ^ 1) * buffer, stride, row0, rows, (stage + 1 < p.stages ? stage + 1 : 0) * count, count);
+                        stage_rows(p, x_smem + (now ^ 1) * buffer, stride, rows, (stage + 1 < p.stages ? stage + 1 : 0) * count, count);
                     asm volatile("cp.async.commit_group;\n" ::: "memory");
                     ++stages_done;
                 }
@@ -251,7 +250,7 @@ w4_kernel(const W4Params p) {
 #pragma unroll
             for (int q = 0; q < 3; ++q)
                 for (int w = 0; w < (q == 0 || p.f32 ? p.wk : 0); ++w) v[q] += here[((size_t)w * NT * 8 + q * rows + r) * pitch + c];
-            const long long at = (long long)(row0 + r) * p.ldo + first + c;
+            const long long at = (long long)r * p.ldo + first + c;
             if (p.f32) static_cast<float*>(p.out)[at] = of_three(v[0], v[1], v[2]);
             else static_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(v[0]);
         }
@@ -269,7 +268,7 @@ constexpr int w4_side(int eights, int strips) { return eights == 2 || (eights ==
 constexpr int w4_whole(int chunks) { return (chunks + W4_WARPS - 1) / W4_WARPS * W4_WARPS; }
 constexpr bool w4_one_piece(int eights, int sp, int chunks) { return w4_bytes(eights, sp, 1, W4_WARPS, w4_whole(chunks), 1) <= W4_SMEM; }
 
-template <int NT, int SP, int AHEAD, int CTAS, bool HALVES, bool ZEROS> int w4_launch(W4Params p, int slabs, cudaStream_t stream) {
+template <int NT, int SP, int AHEAD, int CTAS, bool HALVES, bool ZEROS> int w4_launch(W4Params p, cudaStream_t stream) {
     // x in one stage where it fits: all warps share out the sum.  Else four of them stand side by side, for fewer passes over x.
     p.ws = 1;
     p.wk = W4_WARPS;
@@ -293,15 +292,15 @@ template <int NT, int SP, int AHEAD, int CTAS, bool HALVES, bool ZEROS> int w4_l
     }
     const int tiles = (p.strips + p.ws * SP - 1) / (p.ws * SP);
     const int most = CTAS * 148;
-    tis_launch(w4_kernel<NT, SP, AHEAD, CTAS, HALVES, ZEROS>, dim3((unsigned)(tiles < most ? tiles : most), (unsigned)slabs), dim3(W4_THREADS), smem, stream, p);
+    tis_launch(w4_kernel<NT, SP, AHEAD, CTAS, HALVES, ZEROS>, dim3((unsigned)(tiles < most ? tiles : most)), dim3(W4_THREADS), smem, stream, p);
     return tis_check_launch("gemm_w4");
 }
 
-template <int NT, int SP, int AHEAD, int CTAS, bool HALVES> int w4_zeros(const W4Params& p, int slabs, cudaStream_t stream) {
-    return p.zeros != nullptr ? w4_launch<NT, SP, AHEAD, CTAS, HALVES, true>(p, slabs, stream) : w4_launch<NT, SP, AHEAD, CTAS, HALVES, false>(p, slabs, stream);
+template <int NT, int SP, int AHEAD, int CTAS, bool HALVES> int w4_zeros(const W4Params& p, cudaStream_t stream) {
+    return p.zeros != nullptr ? w4_launch<NT, SP, AHEAD, CTAS, HALVES, true>(p, stream) : w4_launch<NT, SP, AHEAD, CTAS, HALVES, false>(p, stream);
 }
-template <int NT, int SP, int AHEAD, int CTAS> int w4_forms(const W4Params& p, int slabs, cudaStream_t stream) {
-    return p.group_shift == 0 ? w4_zeros<NT, SP, AHEAD, CTAS, true>(p, slabs, stream) : w4_zeros<NT, SP, AHEAD, CTAS, false>(p, slabs, stream);
+template <int NT, int SP, int AHEAD, int CTAS> int w4_forms(const W4Params& p, cudaStream_t stream) {
+    return p.group_shift == 0 ? w4_zeros<NT, SP, AHEAD, CTAS, true>(p, stream) : w4_zeros<NT, SP, AHEAD, CTAS, false>(p, stream);
 }
 
 }  // namespace
@@ -348,22 +347,14 @@ TIS_API int tis_gemm_w4(const W4Args* a) {
         }
         return w4_tc_launch(p, reinterpret_cast<void*>(a->copy), reinterpret_cast<int*>(a->fault), stream);
     }
-    // rows in slabs of about the same size
-    const int most = p.f32 ? W4_ROWS_F32 : W4_ROWS;
-    const int slabs = (rows + most - 1) / most;
-    if (slabs > 65535) {
-        tis_set_error("gemm_w4: %d rows", rows);
+    if ((p.f32 ? 3ll : 1ll) * rows > W4_STAGED) {
+        tis_set_error("gemm_w4: %d rows, of which the mma.sync kernel takes %d", rows, p.f32 ? W4_STAGED / 3 : W4_STAGED);
         return TIS_BAD_SIZE;
     }
-    p.slab = (rows + slabs - 1) / slabs;
-    const int eights = ((p.f32 ? 3 : 1) * p.slab + 7) / 8;
+    const int eights = ((p.f32 ? 3 : 1) * rows + 7) / 8;
     switch (eights) {
-        case 1: return w4_side(1, p.strips) == 1 ? w4_forms<1, 1, 4, 2>(p, slabs, stream) : w4_forms<1, 2, 4, 2>(p, slabs, stream);
-        case 2: return w4_forms<2, 2, 2, 2>(p, slabs, stream);
-        case 3: return w4_forms<3, 1, 4, 2>(p, slabs, stream);
-        case 4: return w4_forms<4, 1, 4, 2>(p, slabs, stream);
-        case 5: return w4_forms<5, 1, 2, 2>(p, slabs, stream);
-        case 6: return w4_forms<6, 1, 2, 2>(p, slabs, stream);
-        default: return w4_forms<8, 1, 2, 2>(p, slabs, stream);
+        case 1: return w4_side(1, p.strips) == 1 ? w4_forms<1, 1, 4, 2>(p, stream) : w4_forms<1, 2, 4, 2>(p, stream);
+        case 2: return w4_forms<2, 2, 2, 2>(p, stream);
+        default: return w4_forms<3, 1, 4, 2>(p, stream);
     }
 }

@@ -8,7 +8,7 @@ struct W4Params {
     const uint4* words; const unsigned* scales; const unsigned short* zeros;
     const void* x; long long ldx;
     void* out; long long ldo;
-    int rows, slab, K, N, chunks, strips, groups, group_shift;      // group_shift: log2 of the halves of a chunk in a group
+    int rows, K, N, chunks, strips, groups, group_shift;      // group_shift: log2 of the halves of a chunk in a group
     int ws, wk, stage_chunks, stages;
     bool f32, vectors;
 };

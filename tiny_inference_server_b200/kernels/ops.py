@@ -718,7 +718,7 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
     lib = _lib or library()
     calls["gemm_w4"] += 1
     staged = n if dtype is torch.bfloat16 else 3 * n
-    tensor = _w4_tensor(staged, k, cols, w.group) if W4_TENSOR is None else W4_TENSOR
+    tensor = _w4_tensor(staged, k, cols, w.group) if W4_TENSOR is None else W4_TENSOR or staged > W4_MMA_ROWS
     copy = at = fault = 0
     if tensor:
         fault = tc_fault().data_ptr()
