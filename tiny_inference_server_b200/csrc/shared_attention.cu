@@ -820,8 +820,9 @@ struct SharedArgs {
 };
 TIS_API int tis_shared_attention(const SharedArgs* a) {
     if (a->rows <= 0) return TIS_OK;
+    // (a lane looks for keys up to 32 pages behind the last: their number is held in 32 bits)
     const long long most = 1ll << 30;
-    if (a->table_stride > most || a->table_width > most || a->num_pages > most || a->page > most || a->rows * a->H > most ||
+    if (a->table_stride > most || a->table_width > most || a->num_pages > most || a->page > (1 << 25) || a->rows * a->H > most ||
         a->own_count * a->own_parts * a->KVH > most || a->wide_count * a->shared_parts * a->KVH > most) {
         tis_set_error("shared_prefix_attention: %lld rows of %lld heads, %lld pages of %lld, tables of %lld", a->rows, a->H, a->num_pages, a->page, a->table_width);
         return TIS_BAD_SIZE;

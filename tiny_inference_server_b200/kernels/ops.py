@@ -1082,7 +1082,7 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     as they were.
 
     ``max_position`` (no row's position is larger; the tables' width unless given) decides only how the requests' own keys are split.
-    ``scale`` multiplies the scores (1 / sqrt(hd) unless given).  bfloat16 or float32 (all in 32 bits), any page size, hd a
+    ``scale`` multiplies the scores (1 / sqrt(hd) unless given).  bfloat16 or float32 (all in 32 bits), pages of up to 2^25 keys, hd a
     multiple of 16 up to 256.  A page that is not there sets ``fault``, as in ``paged_attention``."""
     dtype = q.dtype
     if plane.ndim != 5 or q.ndim != 2 or out.ndim != 2 or block_table.ndim != 2 or plane.dtype is not dtype or out.dtype is not dtype:
@@ -1090,9 +1090,9 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
                           f"{tuple(plane.shape)}: matrices, and a plane [pages, 2, kv heads, page, head size], of one type")
     pages, two, kvh, page, hd = plane.shape
     h, rows = plan.num_heads, plan.rows
-    if two != 2 or kvh != plan.kv_heads or pages < 1 or page < 1 or hd % 16 or not 16 <= hd <= 256 or not plane.is_contiguous():
-        raise KernelError(f"shared_prefix_attention: a plan for {plan.kv_heads} kv heads, a cache plane {tuple(plane.shape)} (contiguous; head "
-                          "sizes that are multiples of 16 up to 256)")
+    if two != 2 or kvh != plan.kv_heads or pages < 1 or not 1 <= page <= 1 << 25 or hd % 16 or not 16 <= hd <= 256 or not plane.is_contiguous():
+        raise KernelError(f"shared_prefix_attention: a plan for {plan.kv_heads} kv heads, a cache plane {tuple(plane.shape)} (contiguous; pages of up to "
+                          "2^25 keys, head sizes that are multiples of 16 up to 256)")
     n, width = q.shape
     ldq, unit = q.stride()
     n_out, width_out = out.shape
