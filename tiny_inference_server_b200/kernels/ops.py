@@ -2089,7 +2089,9 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
     ``uniforms[k]`` times the whole sum, over ``max(p_i - q_i, 0)`` at the first draft that is not kept (``p_i`` where
     nothing is left of the difference; without a distribution ``q_i`` is one at the draft) and over the target's row behind the last
     draft.  Entries that are not positive numbers have no mass; a row without mass gives the token -1.  A draft outside the
-    vocabulary is not kept.  Computed in 64 bits: the tokens do not depend on how the work is shared out."""
+    vocabulary is not kept.  Computed in 64 bits: the tokens do not depend on how the work is shared out.
+
+    Results lie apart from the arguments and from one another; ``accepted`` may be ``draft_lens`` itself."""
     f32, i32 = torch.float32, torch.int32
     if target_probs.dtype is not f32 or uniforms.dtype is not f32 or drafts.dtype is not i32 or target_probs.ndim != 3:
         raise KernelError(f"verify_drafts: float32 probabilities (n, k + 1, V) and numbers and int32 drafts are taken, not "
@@ -2119,13 +2121,19 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
     if not (drafts.is_contiguous() and uniforms.is_contiguous() and tokens.is_contiguous() and accepted.is_contiguous()):
         raise KernelError("verify_drafts: drafts, numbers and results are contiguous")
     drafts_at, uniforms_at, tokens_at = drafts.data_ptr(), uniforms.data_ptr(), tokens.data_ptr()
-    if n > 0 and (tokens_at == uniforms_at or tokens_at == drafts_at or tokens_at == accepted.data_ptr()):
-        raise KernelError("verify_drafts: the tokens do not lie where drafts, numbers or the numbers of kept drafts do")
-    lens = 0
+    lens, accepted_at = 0, accepted.data_ptr()
     if draft_lens is not None:
         if draft_lens.dtype is not i32 or draft_lens.shape != (n,) or not draft_lens.is_contiguous():
             raise KernelError(f"verify_drafts: numbers of drafts {draft_lens.dtype} {tuple(draft_lens.shape)}; contiguous int32 ({n},) is taken")
         lens = draft_lens.data_ptr()
+    # (a request's results are written while others' arguments are still read; all of these are contiguous, in entries of four bytes)
+    tokens_end, accepted_end, uniforms_end, drafts_end = tokens_at + 4 * n * k1, accepted_at + 4 * n, uniforms_at + 4 * n * k1, drafts_at + 4 * n * k
+    if (tokens_at < accepted_end and accepted_at < tokens_end
+            or tokens_at < uniforms_end and uniforms_at < tokens_end or tokens_at < drafts_end and drafts_at < tokens_end
+            or accepted_at < uniforms_end and uniforms_at < accepted_end or accepted_at < drafts_end and drafts_at < accepted_end
+            or lens and (tokens_at < lens + 4 * n and lens < tokens_end or accepted_at != lens and accepted_at < lens + 4 * n and lens < accepted_end)):
+        raise KernelError("verify_drafts: the tokens and the numbers of kept drafts do not lie where drafts, numbers, lengths or one another do (kept drafts "
+                          "may take the place of the lengths)")
     if (device < 0 or drafts.get_device() != device or uniforms.get_device() != device or tokens.get_device() != device
             or accepted.get_device() != device or _current_device() != device or (lens and draft_lens.get_device() != device)
             or (q and draft_probs.get_device() != device)):
@@ -2135,7 +2143,7 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
     lib = _lib or library()
     calls["verify_drafts"] += 1
     _check(lib.tis_verify_drafts(_VERIFY_ARGS.pack(target_probs.data_ptr(), p_request, p_row, q, q_request, q_row, drafts_at,
-                                                   uniforms_at, lens, tokens_at, accepted.data_ptr(), n, k, v,
+                                                   uniforms_at, lens, tokens_at, accepted_at, n, k, v,
                                                    _stream_number(device))), lib)
     return tokens, accepted
 
