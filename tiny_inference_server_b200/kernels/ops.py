@@ -686,6 +686,15 @@ def _w4_tensor(staged: int, k: int, n: int, group: int) -> bool:
     return staged > 16 or tiles <= 148 or group >= (64 if tiles > 296 else 128 if staged > 8 else math.inf)
 
 
+def _rows_meet(a: int, lda: int, wide_a: int, b: int, ldb: int, wide_b: int, rows: int, size: int) -> bool:
+    """Whether rows of two matrices lie on one another: never where one ends before the other begins; rows as far apart as one another's may lie
+    beside each other (columns of one buffer); others that reach into each other count as meeting."""
+    if rows == 0 or a + ((rows - 1) * lda + wide_a) * size <= b or b + ((rows - 1) * ldb + wide_b) * size <= a:
+        return False
+    beside = (b - a) // size % lda if lda else 0
+    return lda != ldb or beside < wide_a or beside + wide_b > lda
+
+
 def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a (n, K) @ w (K, N)`` for weights of four bits (``weights.w4.pack_w4``), a and the result in bfloat16 or float32; row strides
     free.  Every weight is taken as it is, (code - zero) * scale, and a sum is rounded once, when it is stored.  A group's sums are formed before their
@@ -708,7 +717,7 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
         if out.dtype is not dtype or out.shape != (n, cols):
             raise KernelError(f"gemm_w4: result {out.dtype} {tuple(out.shape)} for {n} rows of {dtype} and weights {w.k} x {cols}")
         ldo, unit = out.stride()
-        if (unit != 1 and cols > 1) or (ldo < cols and n > 1) or (out.data_ptr() == a.data_ptr() and n > 0):
+        if (unit != 1 and cols > 1) or (ldo < cols and n > 1) or _rows_meet(a.data_ptr(), lda, k, out.data_ptr(), ldo, cols, n, dtype.itemsize):
             raise KernelError("gemm_w4: a row of the result is contiguous, its rows do not lie on one another, and the result is not where the rows are")
     device = a.get_device()
     if device < 0 or out.get_device() != device or w.words.get_device() != device or _current_device() != device:
@@ -1098,7 +1107,8 @@ def shared_prefix_attention(q: torch.Tensor, out: torch.Tensor, plane: torch.Ten
     n_out, width_out = out.shape
     ldo, unit_out = out.stride()
     q_at, plane_at, out_at = q.data_ptr(), plane.data_ptr(), out.data_ptr()
-    if n < rows or n_out < rows or width < h * hd or width_out < h * hd or unit != 1 or unit_out != 1 or q_at == out_at or (ldo < h * hd and rows > 1):
+    if (n < rows or n_out < rows or width < h * hd or width_out < h * hd or unit != 1 or unit_out != 1 or (ldo < h * hd and rows > 1)
+            or _rows_meet(q_at, ldq, h * hd, out_at, ldo, h * hd, rows, dtype.itemsize)):
         raise KernelError(f"shared_prefix_attention: queries {tuple(q.shape)}, results {tuple(out.shape)} (rows contiguous, not on one another, and not the queries' own) for "
                           f"{rows} rows of {h} heads of {hd}")
     code = 1 if dtype is torch.bfloat16 else 0
