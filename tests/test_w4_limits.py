@@ -68,3 +68,15 @@ def test_float32_rows_up_to_the_largest(kernel):  # noqa: F811
         x[i, i] = v
     got = ops.gemm_w4(x, w)
     assert torch.equal(got, x.sum(1, keepdim=True).expand_as(got))
+
+
+@pytest.mark.gpu
+def test_packed_weights_are_there_when_they_are_returned():
+    """A product's kernel reads weights ahead of the wait for the kernel in front of it: none that packs may still run."""
+    codes = torch.full((4096, 65536), 3, dtype=torch.uint8, device="cuda")      # milliseconds of work
+    scales, z = torch.ones(128, 65536, device="cuda").bfloat16(), codes[:128].clone()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        pack_w4(codes, scales, z, 32)
+        assert s.query()

@@ -700,6 +700,9 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
     free.  Every weight is taken as it is, (code - zero) * scale, and a sum is rounded once, when it is stored.  A group's sums are formed before their
     scale: 15 times the sum of a group's ``|a|``, in float32 twice that, has to stay below 2^128.
 
+    Weights are read while the kernel in front of the call may still run, as those of all products of few rows are: packed ones are there when
+    ``pack_w4`` returns; after a kernel that writes to them (``copy_`` into ``w.scales``) synchronize before the next product.
+
     For few rows: the weights are streamed once for up to 64 rows of bfloat16 and 21 of float32, and again for as many more.  (A prompt's rows
     are better off with ``weights.w4.unpack_w4`` and ``gemm``.)  Two kernels, chosen by the sizes (``_w4_tensor``); float32 rows, and
     bfloat16 ones that do not start on 16 bytes, are copied for the second.  A wait that runs out inside the second sets ``tc_fault``."""

@@ -94,7 +94,8 @@ def _pairs(x: torch.Tensor) -> torch.Tensor:
 
 
 def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, group: int = 128) -> W4Weights:
-    """Lay codes (K, N) uint8 (0..15), scales (groups, N) bfloat16 and zero points (groups, N) uint8 (0..15; None: 8) out for ``gemm_w4``."""
+    """Lay codes (K, N) uint8 (0..15), scales (groups, N) bfloat16 and zero points (groups, N) uint8 (0..15; None: 8) out for ``gemm_w4``.  On the
+    device they are there when it returns."""
     if codes.dim() != 2 or codes.dtype != torch.uint8 or 0 in codes.shape:
         raise ValueError(f"codes (K, N) in uint8 are wanted, not {codes.dtype} {tuple(codes.shape)}")
     k, n = codes.shape
@@ -121,7 +122,10 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Ten
         x = x.permute(5, 0, 6, 8, 2, 1, 4, 3, 7).reshape(b - a, chunks, TILE_STRIPS, 32, 4, 4, 2)
         x = x[..., 0] | (x[..., 1] << 4)                      # bytes, the low nibble first
         words[a:b] = x.contiguous().view(torch.int32).squeeze(-1)
-    return W4Weights(words, _pairs(scales), None if zeros is None else _pairs(zeros), k, n, group)
+    w = W4Weights(words, _pairs(scales), None if zeros is None else _pairs(zeros), k, n, group)
+    if words.is_cuda:                                         # (products read weights without waiting for the kernel in front of them)
+        torch.cuda.current_stream(words.device).synchronize()
+    return w
 
 
 def unpack_w4(w: W4Weights, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
