@@ -3,6 +3,7 @@ head sizes and all pages that it takes, and more own tiles than CTAs.  Tolerance
 import pytest
 import torch
 
+import kernel_refs as ref
 from test_shared_attention import Batch
 from tiny_inference_server_b200.kernels import ops
 
@@ -154,3 +155,23 @@ def test_more_own_tiles_than_ctas(hd, own, dtype, monkeypatch):
     rest = [r for r in range(b.rows) if r not in gone]
     got = b.run()
     assert bool((got[gone] == 0).all()) and torch.equal(got[rest], whole[rest])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("shared,page", [(1040, 16), (1152, 64), (64, 64), (992, 32)])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf")])
+def test_an_infinity_in_the_last_shared_page(hd, shared, page, value, tensor, monkeypatch):
+    """A value that every row sees with a positive weight: infinite there, finite in all other columns, whatever lies behind the last shared key in its tile."""
+    split(monkeypatch, 1)
+    b = Batch([(shared, [(shared + 3, 1), (shared + 40, 2)])], 4, 2, hd, page)
+    whole = b.check()
+    takes_tensor(b)
+    slot = b.plan_groups[0][1][0][0]
+    key = shared - 1
+    row = b.plane[int(b.table[slot, key // page]), 1, 0, key % page]
+    column = int(ref.cache_row(torch.arange(hd).bfloat16(), key)[5])
+    row[5] = value
+    got = b.run().view(b.rows, 4, hd)
+    assert bool((got[:, :2, column] == value).all())
+    rest = [c for c in range(hd) if c != column]
+    assert torch.equal(got[:, :, rest], whole.view(b.rows, 4, hd)[:, :, rest]) and torch.equal(got[:, 2:], whole.view(b.rows, 4, hd)[:, 2:])

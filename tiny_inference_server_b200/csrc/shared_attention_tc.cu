@@ -108,11 +108,13 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const SharedParams 
             const int boxes = BN / p.page * HALVES;                             // of a key tile
             const bool mine = lane < boxes && (lane & 1) == half_of;            // a lane a box, the two warps taking turns
             const int part_bytes = (boxes + 1 - half_of) / 2 * p.page * 128, in_tile = lane / HALVES * p.page;
-            // the page of a lane's keys in tile j, on its way PAGES_AHEAD tiles before its copies are ordered.  Behind the part's end the
-            // last page once more: its keys are masked, and its values are finite if the rows' own results are.
+            // the page of a lane's keys in tile j, on its way PAGES_AHEAD tiles before its copies are ordered.  Behind the part's end (whole
+            // pages) a box begins behind the cache's last row, which brings zeros: a masked key's probability of 0 takes no other value away.
+            auto behind = [&](int j) { return keys.lo + j * BN + in_tile >= keys.hi; };
+            const int behind_all = p.num_pages * 2 * p.KVH * p.page;            // (below 2^31: the launcher)
             auto page_of = [&](int j) -> int {
-                if (j >= T || !mine) return 0;
-                const int index = min(keys.lo + j * BN + in_tile, keys.hi - 1) / p.page;
+                if (j >= T || !mine || behind(j)) return 0;
+                const int index = (keys.lo + j * BN + in_tile) / p.page;
                 return index < p.table_width ? p.table[(size_t)t.slot * p.table_stride + index] : -1;
             };
             int pages[PAGES_AHEAD];
@@ -131,7 +133,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const SharedParams 
                 if (mine) {
                     const int half = lane % HALVES;
                     tma_load_2d(ring + (size_t)s * SLOT_BYTES + half * HALF_BYTES + in_tile * 128, &map_kv, half * 64,
-                                ((page * 2 + kv) * p.KVH + kvh) * p.page, &full[s]);
+                                behind(j) ? behind_all : ((page * 2 + kv) * p.KVH + kvh) * p.page, &full[s]);
                 }
             }
         } else if (warp == 1) {
