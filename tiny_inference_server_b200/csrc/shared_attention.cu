@@ -129,6 +129,20 @@ __device__ __forceinline__ void join_row(const SharedParams& p, float m, float l
     }
 }
 
+// The loading warp's wait for a place that the other warps give back.  They may be waiting for the kernel of the shared tiles, which takes as long as it takes: only
+// behind it (`waited`) does a wait that runs out mean a fault.  (Apart: the loop over items stays short.)
+__device__ __noinline__ bool wait_given_back(unsigned long long* bar, unsigned parity, volatile int* abort, int* fault, bool& waited) {
+    if (!waited) {
+        for (int spin = 0; spin < tc::MBAR_SPINS; ++spin) {
+            if (tc::mbar_done(bar, parity)) return true;
+            if ((spin & 1023) == 1023 && *abort) return false;
+        }
+        pdl_wait();
+        waited = true;
+    }
+    return tc::mbar_wait(bar, parity, abort, fault, 6);
+}
+
 // What the loading warp tells the others of an item (a tile, a kv head and a part).
 struct Item { int rh0, count, kvh, part, lo, hi, least; bool all; };     // all: every row head sees keys (what rows behind them hold stays there)
 
@@ -166,13 +180,16 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
 
     if (warp == 4) {
         int stage = 0, n = 0;                               // tiles and items so far
-        bool ok = true;
+        bool ok = true, waited = !beside;                   // for the kernel before
+        auto wait_free = [&](unsigned long long* bar, unsigned parity) {
+            return tc::mbar_done(bar, parity) || wait_given_back(bar, parity, abort, p.fault, waited);
+        };
         for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++n) {
             const int kvh = item % p.KVH, part = item / p.KVH % parts, slot = n % SLOTS;
             const SharedTile t = tiles[item / p.KVH / parts];
             const int shared = shared_keys(p, t);
             // ---- queries, a copy a row's heads.  (Copies, pages and positions all go out as soon as the tile is known: one round of loads, not three.) ----
-            ok = __all_sync(ALL, tc::mbar_wait(&q_empty[slot], ((n / SLOTS) & 1) ^ 1, abort, p.fault, 6));
+            ok = __all_sync(ALL, wait_free(&q_empty[slot], ((n / SLOTS) & 1) ^ 1));
             if (!ok) break;
             for (int row = t.rh0 / G + lane; row * G < t.rh0 + t.count; row += 32) {
                 const int a = max(t.rh0, row * G), b = min(t.rh0 + t.count, (row + 1) * G);
@@ -216,7 +233,7 @@ shared_mma_kernel(const SharedParams p, const SharedTile* tiles, int items, int 
             // ---- keys and values of tile j: its rows in [lo, hi) ----
             for (int j = 0; j < count; ++j, ++stage) {
                 const int next = page_of(j + 1), s = stage % STAGES;
-                ok = __all_sync(ALL, tc::mbar_wait(&empty[s], ((stage / STAGES) & 1) ^ 1, abort, p.fault, 6));
+                ok = __all_sync(ALL, wait_free(&empty[s], ((stage / STAGES) & 1) ^ 1));
                 if (!ok) break;
                 const int from = max(kt0 + j * KT, keys.lo), to = min(kt0 + (j + 1) * KT, keys.hi);
                 bf16* k = ring + (size_t)s * 2 * TILE_ELEMENTS;

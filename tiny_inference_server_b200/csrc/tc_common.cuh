@@ -41,8 +41,11 @@ __device__ __forceinline__ bool mbar_done(unsigned long long* bar, unsigned pari
 // Bounded wait for the phase with this parity.  Returns false when it ran out (the fault word
 // is set to `code`) or when another role gave up before (`abort`); the caller then leaves its loop.
 // The first look is apart from the loop: a look takes 40 cycles, as a turn of the loop
-// 150 to 220, for a phase that was complete already, in every hand-over of every role.
-constexpr int MBAR_SPINS = 1 << 20;
+// 150 to 220, for a phase that was complete already, in every hand-over of every role.  (A look at one that is not complete waits 1.5 us: 1.6 s in all.)
+#ifndef TIS_MBAR_SPINS
+#define TIS_MBAR_SPINS (1 << 20)
+#endif
+constexpr int MBAR_SPINS = TIS_MBAR_SPINS;
 __device__ __forceinline__ bool mbar_wait_on(unsigned long long* bar, unsigned parity, volatile int* abort, int* fault, int code) {
     for (int spin = 0; spin < MBAR_SPINS; ++spin) {
         if (mbar_done(bar, parity)) return true;
