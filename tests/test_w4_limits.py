@@ -6,7 +6,7 @@ import torch
 
 from test_w4 import dense, kernel, make  # noqa: F401
 from tiny_inference_server_b200.kernels import ops
-from tiny_inference_server_b200.weights.w4 import pack_w4
+from tiny_inference_server_b200.weights.w4 import pack_w4, quantize_w4
 
 
 def behind(x, offset):
@@ -27,6 +27,26 @@ def test_packed_weights_off_their_places():
                 dataclasses.replace(w, **{name: behind(getattr(w, name), offset)})
         for offset in good:
             assert torch.equal(getattr(dataclasses.replace(w, **{name: behind(getattr(w, name), offset)}), name), getattr(w, name))
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_weights_that_have_no_scale(zeros):
+    """One NaN or infinity took its group's other weights with it."""
+    for value in (float("nan"), float("inf"), -float("inf")):
+        w = torch.randn(70, 5, generator=torch.Generator().manual_seed(0))
+        w[66, 2] = value
+        with pytest.raises(ValueError, match="not finite"):
+            quantize_w4(w, 32, zeros)
+    with pytest.raises(ValueError, match="not finite"):
+        quantize_w4(torch.full((4, 4), 1e300, dtype=torch.float64), 32, zeros)
+    # the largest numbers of both signs: a range of twice the largest, in steps that are finite
+    most = torch.finfo(torch.float32).max
+    w = torch.tensor([[most], [-most], [0.0], [most / 2]])
+    codes, scales, z = quantize_w4(w, 32, zeros)
+    assert bool(torch.isfinite(scales.float()).all())
+    at = codes.double() - (z.double() if zeros else 8.0)
+    # half a step, one more half for the zero point, and the scale's rounding (2^-8) over up to 15 steps
+    assert bool(((at * scales.double() - w.double()).abs() <= scales.double() * (1.0 + 15 * 2.0 ** -8)).all())
 
 
 @pytest.mark.gpu

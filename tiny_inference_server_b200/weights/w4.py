@@ -71,10 +71,13 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False):
     groups = _groups(k, group)
     x = torch.zeros((groups * group, n), dtype=torch.float32, device=w.device)
     x[:k] = w
+    if not bool(torch.isfinite(x).all()):                     # (no scale: the whole group would be lost)
+        raise ValueError("weights that are not finite in float32")
     x = x.reshape(groups, group, n)
     if zeros:
         low, high = x.amin(1).clamp(max=0.0), x.amax(1).clamp(min=0.0)
-        scales = ((high - low) / 15.0).to(torch.bfloat16)
+        span = high - low                                     # (of the largest numbers of both signs: beyond float32)
+        scales = torch.where(torch.isfinite(span), span / 15.0, high / 15.0 - low / 15.0).to(torch.bfloat16)
     else:
         scales = (x.abs().amax(1) / 7.0).to(torch.bfloat16)
     scales = torch.where(scales > 0, scales, 1.0).to(torch.bfloat16)        # (a group of zeros)
