@@ -1062,7 +1062,9 @@ def shared_attention_library(head_dim: int):
 #: row heads of a group from which its shared keys go to the tcgen05 kernel whatever their number, and the number from which they do with more than 16
 #: row heads.  us a call, mma.sync / tcgen05, 32 heads on 8 of 128, requests of one row with 64 keys of their own, behind 512, 2048, 8192 shared
 #: ones: 2 requests (8 row heads) 9.6 / 13.2, 11.7 / 17.3, 20.0 / 21.8; 16 (64) 11.0 / 14.0, 17.8 / 21.6, 32.5 / 26.6; 64 (256) 27.6 / 24.7,
-#: 52.2 / 28.6, 105.6 / 36.0; 12 heads on 3, 16 requests behind 2048 and 4096 14.9 / 16.0, 18.9 / 16.7
+#: 52.2 / 28.6, 105.6 / 36.0; 12 heads on 3, 16 requests behind 2048 and 4096 14.9 / 16.0, 18.9 / 16.7.  Heads of 64 cross at the same places, pages of 64 and
+#: 128 too: 8 requests (32 row heads) behind 2048, 4096, 8192 12.3 / 16.0, 16.0 / 17.1, 20.7 / 19.4; 16 13.1 / 16.3, 18.1 / 17.2, 22.2 / 19.7; 32 (128) behind 512
+#: 15.3 / 13.5; 12 heads on 3, 16 requests behind 2048 12.0 / 11.8
 SHARED_TC_HEADS, SHARED_TC_KEYS = 64, 2500
 
 
