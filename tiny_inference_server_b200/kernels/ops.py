@@ -689,7 +689,8 @@ def _w4_tensor(staged: int, k: int, n: int, group: int) -> bool:
 def _rows_meet(a: int, lda: int, wide_a: int, b: int, ldb: int, wide_b: int, rows: int, size: int) -> bool:
     """Whether rows of two matrices lie on one another: never where one ends before the other begins; rows as far apart as one another's may lie
     beside each other (columns of one buffer); others that reach into each other count as meeting."""
-    if rows == 0 or a + ((rows - 1) * lda + wide_a) * size <= b or b + ((rows - 1) * ldb + wide_b) * size <= a:
+    last = rows - 1
+    if a + (last * lda + wide_a) * size <= b or b + (last * ldb + wide_b) * size <= a or last < 0:
         return False
     beside = (b - a) // size % lda if lda else 0
     return lda != ldb or beside < wide_a or beside + wide_b > lda
@@ -713,18 +714,20 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
     lda, unit = a.stride()
     if k != w.k or (unit != 1 and k > 1):
         raise KernelError(f"gemm_w4: rows {tuple(a.shape)}, strides {a.stride()}, for weights {w.k} x {w.n}")
-    cols = w.n
+    cols, words, a_at = w.n, w.words, a.data_ptr()
     if out is None:
         out, ldo = torch.empty((n, cols), dtype=dtype, device=a.device), cols
+        out_at = out.data_ptr()
     else:
         if out.dtype is not dtype or out.shape != (n, cols):
             raise KernelError(f"gemm_w4: result {out.dtype} {tuple(out.shape)} for {n} rows of {dtype} and weights {w.k} x {cols}")
         ldo, unit = out.stride()
-        if (unit != 1 and cols > 1) or (ldo < cols and n > 1) or _rows_meet(a.data_ptr(), lda, k, out.data_ptr(), ldo, cols, n, dtype.itemsize):
+        out_at = out.data_ptr()
+        if (unit != 1 and cols > 1) or (ldo < cols and n > 1) or _rows_meet(a_at, lda, k, out_at, ldo, cols, n, 2 if dtype is torch.bfloat16 else 4):
             raise KernelError("gemm_w4: a row of the result is contiguous, its rows do not lie on one another, and the result is not where the rows are")
     device = a.get_device()
-    if device < 0 or out.get_device() != device or w.words.get_device() != device or _current_device() != device:
-        _elsewhere("gemm_w4", a, out, w.words)
+    if device < 0 or out.get_device() != device or words.get_device() != device or _current_device() != device:
+        _elsewhere("gemm_w4", a, out, words)
     if n == 0:
         return out
     lib = _lib or library()
@@ -734,11 +737,11 @@ def gemm_w4(a: torch.Tensor, w: "W4Weights", out: Optional[torch.Tensor] = None)
     copy = at = fault = 0
     if tensor:
         fault = tc_fault().data_ptr()
-        if dtype is not torch.bfloat16 or k % 8 or lda % 8 or lda < k or a.data_ptr() % 16:
+        if dtype is not torch.bfloat16 or k % 8 or lda % 8 or lda < k or a_at % 16:
             copy = torch.empty((staged, -(-k // 8) * 8), dtype=torch.bfloat16, device=a.device)
             at = copy.data_ptr()
-    _check(lib.tis_gemm_w4(_W4_ARGS.pack(1 if dtype is torch.bfloat16 else 0, a.data_ptr(), lda, w.words.data_ptr(), w.scales.data_ptr(),
-                                         0 if w.zeros is None else w.zeros.data_ptr(), out.data_ptr(), ldo, n, k, cols, w.group,
+    _check(lib.tis_gemm_w4(_W4_ARGS.pack(1 if dtype is torch.bfloat16 else 0, a_at, lda, words.data_ptr(), w.scales.data_ptr(),
+                                         0 if w.zeros is None else w.zeros.data_ptr(), out_at, ldo, n, k, cols, w.group,
                                          tensor, at, fault, _stream_number(device))), lib)
     return out
 
